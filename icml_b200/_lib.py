@@ -30,6 +30,13 @@ class Epilogue(ctypes.Structure):
     ]
 
 
+class Strides(ctypes.Structure):
+    """pgf_strides of include/pgf.h."""
+    _fields_ = [("batch", c_int64), ("token", c_int64), ("head", c_int64)]
+
+
+_S = ctypes.POINTER(Strides)
+
 # name -> (restype, argtypes); mirrors include/pgf.h
 SIGNATURES = {
     "pgf_last_error": (c_char_p, []),
@@ -119,6 +126,18 @@ SIGNATURES = {
                                    [I64] * 7 + [c_int, P, c_size_t, P]),
     "pgf_ssm_compose_ranks_fwd": (c_int, [P, I64, c_int, c_int, P, c_int, P, I64, I64, I64, P]),
     "pgf_ssm_compose_ranks_bwd": (c_int, [P, I64, c_int, c_int, P, c_int, P, P, I64, I64, I64, P]),
+    "pgf_qk_norm_rotate_fwd": (c_int, [P, _S, P, _S, P, P, P, P, I64, P, P] + [I64] * 6 + [c_int, c_float, c_int, P]),
+    "pgf_qk_norm_rotate_bwd_workspace": (c_size_t, [I64]),
+    "pgf_qk_norm_rotate_bwd": (c_int, [P, _S, P, _S, P, P, P, P, P, P, I64, P, P, P, P, c_int] + [I64] * 6 +
+                               [c_int, c_float, c_int, P, c_size_t, P]),
+    "pgf_decay_attn_workspace": (c_size_t, [I64] * 8 + [c_int, c_int]),
+    "pgf_decay_attn_fwd": (c_int, [P, _S, P, _S, P, _S, P, P, P, P, P] + [I64] * 8 +
+                           [c_float, c_int, P, c_size_t, P]),
+    "pgf_decay_attn_bwd": (c_int, [P, _S, P, _S, P, _S, P, P, P, P, _S, P, P, P, P, P, P, c_int] + [I64] * 8 +
+                           [c_float, c_int, P, c_size_t, P]),
+    "pgf_decay_attn_step": (c_int, [P, _S, P, _S, P, _S, P, P, P, I64, P, P] + [I64] * 7 + [c_float, c_int, P]),
+    "pgf_beam_select": (c_int, [P] * 7 + [I64] * 4 + [c_int, P]),
+    "pgf_beam_reorder": (c_int, [P, P, P, c_int, P, I64, I64, P]),
 }
 
 

@@ -1,0 +1,377 @@
+// One step of a beam search: selection over beams and vocabulary, and the reordering of the beams'
+// recurrent states.
+//
+//   c[k, v] = score[k] + (logit[k, v] - lse[k]),   lse[k] = log sum_v exp(logit[k, v])
+//
+// and the K candidates of K x V that come first in the order (c descending, flat index k V + v
+// ascending).  c is formed in float32 with those two roundings, and the order is total, so the
+// selection is the same on every run.  A beam that has finished has one candidate: the end token at its
+// own score.  A NaN (a NaN or +inf logit, a row of -inf) counts as -inf: such candidates come last, in
+// index order.
+//
+// Bound by latency and, for large batches, by reading the logits.  One cluster of eight CTAs takes one
+// sequence, so that the whole step is one launch: the K rows (cut into parts where K < 8) go to the CTAs;
+// pass 1 takes the running maximum and sum of exponentials of each part and the largest logit of each
+// group of lanes; the parts' statistics meet through distributed shared memory; pass 2 (its reads hit L2)
+// forms c and keeps what is not below c at the K-th largest group maximum, a bound that at least K
+// candidates reach: a short list, ranked by counting.  The parts' best K keys meet the same way in one
+// CTA, which ranks them and writes the step's outputs.  A key is the order-preserving image of c above
+// the complement of the flat index, so one 64-bit comparison is the whole order.  A list that does not
+// fit (rows of equal logits) falls back to K passes of a plain maximum.
+#include "common.cuh"
+
+#include <cooperative_groups.h>
+
+namespace pgf {
+namespace beam {
+
+namespace cg = cooperative_groups;
+
+constexpr int CS = 8;              // CTAs of a cluster: one sequence
+constexpr int THREADS = 512;
+constexpr int MAX_K = 32;
+constexpr int UNITS = MAX_K / CS;  // (row, part) units of one CTA at most
+constexpr int LIST = 1024;
+
+struct Args {
+  const void* logits;        // (B, K, V)
+  const float* scores;       // (B, K)
+  const uint8_t* finished;   // (B, K) or NULL
+  float* out_scores;         // (B, K)
+  int64_t* out_rows;         // (B, K): flat row b K + k of the beam that goes on
+  int64_t* out_tokens;       // (B, K)
+  uint8_t* out_finished;     // (B, K)
+  int K, V, end, parts;
+};
+
+__device__ __forceinline__ float candidate(float x, float lse, float score) {
+  const float c = __fadd_rn(score, __fsub_rn(x, lse));
+  return c == c ? c : -INFINITY;
+}
+__device__ __forceinline__ uint64_t key_of(float c, uint32_t flat) {
+  const uint32_t u = __float_as_uint(c + 0.f);  // -0 as +0: they are equal
+  return uint64_t(u & 0x80000000u ? ~u : u | 0x80000000u) << 32 | (0xFFFFFFFFu - flat);
+}
+__device__ __forceinline__ float score_of(uint64_t key) {
+  const uint32_t u = uint32_t(key >> 32);
+  return __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u);
+}
+
+__device__ __forceinline__ void each16(const float* p, float (&f)[4]) {
+  const float4 t = __ldg(reinterpret_cast<const float4*>(p));
+  f[0] = t.x; f[1] = t.y; f[2] = t.z; f[3] = t.w;
+}
+__device__ __forceinline__ void each16(const __nv_bfloat16* p, float (&f)[8]) {
+  const uint4 t = __ldg(reinterpret_cast<const uint4*>(p));
+  const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    f[2 * k] = __uint_as_float(w[k] << 16);
+    f[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
+  }
+}
+
+// body(v, n, at): n consecutive elements from column `at`, for this thread's share of [lo, hi): 16-byte
+// loads where the address allows, single elements in front of and behind them (a row of an odd
+// vocabulary starts anywhere).
+template <class T, class Body>
+__device__ __forceinline__ void scan_row(const T* row, int lo, int hi, Body body) {
+  constexpr int W = 16 / int(sizeof(T));
+  const int mis = int((reinterpret_cast<uintptr_t>(row + lo) & 15) / sizeof(T));
+  const int a0 = min(hi, mis ? lo + W - mis : lo);
+  const int nv = (hi - a0) / W;
+  float f[W];
+  if (lo + int(threadIdx.x) < a0) {
+    f[0] = ld(row, lo + threadIdx.x);
+    body(f, 1, lo + int(threadIdx.x));
+  }
+#pragma unroll 4
+  for (int i = threadIdx.x; i < nv; i += THREADS) {
+    each16(row + a0 + i * W, f);
+    body(f, W, a0 + i * W);
+  }
+  const int tail = a0 + nv * W + int(threadIdx.x);
+  if (tail < hi) {
+    f[0] = ld(row, tail);
+    body(f, 1, tail);
+  }
+}
+
+template <class T>
+__global__ void __cluster_dims__(CS, 1, 1) __launch_bounds__(THREADS) select_kernel(const Args a) {
+  constexpr int WARPS = THREADS / 32;
+  __shared__ float s_max[UNITS], s_sum[UNITS];       // a unit's maximum and sum, read by the cluster
+  __shared__ float s_tau[UNITS];                     // the logit that at least K of the unit reach
+  __shared__ uint64_t s_best[UNITS][MAX_K];          // a unit's first K keys, read by the cluster
+  __shared__ uint64_t s_list[LIST];
+  __shared__ float s_wm[WARPS], s_ws[WARPS], s_g[2 * WARPS];
+  __shared__ int s_n;
+  __shared__ uint64_t s_wk[WARPS];
+  cg::cluster_group cl = cg::this_cluster();
+  const int rank = int(cl.block_rank());
+  const int64_t b = blockIdx.x / CS;
+  const int K = a.K, V = a.V, P = a.parts, U = K * P;
+  const int len = (V + P - 1) / P;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  constexpr float L2E = 1.4426950408889634f;
+
+  // a unit without candidates of its own scan: its row has finished, or cannot go on at all
+  auto fixed = [&](int k) { return (a.finished && a.finished[b * K + k]) || a.scores[b * K + k] == -INFINITY; };
+
+  // ---- pass 1: maximum, sum of exponentials, group maxima
+  for (int u = rank, n = 0; u < U; u += CS, ++n) {
+    const int k = u / P, lo = min(V, (u % P) * len), hi = min(V, lo + len);
+    float m = -INFINITY, s = 0.f;
+    if (!fixed(k)) {
+      scan_row(static_cast<const T*>(a.logits) + (b * K + k) * V, lo, hi, [&](const float* f, int cnt, int) {
+        float mm = m;
+        for (int e = 0; e < cnt; ++e) mm = fmaxf(mm, f[e]);
+        if (mm > m) {
+          s *= exp2f((m - mm) * L2E);
+          m = mm;
+        }
+        if (m != -INFINITY)
+          for (int e = 0; e < cnt; ++e) s += exp2f((f[e] - m) * L2E);
+      });
+    }
+    // the K-th largest of the maxima of 16 warps (K <= 16) or 32 half warps: that many candidates reach it
+    float gm = m;
+    for (int o = 8; o > 0; o >>= 1) gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, o));
+    if (K <= WARPS) gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, 16));
+    const int groups = K <= WARPS ? WARPS : 2 * WARPS;
+    if (K <= WARPS ? lane == 0 : (lane & 15) == 0) s_g[K <= WARPS ? warp : threadIdx.x >> 4] = gm;
+    const float wm = warp_max(m);
+    s = wm == -INFINITY ? s : s * exp2f((m - wm) * L2E);
+    s = warp_sum(s);
+    if (lane == 0) { s_wm[warp] = wm; s_ws[warp] = s; }
+    __syncthreads();
+    if (threadIdx.x < groups) {
+      const float mine = s_g[threadIdx.x];
+      int before = 0;
+      for (int g = 0; g < groups; ++g) before += s_g[g] > mine || (s_g[g] == mine && g < int(threadIdx.x));
+      if (before == K - 1) s_tau[n] = mine;
+    }
+    if (threadIdx.x == 0) {
+      float tm = -INFINITY, ts = 0.f;
+      for (int w = 0; w < WARPS; ++w) tm = fmaxf(tm, s_wm[w]);
+      for (int w = 0; w < WARPS; ++w) ts += s_wm[w] == -INFINITY ? s_ws[w] : s_ws[w] * exp2f((s_wm[w] - tm) * L2E);
+      s_max[n] = tm;
+      s_sum[n] = ts;
+    }
+    __syncthreads();
+  }
+  cl.sync();
+
+  // ---- pass 2: the unit's first K keys
+  for (int u = rank, n = 0; u < U; u += CS, ++n) {
+    const int k = u / P, lo = min(V, (u % P) * len), hi = min(V, lo + len);
+    const float score = a.scores[b * K + k];
+    const uint32_t flat0 = uint32_t(k) * uint32_t(V);
+    if (threadIdx.x < MAX_K) s_best[n][threadIdx.x] = 0;  // below every key
+    if (threadIdx.x == 0) s_n = 0;
+    __syncthreads();
+    if (fixed(k)) {
+      // the end token at the score (if it has finished), then -inf from the lowest index
+      const bool done = a.finished && a.finished[b * K + k] && score > -INFINITY;
+      const int j = threadIdx.x;
+      if (u % P == 0 && j < K) {
+        if (done && j == 0) {
+          s_best[n][0] = key_of(score, flat0 + a.end);
+        } else {
+          int v = done ? j - 1 : j;
+          if (done && v >= a.end) ++v;
+          if (v < V) s_best[n][j] = key_of(-INFINITY, flat0 + v);
+        }
+      }
+      __syncthreads();
+      continue;
+    }
+    float m = -INFINITY, s = 0.f;
+    for (int p = 0; p < P; ++p) {
+      const int v = k * P + p;
+      m = fmaxf(m, cl.map_shared_rank(s_max, v % CS)[v / CS]);
+    }
+    for (int p = 0; p < P; ++p) {
+      const int v = k * P + p;
+      const float pm = cl.map_shared_rank(s_max, v % CS)[v / CS], ps = cl.map_shared_rank(s_sum, v % CS)[v / CS];
+      s += pm == -INFINITY ? ps : ps * exp2f((pm - m) * L2E);
+    }
+    const float lse = m + logf(s);
+    const float bound = candidate(s_tau[n], lse, score);
+    const T* row = static_cast<const T*>(a.logits) + (b * K + k) * V;
+    scan_row(row, lo, hi, [&](const float* f, int cnt, int at) {
+      for (int e = 0; e < cnt; ++e) {
+        const float c = candidate(f[e], lse, score);
+        if (c >= bound) {
+          const int i = atomicAdd(&s_n, 1);
+          if (i < LIST) s_list[i] = key_of(c, flat0 + at + e);
+        }
+      }
+    });
+    __syncthreads();
+    const int cnt = s_n;
+    if (cnt <= LIST) {
+      for (int i = threadIdx.x; i < cnt; i += THREADS) {
+        const uint64_t mine = s_list[i];
+        int before = 0;
+        for (int j = 0; j < cnt; ++j) before += s_list[j] > mine;
+        if (before < K) s_best[n][before] = mine;
+      }
+    } else {
+      uint64_t last = ~uint64_t(0);
+      for (int j = 0; j < K; ++j) {
+        uint64_t top = 0;
+        scan_row(row, lo, hi, [&](const float* f, int c, int at) {
+          for (int e = 0; e < c; ++e) {
+            const uint64_t key = key_of(candidate(f[e], lse, score), flat0 + at + e);
+            if (key < last && key > top) top = key;
+          }
+        });
+        for (int o = 16; o > 0; o >>= 1) {
+          const uint64_t other = __shfl_xor_sync(0xffffffffu, top, o);
+          top = other > top ? other : top;
+        }
+        if (lane == 0) s_wk[warp] = top;
+        __syncthreads();
+        for (int w = 0; w < WARPS; ++w) top = s_wk[w] > top ? s_wk[w] : top;
+        last = top;
+        if (threadIdx.x == 0) s_best[n][j] = top;
+        __syncthreads();
+      }
+    }
+    __syncthreads();
+  }
+  cl.sync();
+
+  // ---- the sequence's K: all units' keys ranked by counting
+  if (rank == 0) {
+    static_assert(MAX_K * MAX_K <= LIST && CS * CS <= LIST, "the units' keys fit the list");
+    for (int i = threadIdx.x; i < U * K; i += THREADS) {
+      const int u = i / K;
+      s_list[i] = cl.map_shared_rank(&s_best[0][0], u % CS)[(u / CS) * MAX_K + i % K];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < U * K; i += THREADS) {
+      const uint64_t mine = s_list[i];
+      if (mine == 0) continue;
+      int before = 0;
+      for (int j = 0; j < U * K; ++j) before += s_list[j] > mine;
+      if (before >= K) continue;
+      const uint32_t flat = 0xFFFFFFFFu - uint32_t(mine);
+      const int k = int(flat / uint32_t(V)), v = int(flat % uint32_t(V));
+      const int64_t o = b * K + before;
+      a.out_scores[o] = score_of(mine);
+      a.out_rows[o] = b * K + k;
+      a.out_tokens[o] = v;
+      if (a.out_finished) a.out_finished[o] = (a.finished && a.finished[b * K + k]) || v == a.end;
+    }
+  }
+  cl.sync();  // the others' shared memory stays until it has been read
+}
+
+constexpr int MAX_T = 64;           // tensors of one reorder launch
+constexpr int PIECE = 16384;        // bytes of a row that one CTA copies
+
+struct Table {
+  const uint8_t* src[MAX_T];
+  uint8_t* dst[MAX_T];
+  int64_t bytes[MAX_T];             // of one row
+  int64_t first[MAX_T + 1];         // first CTA of the tensor
+  int count;
+};
+
+template <class W>
+__device__ __forceinline__ void copy_piece(uint8_t* d, const uint8_t* s, int64_t n) {
+  const int m = int(n / int64_t(sizeof(W)));
+#pragma unroll 4
+  for (int i = threadIdx.x; i < m; i += 256) {
+    W w = {};
+    if (s) w = __ldg(reinterpret_cast<const W*>(s) + i);
+    reinterpret_cast<W*>(d)[i] = w;
+  }
+}
+
+// dst[i] = src[rows[i]] of every tensor; a row out of range gives zeros (the call does not
+// synchronise to report it).
+__global__ void __launch_bounds__(256) reorder_kernel(const __grid_constant__ Table t, const int64_t* __restrict__ rows,
+                                                      int64_t n_src) {
+  int z = 0;
+  while (z + 1 < t.count && int64_t(blockIdx.x) >= t.first[z + 1]) ++z;
+  const int64_t bytes = t.bytes[z];
+  const int64_t pieces = (bytes + PIECE - 1) / PIECE, i = int64_t(blockIdx.x) - t.first[z];
+  const int64_t row = i / pieces, off = (i % pieces) * PIECE;
+  const int64_t n = min(int64_t(PIECE), bytes - off), from = rows[row];
+  const uint8_t* s = from >= 0 && from < n_src ? t.src[z] + from * bytes + off : nullptr;
+  uint8_t* d = t.dst[z] + row * bytes + off;
+  const uintptr_t al = reinterpret_cast<uintptr_t>(t.src[z]) | reinterpret_cast<uintptr_t>(t.dst[z]) | uintptr_t(bytes);
+  if (al % 16 == 0) copy_piece<uint4>(d, s, n);
+  else if (al % 4 == 0) copy_piece<uint32_t>(d, s, n);
+  else copy_piece<uint8_t>(d, s, n);
+}
+
+}  // namespace beam
+}  // namespace pgf
+
+using namespace pgf;
+
+extern "C" int pgf_beam_select(const void* logits, const float* scores, const uint8_t* finished, float* out_scores,
+                               int64_t* out_rows, int64_t* out_tokens, uint8_t* out_finished, int64_t Bsz, int64_t K,
+                               int64_t V, int64_t end_id, int dtype, pgf_stream_t stream) {
+  clear_error();
+  PGF_CHECK_ARG(Bsz >= 0 && Bsz < (int64_t(1) << 27) && K >= 1 && K <= beam::MAX_K && V >= 1 &&
+                    K * V < (int64_t(1) << 31),
+                "beam_select: bad shape B=%lld K=%lld (1 to %d) V=%lld", (long long)Bsz, (long long)K, beam::MAX_K,
+                (long long)V);
+  PGF_CHECK_ARG(end_id >= -1 && end_id < V, "beam_select: end token %lld of %lld", (long long)end_id, (long long)V);
+  PGF_CHECK_ARG(!finished || end_id >= 0, "beam_select: finished beams need an end token");
+  PGF_CHECK_ARG(dtype == PGF_DTYPE_F32 || dtype == PGF_DTYPE_BF16, "beam_select: dtype %d", dtype);
+  if (Bsz == 0) return PGF_OK;
+  PGF_CHECK_ARG(logits && scores && out_scores && out_rows && out_tokens, "beam_select: null pointer");
+  PGF_CHECK_ARG(aligned(logits, dtype == PGF_DTYPE_BF16 ? 2 : 4), "beam_select: misaligned logits");
+  beam::Args a = {logits, scores, finished, out_scores, out_rows, out_tokens, out_finished,
+                  int(K), int(V), int(end_id), K < beam::CS ? int(beam::CS / K) : 1};
+  const unsigned grid = unsigned(Bsz * beam::CS);
+  if (dtype == PGF_DTYPE_BF16)
+    beam::select_kernel<__nv_bfloat16><<<grid, beam::THREADS, 0, as_stream(stream)>>>(a);
+  else
+    beam::select_kernel<float><<<grid, beam::THREADS, 0, as_stream(stream)>>>(a);
+  PGF_LAUNCH_CHECK();
+  return PGF_OK;
+}
+
+extern "C" int pgf_beam_reorder(const void* const* src, void* const* dst, const int64_t* row_bytes, int count,
+                                const int64_t* rows, int64_t n_rows, int64_t n_src, pgf_stream_t stream) {
+  clear_error();
+  PGF_CHECK_ARG(count >= 0 && n_rows >= 0 && n_src >= 0, "beam_reorder: bad shape");
+  if (count == 0 || n_rows == 0) return PGF_OK;
+  PGF_CHECK_ARG(src && dst && row_bytes && rows, "beam_reorder: null pointer");
+  for (int i = 0; i < count; ++i) {
+    PGF_CHECK_ARG(row_bytes[i] >= 0, "beam_reorder: row of %lld bytes", (long long)row_bytes[i]);
+    if (row_bytes[i] == 0) continue;
+    PGF_CHECK_ARG(dst[i] && (src[i] || n_src == 0), "beam_reorder: null pointer");
+    const char *s0 = static_cast<const char*>(src[i]), *s1 = s0 + n_src * row_bytes[i];
+    const char *d0 = static_cast<const char*>(dst[i]), *d1 = d0 + n_rows * row_bytes[i];
+    PGF_CHECK_ARG(d1 <= s0 || s1 <= d0, "beam_reorder: tensor %d would overwrite rows that it reads", i);
+  }
+  for (int i = 0; i < count;) {
+    beam::Table t;
+    t.count = 0;
+    int64_t ctas = 0;
+    for (; i < count && t.count < beam::MAX_T; ++i) {
+      if (row_bytes[i] == 0) continue;
+      const int64_t need = n_rows * ((row_bytes[i] + beam::PIECE - 1) / beam::PIECE);
+      PGF_CHECK_ARG(need < 0x7fffffff, "beam_reorder: tensor %d is too large", i);
+      if (ctas + need >= 0x7fffffff) break;
+      t.src[t.count] = static_cast<const uint8_t*>(src[i]);
+      t.dst[t.count] = static_cast<uint8_t*>(dst[i]);
+      t.bytes[t.count] = row_bytes[i];
+      t.first[t.count++] = ctas;
+      ctas += need;
+    }
+    if (!ctas) continue;
+    t.first[t.count] = ctas;
+    beam::reorder_kernel<<<unsigned(ctas), 256, 0, as_stream(stream)>>>(t, rows, n_src);
+    PGF_LAUNCH_CHECK();
+  }
+  return PGF_OK;
+}

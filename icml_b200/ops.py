@@ -7,11 +7,13 @@ parameter gradients are float32.  Nothing here runs on the CPU: a CPU tensor is 
 """
 from __future__ import annotations
 
+import ctypes
+import math
 from typing import Dict, Optional, Tuple
 
 import torch
 
-from ._lib import Epilogue, check, lib
+from ._lib import Epilogue, Strides, check, lib
 
 F32, BF16 = 0, 1
 ACT = {None: 0, "none": 0, "gelu": 1, "relu": 2, "tanh": 3}
@@ -829,3 +831,270 @@ def mamba_mixer_bwd_finish(state, dh_end=None, dA_end=None, want_g_halo=False):
                                            *[_p(grads[k]) for k in MIXER_KEYS], _p(gx), _p(gh), 0, Bsz, L_, d, E, R,
                                            N, K, _dt(x), _p(ws), ws.numel(), _stream()), "mamba_mixer_bwd_finish")
     return grads, gx, gh
+
+
+# --------------------------------------------------------------------------- decay-attention layer
+PAIRS = {"halves": 0, "neighbours": 1}
+
+
+def rotary_turns(dim: int, base: float = 10000.0, device="cuda") -> torch.Tensor:
+    """The rotation's table for `dim` rotated elements: frequency base^(-2i/dim) radians per position
+    of pair i as a 64-bit fixed-point fraction of a turn (int64, dim/2).  Build it once."""
+    if dim < 0 or dim % 2:
+        raise ValueError(f"rotary_turns: rotated width {dim} must be even")
+    f = float(base) ** (-torch.arange(0, dim, 2, dtype=torch.float64) / max(dim, 1)) / 6.283185307179586
+    if bool((f >= 0.5).any()):
+        raise ValueError("rotary_turns: base must keep every frequency below half a turn per position")
+    return (f * 2.0 ** 64).to(torch.int64).to(device)
+
+
+def _view(t: torch.Tensor):
+    """(tensor, its strides for the C boundary): any (B, L, heads, D) or (B, heads, D) view whose last
+    dimension is contiguous goes as it is, anything else is copied."""
+    if t.stride(-1) != 1 and t.shape[-1] > 1:
+        t = t.contiguous()
+    if t.dim() == 3:
+        return t, Strides(t.stride(0), 0, t.stride(1))
+    return t, Strides(t.stride(0), t.stride(1), t.stride(2))
+
+
+def _same(name: str, *ts: Optional[torch.Tensor]) -> None:
+    """One device and, for activations, one type."""
+    ts = [t for t in ts if t is not None]
+    for t in ts[1:]:
+        if t.device != ts[0].device:
+            raise ValueError(f"{name}: tensors on {ts[0].device} and {t.device}")
+        if t.dtype != ts[0].dtype:
+            raise TypeError(f"{name}: tensors of {ts[0].dtype} and {t.dtype}")
+
+
+def _qk_args(name, q, k, wq, wk, turns, positions, pairs):
+    _cuda(q, k, wq, wk, turns, positions)
+    _same(name, q, k)
+    if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
+        raise ValueError(f"{name}: queries {tuple(q.shape)} and keys {tuple(k.shape)}, want (B, L, heads, D)")
+    B, L_, _, D = q.shape
+    for w in (wq, wk):
+        if w is not None and tuple(w.shape) != (D,):
+            raise ValueError(f"{name}: weight {tuple(w.shape)} for heads of {D}")
+    if turns is not None and (turns.dtype != torch.int64 or turns.dim() != 1 or 2 * turns.numel() > D):
+        raise ValueError(f"{name}: turns must be int64 of at most {D // 2} entries (rotary_turns)")
+    if positions is not None:
+        if positions.dtype.is_floating_point or tuple(positions.shape) not in ((B, L_), (L_,)):
+            raise ValueError(f"{name}: positions {positions.dtype} {tuple(positions.shape)} for {(B, L_)}")
+        positions = positions.long().expand(B, L_).contiguous()
+    if pairs not in PAIRS:
+        raise ValueError(f"{name}: pairs {pairs!r} (halves or neighbours)")
+    return _f32(wq), _f32(wk), _c(turns), positions, 0 if turns is None else 2 * turns.numel()
+
+
+def qk_norm_rotate_fwd(q, k, wq=None, wk=None, turns=None, *, positions=None, start: int = 0, eps: float = 1e-6,
+                       pairs: str = "halves"):
+    """(queries, keys) normed for each head, weighted by wq / wk (D, None: ones) and rotated by position
+    in one pass.  q (B, L, Hq, D) and k (B, L, Hk, D) may be views of one projection's rows.  turns:
+    rotary_turns(R) for the first R elements of a head (None: no rotation); positions (B, L) or (L,),
+    default start, start + 1, ...; pairs "halves" (i with i + R/2) or "neighbours" (2i with 2i + 1)."""
+    wq, wk, turns, positions, R = _qk_args("qk_norm_rotate_fwd", q, k, wq, wk, turns, positions, pairs)
+    (q, qs), (k, ks) = _view(q), _view(k)
+    B, L_, Hq, D = q.shape
+    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    check(lib().pgf_qk_norm_rotate_fwd(_p(q), qs, _p(k), ks, _p(wq), _p(wk), _p(turns), _p(positions), start, _p(qo),
+                                       _p(ko), B, L_, Hq, k.shape[2], D, R, PAIRS[pairs], eps, _dt(q), _stream()),
+          "qk_norm_rotate_fwd")
+    return qo, ko
+
+
+def qk_norm_rotate_bwd(q, k, gq, gk, wq=None, wk=None, turns=None, *, positions=None, start: int = 0,
+                       eps: float = 1e-6, pairs: str = "halves", acc=None) -> Dict[str, torch.Tensor]:
+    """Gradients of qk_norm_rotate_fwd from its inputs and the gradients of its outputs: grad_q, grad_k,
+    and grad_wq, grad_wk (float32) where a weight was given.  acc: a dict of float32 grad_wq / grad_wk
+    buffers to add into (both or none)."""
+    name = "qk_norm_rotate_bwd"
+    has_q, has_k = wq is not None, wk is not None
+    wq, wk, turns, positions, R = _qk_args(name, q, k, wq, wk, turns, positions, pairs)
+    _cuda(gq, gk)
+    _same(name, q, gq, gk)
+    if gq.shape != q.shape or gk.shape != k.shape:
+        raise ValueError(f"{name}: gradients {tuple(gq.shape)}, {tuple(gk.shape)} of {tuple(q.shape)}, {tuple(k.shape)}")
+    (q, qs), (k, ks) = _view(q), _view(k)
+    gq, gk = _c(gq), _c(gk)
+    B, L_, Hq, D = q.shape
+    out = {"grad_q": torch.empty(q.shape, dtype=q.dtype, device=q.device),
+           "grad_k": torch.empty(k.shape, dtype=k.dtype, device=k.device)}
+    acc = acc or {}
+    flags = set()
+    for key, has in (("grad_wq", has_q), ("grad_wk", has_k)):
+        if has:
+            out[key], a = _acc_buffer(acc.get(key), (D,), q.device, name)
+            flags.add(a)
+    if len(flags) > 1:
+        raise ValueError(f"{name}: give both accumulators or none")
+    L = lib()
+    ws = _ws(L.pgf_qk_norm_rotate_bwd_workspace(D), q.device)
+    check(L.pgf_qk_norm_rotate_bwd(_p(q), qs, _p(k), ks, _p(gq), _p(gk), _p(wq), _p(wk), _p(turns), _p(positions), start,
+                                   _p(out["grad_q"]), _p(out["grad_k"]), _p(out.get("grad_wq")),
+                                   _p(out.get("grad_wk")), int(flags == {1}), B, L_, Hq, k.shape[2], D, R, PAIRS[pairs],
+                                   eps, _dt(q), _p(ws), ws.numel(), _stream()), name)
+    return out
+
+
+def _decay_args(name, q, k, v, log_decay, dims):
+    """Checks what the decay-attention calls share; (B, L, H, Hq, Hk, Hv, Dk, Dv)."""
+    _cuda(q, k, v, log_decay)
+    _same(name, q, k, v)
+    if log_decay.dtype != torch.float32 or log_decay.dim() != 1 or log_decay.device != q.device:
+        raise ValueError(f"{name}: log_decay must be float32 of one entry per head on {q.device}")
+    if any(t.dim() != dims for t in (q, k, v)) or q.shape[:-2] != k.shape[:-2] or q.shape[:-2] != v.shape[:-2] \
+            or q.shape[-1] != k.shape[-1]:
+        raise ValueError(f"{name}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, want "
+                         f"({'B, L' if dims == 4 else 'B'}, heads, D)")
+    return (q.shape[0], q.shape[1] if dims == 4 else 1, log_decay.numel(), q.shape[-2], k.shape[-2], v.shape[-2],
+            q.shape[-1], v.shape[-1])
+
+
+def _state_arg(name, t, shape, device):
+    if t is None:
+        return None
+    if tuple(t.shape) != tuple(shape) or t.dtype != torch.float32 or t.device != device:
+        raise ValueError(f"{name}: state {t.dtype} {tuple(t.shape)} on {t.device}, want float32 {tuple(shape)} on {device}")
+    return t.contiguous()
+
+
+def _lengths_arg(name, lengths, B, device):
+    if lengths is None:
+        return None
+    _cuda(lengths)
+    if lengths.dtype.is_floating_point or tuple(lengths.shape) != (B,) or lengths.device != device:
+        raise ValueError(f"{name}: lengths {lengths.dtype} {tuple(lengths.shape)}, want whole numbers ({B},) on {device}")
+    return lengths.to(torch.int32).contiguous()
+
+
+def decay_attn_fwd(q, k, v, log_decay, *, scale: Optional[float] = None, state=None, lengths=None,
+                   want_state: bool = True):
+    """(out, final state) of linear attention with a decay for each head:
+    S_t = exp(log_decay) S_{t-1} + k_t v_t^T, o_t = scale q_t S_t.  q (B, L, Hq, Dk), k (B, L, Hk, Dk),
+    v (B, L, Hv, Dv), log_decay (H) float32; each head count divides H, out is (B, L, H, Dv).  scale
+    defaults to Dk^-0.5.  state: float32 (B, H, Dk, Dv) that came before (None: zeros); lengths (B):
+    tokens past a row's length are not there."""
+    name = "decay_attn_fwd"
+    B, L_, H, Hq, Hk, Hv, Dk, Dv = _decay_args(name, q, k, v, log_decay, 4)
+    state = _state_arg(name, state, (B, H, Dk, Dv), q.device)
+    lengths = _lengths_arg(name, lengths, B, q.device)
+    (q, qs), (k, ks), (v, vs) = _view(q), _view(k), _view(v)
+    out = torch.empty(B, L_, H, Dv, dtype=q.dtype, device=q.device)
+    end = torch.empty(B, H, Dk, Dv, dtype=torch.float32, device=q.device) if want_state else None
+    L = lib()
+    ws = _ws(L.pgf_decay_attn_workspace(B, L_, H, Hq, Hk, Hv, Dk, Dv, _dt(q), 0), q.device)
+    check(L.pgf_decay_attn_fwd(_p(q), qs, _p(k), ks, _p(v), vs, _p(_c(log_decay)), _p(state), _p(lengths), _p(out),
+                               _p(end), B, L_, H, Hq, Hk, Hv, Dk, Dv, Dk ** -0.5 if scale is None else scale, _dt(q),
+                               _p(ws), ws.numel(), _stream()), name)
+    return out, end
+
+
+def decay_attn_bwd(q, k, v, log_decay, g, *, scale: Optional[float] = None, state=None, g_state=None, lengths=None,
+                   need_g_log_decay: bool = False, g_log_decay_acc=None) -> Dict[str, torch.Tensor]:
+    """Gradients of decay_attn_fwd from its inputs, g (of out) and g_state (of the final state, None:
+    zeros): grad_q, grad_k, grad_v, grad_state (float32, of the state that came before; with `state`
+    or g_state given or not) and, when asked for, grad_log_decay (H) float32."""
+    name = "decay_attn_bwd"
+    B, L_, H, Hq, Hk, Hv, Dk, Dv = _decay_args(name, q, k, v, log_decay, 4)
+    _cuda(g)
+    _same(name, q, g)
+    if tuple(g.shape) != (B, L_, H, Dv):
+        raise ValueError(f"{name}: gradient {tuple(g.shape)} of an output {(B, L_, H, Dv)}")
+    state = _state_arg(name, state, (B, H, Dk, Dv), q.device)
+    g_state = _state_arg(name, g_state, (B, H, Dk, Dv), q.device)
+    lengths = _lengths_arg(name, lengths, B, q.device)
+    (q, qs), (k, ks), (v, vs), (g, gs) = _view(q), _view(k), _view(v), _view(g)
+    dev = q.device
+    out = {"grad_q": torch.empty(q.shape, dtype=q.dtype, device=dev),
+           "grad_k": torch.empty(k.shape, dtype=q.dtype, device=dev),
+           "grad_v": torch.empty(v.shape, dtype=q.dtype, device=dev),
+           "grad_state": torch.empty(B, H, Dk, Dv, dtype=torch.float32, device=dev)}
+    accum = 0
+    if need_g_log_decay or g_log_decay_acc is not None:
+        out["grad_log_decay"], accum = _acc_buffer(g_log_decay_acc, (H,), dev, name)
+    L = lib()
+    ws = _ws(L.pgf_decay_attn_workspace(B, L_, H, Hq, Hk, Hv, Dk, Dv, _dt(q), 1), dev)
+    check(L.pgf_decay_attn_bwd(_p(q), qs, _p(k), ks, _p(v), vs, _p(_c(log_decay)), _p(state), _p(lengths), _p(g), gs,
+                               _p(g_state), _p(out["grad_q"]), _p(out["grad_k"]), _p(out["grad_v"]),
+                               _p(out.get("grad_log_decay")), _p(out["grad_state"]), accum, B, L_, H, Hq, Hk, Hv, Dk, Dv,
+                               Dk ** -0.5 if scale is None else scale, _dt(q), _p(ws), ws.numel(), _stream()), name)
+    return out
+
+
+def decay_attn_step(q, k, v, log_decay, state, *, scale: Optional[float] = None, rows=None, out_state=None):
+    """(out (B, H, Dv), new state) for one token of every row: q (B, Hq, Dk), k (B, Hk, Dk), v (B, Hv, Dv).
+    rows (B): row b goes on from state row rows[b] (a beam's parent) instead of its own.  out_state:
+    where the new state goes (`state` itself updates in place, without rows); default a new tensor."""
+    name = "decay_attn_step"
+    B, _, H, Hq, Hk, Hv, Dk, Dv = _decay_args(name, q, k, v, log_decay, 3)
+    _cuda(state, rows, out_state)
+    n_src = B if rows is None else state.shape[0]
+    if not state.is_contiguous():
+        raise ValueError(f"{name}: state must be contiguous")
+    state = _state_arg(name, state, (n_src, H, Dk, Dv), q.device)
+    if rows is not None:
+        if rows.dtype.is_floating_point or tuple(rows.shape) != (B,):
+            raise ValueError(f"{name}: rows {rows.dtype} {tuple(rows.shape)}, want whole numbers ({B},)")
+        rows = rows.long().contiguous()
+    new = _out_buf(out_state, (B, H, Dk, Dv), torch.float32, q.device, name)
+    (q, qs), (k, ks), (v, vs) = _view(q), _view(k), _view(v)
+    out = torch.empty(B, H, Dv, dtype=q.dtype, device=q.device)
+    check(lib().pgf_decay_attn_step(_p(q), qs, _p(k), ks, _p(v), vs, _p(_c(log_decay)), _p(state), _p(rows), n_src,
+                                    _p(out), _p(new), B, H, Hq, Hk, Hv, Dk, Dv, Dk ** -0.5 if scale is None else scale,
+                                    _dt(q), _stream()), name)
+    return out, new
+
+
+# --------------------------------------------------------------------------- beam search
+def beam_select(logits, scores, finished=None, *, end_id: Optional[int] = None):
+    """One selection step of a beam search: (scores, rows, tokens, finished), each (B, K), best first.
+    logits (B, K, V), scores (B, K) float32; the candidates scores + log_softmax(logits) of all K V
+    continuations in the order (value descending, flat index ascending).  rows: the flat row b K + k
+    that each new beam goes on from (for beam_reorder and decay_attn_step).  finished (B, K) bool: such
+    a beam's one candidate is end_id at its own score.  A NaN candidate counts as -inf."""
+    name = "beam_select"
+    _cuda(logits, scores, finished)
+    if logits.dim() != 3 or tuple(scores.shape) != tuple(logits.shape[:2]):
+        raise ValueError(f"{name}: logits {tuple(logits.shape)} and scores {tuple(scores.shape)}, want (B, K, V), (B, K)")
+    if scores.dtype != torch.float32:
+        raise TypeError(f"{name}: scores must be float32, not {scores.dtype}")
+    if finished is not None and (finished.dtype != torch.bool or finished.shape != scores.shape):
+        raise ValueError(f"{name}: finished must be bool {tuple(scores.shape)}")
+    dt = _dt(logits)
+    B, K, V = logits.shape
+    logits, scores, finished = _c(logits), _c(scores), _c(finished)
+    so = torch.empty(B, K, dtype=torch.float32, device=logits.device)
+    rows = torch.empty(B, K, dtype=torch.int64, device=logits.device)
+    tokens = torch.empty_like(rows)
+    fo = torch.empty(B, K, dtype=torch.bool, device=logits.device)
+    check(lib().pgf_beam_select(_p(logits), _p(scores), _p(finished), _p(so), _p(rows), _p(tokens), _p(fo), B, K, V,
+                                -1 if end_id is None else end_id, dt, _stream()), name)
+    return so, rows, tokens, fo
+
+
+def beam_reorder(states, rows, out=None):
+    """[s[rows] for s in states], in one launch: states of any type, (n, ...) contiguous; rows of any
+    shape (flattened).  out: contiguous tensors to write (not the states themselves)."""
+    name = "beam_reorder"
+    states = list(states)
+    _cuda(rows, *states)
+    if rows.dtype.is_floating_point:
+        raise TypeError(f"{name}: rows must be whole numbers, not {rows.dtype}")
+    rows = rows.reshape(-1).long().contiguous()
+    if not states:
+        return []
+    n_src, n = states[0].shape[0], rows.numel()
+    states = [_c(s) for s in states]
+    if any(s.shape[0] != n_src or s.device != rows.device for s in states):
+        raise ValueError(f"{name}: every state needs {n_src} rows on {rows.device}")
+    outs = [_out_buf(None if out is None else out[i], (n, *s.shape[1:]), s.dtype, s.device, name)
+            for i, s in enumerate(states)]
+    c = len(states)
+    src = (ctypes.c_void_p * c)(*[s.data_ptr() for s in states])
+    dst = (ctypes.c_void_p * c)(*[o.data_ptr() for o in outs])
+    nb = (ctypes.c_int64 * c)(*[math.prod(s.shape[1:]) * s.element_size() for s in states])
+    check(lib().pgf_beam_reorder(src, dst, nb, c, _p(rows), n, n_src, _stream()), name)
+    return outs

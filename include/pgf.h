@@ -547,6 +547,88 @@ int pgf_frechet_jvp(const float* u, const float* u_dot, const float* W_cat, cons
                     float* y_dot, float* h_end, float* h_end_dot, int64_t L, int64_t D, int64_t N, void* ws,
                     size_t ws_bytes, pgf_stream_t stream);
 
+/* ------------------------------------------------------------------------------------------
+ * A decay-attention layer: operators that the reference does not have, for models that mix its
+ * blocks with linear attention, trained with the same step and decoded token by token.
+ *
+ * Their inputs may be views (the query, key and value parts of one projection's rows): `*_strides`
+ * gives the distance in elements between batch rows, tokens and heads of a (B, L, heads, D) tensor
+ * whose last dimension is contiguous; NULL means contiguous.  Outputs are contiguous.
+ * ------------------------------------------------------------------------------------------ */
+typedef struct pgf_strides {
+  int64_t batch, token, head;
+} pgf_strides;
+
+/* which elements of a head the rotation pairs: i with i + R/2, or 2i with 2i + 1 */
+#define PGF_PAIRS_HALVES 0
+#define PGF_PAIRS_NEIGHBOURS 1
+
+/* Norms of queries (B, L, Hq, D) and keys (B, L, Hk, D) for each head, with the position rotation
+ * in the same pass: u = x / sqrt(mean x^2 + eps) * w, then pair i of the first R elements turned by
+ * 2 pi frac(position * turns[i]).  wq, wk (D) may be NULL (ones); Hq or Hk may be 0.  turns (R/2):
+ * frequencies as 64-bit fixed-point fractions of a turn per position, so that whole turns fall off
+ * exactly.  positions (B, L), or NULL: token l stands at start + l.  1 <= D <= 256, R even, R <= D.
+ * The backward recomputes the norms from q and k; gq, gk contiguous; grad_wq, grad_wk may be NULL. */
+int pgf_qk_norm_rotate_fwd(const void* q, const pgf_strides* q_strides, const void* k,
+                           const pgf_strides* k_strides, const float* wq, const float* wk,
+                           const int64_t* turns, const int64_t* positions, int64_t start, void* q_out,
+                           void* k_out, int64_t Bsz, int64_t L, int64_t Hq, int64_t Hk, int64_t D, int64_t R,
+                           int pairs, float eps, int dtype, pgf_stream_t stream);
+size_t pgf_qk_norm_rotate_bwd_workspace(int64_t D);
+int pgf_qk_norm_rotate_bwd(const void* q, const pgf_strides* q_strides, const void* k,
+                           const pgf_strides* k_strides, const void* gq, const void* gk, const float* wq,
+                           const float* wk, const int64_t* turns, const int64_t* positions, int64_t start,
+                           void* grad_q, void* grad_k, float* grad_wq, float* grad_wk, int accumulate,
+                           int64_t Bsz, int64_t L, int64_t Hq, int64_t Hk, int64_t D, int64_t R, int pairs,
+                           float eps, int dtype, void* ws, size_t ws_bytes, pgf_stream_t stream);
+
+/* Linear attention with a decay for each of H heads:
+ *   S_t = exp(log_decay) S_{t-1} + k_t v_t^T,   o_t = scale q_t S_t
+ * q (B, L, Hq, Dk), k (B, L, Hk, Dk), v (B, L, Hv, Dv), each head count a divisor of H (head h reads
+ * head h / (H / Hq) and so on); out (B, L, H, Dv).  state / state_out: float32 (B, H, Dk, Dv) before
+ * the first and after the last token, each may be NULL (zeros / not wanted).  lengths (B): tokens past
+ * a row's length are not there (whatever they hold), their outputs and gradients are zeros.
+ * log_decay (H) float32, normally <= 0.  1 <= Dk, Dv <= 256.
+ * The backward recomputes every state; g (B, L, H, Dv) is the output's gradient, g_state the final
+ * state's (may be NULL); grad_log_decay (H) and grad_state may be NULL; `accumulate` concerns
+ * grad_log_decay.
+ * The step takes one token per row (a token stride is unused) and may update in place (state_out ==
+ * state) when rows is NULL; with rows (B), row b goes on from state row rows[b] of n_src (a beam's
+ * parent; out of range: zeros), and state_out must not overlap state. */
+size_t pgf_decay_attn_workspace(int64_t Bsz, int64_t L, int64_t H, int64_t Hq, int64_t Hk, int64_t Hv, int64_t Dk,
+                                int64_t Dv, int dtype, int backward);
+int pgf_decay_attn_fwd(const void* q, const pgf_strides* q_strides, const void* k, const pgf_strides* k_strides,
+                       const void* v, const pgf_strides* v_strides, const float* log_decay, const float* state,
+                       const int32_t* lengths, void* out, float* state_out, int64_t Bsz, int64_t L, int64_t H,
+                       int64_t Hq, int64_t Hk, int64_t Hv, int64_t Dk, int64_t Dv, float scale, int dtype, void* ws,
+                       size_t ws_bytes, pgf_stream_t stream);
+int pgf_decay_attn_bwd(const void* q, const pgf_strides* q_strides, const void* k, const pgf_strides* k_strides,
+                       const void* v, const pgf_strides* v_strides, const float* log_decay, const float* state,
+                       const int32_t* lengths, const void* g, const pgf_strides* g_strides, const float* g_state,
+                       void* grad_q, void* grad_k, void* grad_v, float* grad_log_decay, float* grad_state,
+                       int accumulate, int64_t Bsz, int64_t L, int64_t H, int64_t Hq, int64_t Hk, int64_t Hv,
+                       int64_t Dk, int64_t Dv, float scale, int dtype, void* ws, size_t ws_bytes,
+                       pgf_stream_t stream);
+int pgf_decay_attn_step(const void* q, const pgf_strides* q_strides, const void* k, const pgf_strides* k_strides,
+                        const void* v, const pgf_strides* v_strides, const float* log_decay, const float* state,
+                        const int64_t* rows, int64_t n_src, void* out, float* state_out, int64_t Bsz, int64_t H,
+                        int64_t Hq, int64_t Hk, int64_t Hv, int64_t Dk, int64_t Dv, float scale, int dtype,
+                        pgf_stream_t stream);
+
+/* One step of a beam search.  pgf_beam_select takes the first K of the K x V candidates
+ *   c[k, v] = scores[k] + (logits[k, v] - logsumexp(logits[k]))
+ * of each sequence in the order (c descending, k V + v ascending): logits (B, K, V), scores (B, K);
+ * finished (B, K) bytes or NULL: such a beam has one candidate, end_id at its own score.  NaN counts
+ * as -inf.  Outputs (B, K), best first: scores, rows (flat row b K + k that goes on), tokens, and
+ * finished (may be NULL): the row had finished or the token is end_id (-1: none).  K <= 32, K V < 2^31.
+ * pgf_beam_reorder copies dst[i] = src[rows[i]] for `count` tensors of n_src rows of row_bytes each
+ * (host arrays, read during the call); a row out of range gives zeros. */
+int pgf_beam_select(const void* logits, const float* scores, const uint8_t* finished, float* out_scores,
+                    int64_t* out_rows, int64_t* out_tokens, uint8_t* out_finished, int64_t Bsz, int64_t K, int64_t V,
+                    int64_t end_id, int dtype, pgf_stream_t stream);
+int pgf_beam_reorder(const void* const* src, void* const* dst, const int64_t* row_bytes, int count,
+                     const int64_t* rows, int64_t n_rows, int64_t n_src, pgf_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
