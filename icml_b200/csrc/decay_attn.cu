@@ -1,6 +1,6 @@
 // Linear attention with a decay for each head: the float32 engine (any width up to 256, any strides,
 // both types), the single-token step, and the entry points.  decay_attn.cuh has the formulas.
-#include "decay_attn.cuh"
+#include "decay_attn_tc.cuh"
 
 namespace pgf {
 namespace da {
@@ -89,7 +89,9 @@ __global__ void __launch_bounds__(THREADS) walk_kernel(const Job job, const Tang
   }
   float tsum = 0.f;
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
-  const int chunks = int((s1 - s0 + C - 1) / C);
+  // (the end state of the walk's last piece enters no other piece)
+  const bool idle = MODE == MODE_STATE && seg == (job.rev ? 0 : job.segs - 1);
+  const int chunks = idle ? 0 : int((s1 - s0 + C - 1) / C);
   for (int ci = 0; ci < chunks; ++ci) {
     const int64_t t0 = s0 + int64_t(job.rev ? chunks - 1 - ci : ci) * C;
     const int n = int(min(int64_t(C), s1 - t0));
@@ -260,7 +262,7 @@ __global__ void __launch_bounds__(THREADS) walk_kernel(const Job job, const Tang
     float* end = MODE == MODE_STATE
                      ? const_cast<float*>(job.start) + (b * job.H + h) * job.start_stride + int64_t(seg) * dx * dz
                      : (job.end && seg == (job.rev ? 0 : job.segs - 1) ? job.end + (b * job.H + h) * dx * dz : nullptr);
-    if (end)
+    if (end && !idle)
       for (int i = threadIdx.x; i < dx * cw; i += THREADS) end[int64_t(i / cw) * dz + c0 + i % cw] = sS[(i / cw) * E + i % cw];
   } else {
     if (tan.behind) {
@@ -282,7 +284,7 @@ __global__ void __launch_bounds__(THREADS) walk_kernel(const Job job, const Tang
 
 // The pieces' own end states (B, H, segs, n) become the states that enter each piece: one thread per
 // state element walks the pieces in the direction of time (or back).
-__global__ void __launch_bounds__(256) enter_kernel(float* pieces, const float* first, float* last, const float* log_decay,
+__global__ void __launch_bounds__(256) enter_kernel(float* pieces, const float* first, const float* log_decay,
                                                     const int32_t* lengths, int64_t L, int H, int segs, int64_t seg_len,
                                                     int rev, int64_t n, int blocks) {
   const int64_t bh = blockIdx.x / blocks, b = bh / H;
@@ -294,14 +296,14 @@ __global__ void __launch_bounds__(256) enter_kernel(float* pieces, const float* 
   float cur = first ? first[bh * n + i] : 0.f;
   float* p = pieces + bh * segs * n + i;
 #pragma unroll 4
-  for (int k = 0; k < segs; ++k) {
+  for (int k = 0; k + 1 < segs; ++k) {
     const int s = rev ? segs - 1 - k : k;
     const int64_t s0 = min(len, s * seg_len), s1 = min(len, s0 + seg_len);
     const float own = p[s * n];
     p[s * n] = cur;
     cur = fmaf(exp2f(l2 * float(s1 - s0)), cur, own);
   }
-  if (last) last[bh * n + i] = cur;
+  p[(rev ? 0 : segs - 1) * n] = cur;
 }
 
 // out (tokens, heads, d) = sum over the H / heads operator heads that share each head of part (tokens, H, d)
@@ -446,16 +448,29 @@ __global__ void __launch_bounds__(256) step_kernel(const StepArgs a) {
 // ---------------------------------------------------------------------------------------------
 // host
 // ---------------------------------------------------------------------------------------------
-// Pieces of the sequence: enough CTAs to fill the GPU, none shorter than two chunks (a piece costs a
-// second pass over its y and z).
-static void split(int64_t B, int64_t H, int64_t L, int slices, int chunk, int* segs, int64_t* seg_len) {
-  const int64_t ctas = B * H * slices, chunks = (L + chunk - 1) / chunk;
-  int64_t s = ctas >= 148 || ctas == 0 ? 1 : (2 * 148 + ctas - 1) / ctas;
-  if (s > (chunks + 1) / 2) s = (chunks + 1) / 2;
-  if (s < 1) s = 1;
-  const int64_t per = (chunks + s - 1) / s;
-  *seg_len = (per ? per : 1) * chunk;
-  *segs = int(chunks ? (chunks + per - 1) / per : 1);
+// How the sequence is cut.  Pieces run side by side, but all except one have their y and z read a second time
+// (for the states that enter the others), so the cut is the one with the least time over the waves of CTAs:
+// chunks of a piece (1.5 x when cut) plus a fixed 2.5 chunks of start and end per piece and 3 for the extra
+// launches, in units of one chunk's time.
+struct Cut {
+  int segs;
+  int64_t seg_len;
+};
+static Cut cut(int64_t ctas, int64_t L, int chunk, int resident) {
+  const int64_t chunks = (L + chunk - 1) / chunk, slots = 148 * resident;
+  Cut best = {1, (chunks ? chunks : 1) * chunk};
+  if (ctas == 0) return best;
+  double least = 0;
+  for (int64_t s = 1; s <= chunks && s <= 2 * slots; ++s) {
+    const int64_t per = (chunks + s - 1) / s, n = (chunks + per - 1) / per;
+    if (n != s) continue;
+    const double t = double((ctas * n + slots - 1) / slots) * (double(per) * (n > 1 ? 1.5 : 1.0) + 2.5) + (n > 1 ? 3.0 : 0.0);
+    if (s == 1 || t < least) {
+      least = t;
+      best = {int(n), per * chunk};
+    }
+  }
+  return best;
 }
 
 struct Shape {
@@ -485,35 +500,62 @@ static Tensor tensor(const void* p, const pgf_strides* s, int64_t L, int64_t hea
   return t;
 }
 
-// One F call on the float32 engine, with the states that enter its pieces already in `job.start`.
-static int f_states(Job job, const float* first, float* pieces, float* last, int dtype, cudaStream_t s) {
-  // the pieces' own end states, then the states that enter them
+// The calls of one entry point take one engine and one cut.
+struct Plan {
+  bool tc;
+  Cut c;
+};
+static Plan plan(const Shape& p, bool tc, bool backward) {
+  if (tc) return {true, cut(p.B * p.H, p.L, TC_CHUNK, 1)};
+  // a backward's calls have either width as columns and either as rows
+  const int64_t cols = backward && p.Dk < p.Dv ? p.Dk : p.Dv, rows = backward && p.Dv > p.Dk ? p.Dv : p.Dk;
+  return {false, cut(p.B * p.H * ceil_div(cols, E), p.L, chunk_of(int(rows)), 1)};
+}
+
+// The state that enters each piece of a walk: (B, H, segs, rows, columns).
+struct Entering {
+  const float* p;       // NULL: zeros (an uncut walk without a first state)
+  int64_t stride;
+};
+
+static int f_call(const Job& job, const Plan& pl, int dtype, cudaStream_t s) {
+  if (pl.tc) return tc_walk(job, false, s);
+  return walk<MODE_OUT>(job, TangentArgs{}, dtype, s);
+}
+
+// What enters the pieces of a walk that begins with `first`; `pieces` is scratch for them.
+static int entering(Job job, const Plan& pl, const float* first, float* pieces, Entering* e, int dtype, cudaStream_t s) {
+  const int64_t n = int64_t(job.y.d) * job.z.d;
+  *e = {first, n};
+  if (job.segs == 1) return PGF_OK;
   job.start = pieces;
-  job.start_stride = int64_t(job.segs) * job.x.d * job.z.d;
+  job.start_stride = job.segs * n;
   job.start_t = 0;
-  PGF_TRY(walk<MODE_STATE>(job, TangentArgs{}, dtype, s));
-  const int64_t n = int64_t(job.x.d) * job.z.d;
+  if (pl.tc) PGF_TRY(tc_walk(job, true, s));
+  else PGF_TRY(walk<MODE_STATE>(job, TangentArgs{}, dtype, s));
   const int blocks = ceil_div(n, 256);
-  enter_kernel<<<unsigned(job.B * job.H * blocks), 256, 0, s>>>(pieces, first, last, job.log_decay, job.lengths, job.L,
-                                                                job.H, job.segs, job.seg_len, job.rev, n, blocks);
+  enter_kernel<<<unsigned(job.B * job.H * blocks), 256, 0, s>>>(pieces, first, job.log_decay, job.lengths, job.L, job.H,
+                                                                job.segs, job.seg_len, job.rev, n, blocks);
   PGF_LAUNCH_CHECK();
+  *e = {pieces, job.segs * n};
   return PGF_OK;
 }
 
-static size_t f32_workspace(const Shape& p, int backward) {
-  int segs;
-  int64_t len;
-  split(p.B, p.H, p.L, ceil_div(p.Dv < p.Dk ? p.Dv : p.Dk, E), 32, &segs, &len);
-  size_t n = 0;
-  const size_t state = size_t(p.B) * p.H * segs * p.Dk * p.Dv * sizeof(float);
-  n += Workspace::round(state) + 256;
+static size_t workspace(const Shape& p, bool backward) {
+  const size_t state = size_t(p.B) * p.H * p.Dk * p.Dv * sizeof(float);
+  const Plan f = plan(p, false, backward), t = plan(p, true, backward);
+  size_t pieces = 0;
+  for (const Plan& q : {f, t})
+    if (q.c.segs > 1 && q.c.segs * state > pieces) pieces = q.c.segs * state;
+  size_t n = 256;
+  if (pieces) n += (backward ? 2 : 1) * (Workspace::round(pieces) + 256);
   if (backward) {
-    n += Workspace::round(state) + 256;
+    const int segs = f.c.segs > t.c.segs ? f.c.segs : t.c.segs;
     n += Workspace::round(size_t(p.H) * p.B * segs * ceil_div(p.Dv, E) * sizeof(float)) + 256;
-    const size_t t = size_t(p.B) * p.L * p.H * sizeof(float);
-    if (p.Hq < p.H) n += Workspace::round(t * p.Dk) + 256;
-    if (p.Hk < p.H) n += Workspace::round(t * p.Dk) + 256;
-    if (p.Hv < p.H) n += Workspace::round(t * p.Dv) + 256;
+    const size_t tok = size_t(p.B) * p.L * p.H * sizeof(float);
+    if (p.Hq < p.H) n += Workspace::round(tok * p.Dk) + 256;
+    if (p.Hk < p.H) n += Workspace::round(tok * p.Dk) + 256;
+    if (p.Hv < p.H) n += Workspace::round(tok * p.Dv) + 256;
   }
   return n;
 }
@@ -537,7 +579,7 @@ extern "C" size_t pgf_decay_attn_workspace(int64_t Bsz, int64_t L, int64_t H, in
                                            int64_t Dk, int64_t Dv, int dtype, int backward) {
   const da::Shape p = {Bsz, L, H, Hq, Hk, Hv, Dk, Dv};
   if (da::check("decay_attn_workspace", p, dtype) != PGF_OK) return 0;
-  return da::f32_workspace(p, backward);
+  return da::workspace(p, backward != 0);
 }
 
 extern "C" int pgf_decay_attn_fwd(const void* q, const pgf_strides* q_strides, const void* k,
@@ -564,21 +606,25 @@ extern "C" int pgf_decay_attn_fwd(const void* q, const pgf_strides* q_strides, c
   job.scale = scale;
   job.z_scale = 1.f;
   job.B = Bsz; job.L = L; job.H = int(H);
-  da::split(Bsz, H, L, ceil_div(Dv, da::E), da::chunk_of(int(Dk)), &job.segs, &job.seg_len);
-  job.start = state;
-  job.start_stride = Dk * Dv;
+  const bool tc = dtype == PGF_DTYPE_BF16 && L > 0 && da::tc_fits(job.x, Bsz, L) && da::tc_fits(job.y, Bsz, L) &&
+                  da::tc_fits(job.z, Bsz, L) && aligned(out, 16);
+  const da::Plan pl = da::plan(p, tc, false);
+  job.segs = pl.c.segs;
+  job.seg_len = pl.c.seg_len;
+  float* pieces = nullptr;
   if (job.segs > 1) {
     Workspace w(ws, ws_bytes);
-    float* pieces = w.take<float>(size_t(Bsz) * H * job.segs * Dk * Dv);
+    pieces = w.take<float>(size_t(Bsz) * H * job.segs * Dk * Dv);
     if (!ws || !pieces) {
       set_error("decay_attn_fwd: workspace of %zu bytes is too small", ws_bytes);
       return PGF_ERR_WORKSPACE;
     }
-    PGF_TRY(da::f_states(job, state, pieces, nullptr, dtype, s));
-    job.start = pieces;
-    job.start_stride = int64_t(job.segs) * Dk * Dv;
   }
-  return da::walk<da::MODE_OUT>(job, da::TangentArgs{}, dtype, s);
+  da::Entering S;
+  PGF_TRY(da::entering(job, pl, state, pieces, &S, dtype, s));
+  job.start = S.p;
+  job.start_stride = S.stride;
+  return da::f_call(job, pl, dtype, s);
 }
 
 extern "C" int pgf_decay_attn_bwd(const void* q, const pgf_strides* q_strides, const void* k,
@@ -599,78 +645,82 @@ extern "C" int pgf_decay_attn_bwd(const void* q, const pgf_strides* q_strides, c
   PGF_CHECK_ARG(log_decay && (L == 0 || (q && k && v && g && grad_q && grad_k && grad_v)), "decay_attn_bwd: null pointer");
   const da::Tensor tq = da::tensor(q, q_strides, L, Hq, Dk), tk = da::tensor(k, k_strides, L, Hk, Dk),
                    tv = da::tensor(v, v_strides, L, Hv, Dv), tg = da::tensor(g, g_strides, L, H, Dv);
+  const bool tc = dtype == PGF_DTYPE_BF16 && L > 0 && da::tc_fits(tq, Bsz, L) && da::tc_fits(tk, Bsz, L) &&
+                  da::tc_fits(tv, Bsz, L) && da::tc_fits(tg, Bsz, L) && aligned(grad_q, 16) && aligned(grad_k, 16) &&
+                  aligned(grad_v, 16);
+  const da::Plan pl = da::plan(p, tc, true);
   da::Job job = {};
   job.log_decay = log_decay;
   job.lengths = lengths;
   job.B = Bsz; job.L = L; job.H = int(H);
-  da::split(Bsz, H, L, ceil_div(Dv < Dk ? Dv : Dk, da::E), da::chunk_of(int(Dk > Dv ? Dk : Dv)), &job.segs, &job.seg_len);
+  job.scale = 1.f;
+  job.segs = pl.c.segs;
+  job.seg_len = pl.c.seg_len;
   Workspace w(ws, ws_bytes);
   const size_t states = size_t(Bsz) * H * job.segs * Dk * Dv;
-  float* S = w.take<float>(states);
-  float* X = w.take<float>(states);
+  float* sp = job.segs > 1 ? w.take<float>(states) : nullptr;
+  float* xp = job.segs > 1 ? w.take<float>(states) : nullptr;
   float* part = w.take<float>(size_t(H) * Bsz * job.segs * ceil_div(Dv, da::E));
   const int64_t tokens = Bsz * L;
   float* pq = Hq < H ? w.take<float>(size_t(tokens) * H * Dk) : nullptr;
   float* pk = Hk < H ? w.take<float>(size_t(tokens) * H * Dk) : nullptr;
   float* pv = Hv < H ? w.take<float>(size_t(tokens) * H * Dv) : nullptr;
-  if (!ws || !S || !X || !part || (Hq < H && !pq) || (Hk < H && !pk) || (Hv < H && !pv)) {
+  if (!ws || !part || (job.segs > 1 && (!sp || !xp)) || (Hq < H && !pq) || (Hk < H && !pk) || (Hv < H && !pv)) {
     set_error("decay_attn_bwd: workspace of %zu bytes is too small", ws_bytes);
     return PGF_ERR_WORKSPACE;
   }
-  // the states that enter the pieces, from both ends; X carries the scale of g
+  // what enters the pieces from both ends; X carries the scale of g
+  da::Entering S, X;
   da::Job js = job;
-  js.y = tk; js.z = tv; js.x = tk;
+  js.x = js.y = tk; js.z = tv;
   js.z_scale = 1.f;
-  PGF_TRY(da::f_states(js, state, S, nullptr, dtype, s));
-  js.y = tq; js.z = tg; js.x = tq;
+  PGF_TRY(da::entering(js, pl, state, sp, &S, dtype, s));
+  js.x = js.y = tq; js.z = tg;
   js.z_scale = scale;
   js.rev = 1;
-  PGF_TRY(da::f_states(js, g_state, X, grad_state, dtype, s));
-  if (L == 0) {
-    if (grad_log_decay && !accumulate) PGF_CUDA(cudaMemsetAsync(grad_log_decay, 0, size_t(H) * sizeof(float), s));
-    return PGF_OK;
-  }
-  job.start_stride = int64_t(job.segs) * Dk * Dv;
+  PGF_TRY(da::entering(js, pl, g_state, xp, &X, dtype, s));
   const int f32 = dtype == PGF_DTYPE_F32;
   // grad q = scale F(g, v, k; S^T)
   da::Job jq = job;
   jq.x = tg; jq.y = tv; jq.z = tk;
-  jq.start = S; jq.start_t = 1;
+  jq.start = S.p; jq.start_stride = S.stride; jq.start_t = 1;
   jq.scale = scale; jq.z_scale = 1.f;
   jq.out = pq ? static_cast<void*>(pq) : grad_q;
   jq.out_f32 = f32 || pq;
-  PGF_TRY(da::walk<da::MODE_OUT>(jq, da::TangentArgs{}, dtype, s));
+  PGF_TRY(da::f_call(jq, pl, dtype, s));
   // grad v = F(k, q, scale g; X) from the end
   da::Job jv = job;
   jv.x = tk; jv.y = tq; jv.z = tg;
-  jv.start = X; jv.rev = 1;
-  jv.scale = 1.f; jv.z_scale = scale;
+  jv.start = X.p; jv.start_stride = X.stride; jv.rev = 1;
+  jv.z_scale = scale;
   jv.out = pv ? static_cast<void*>(pv) : grad_v;
   jv.out_f32 = f32 || pv;
-  PGF_TRY(da::walk<da::MODE_OUT>(jv, da::TangentArgs{}, dtype, s));
+  jv.end = grad_state;
+  PGF_TRY(da::f_call(jv, pl, dtype, s));
   // grad k = F(v, g, scale q; X^T) from the end
   da::Job jk = job;
   jk.x = tv; jk.y = tg; jk.z = tq;
-  jk.start = X; jk.start_t = 1; jk.rev = 1;
-  jk.scale = 1.f; jk.z_scale = scale;
+  jk.start = X.p; jk.start_stride = X.stride; jk.start_t = 1; jk.rev = 1;
+  jk.z_scale = scale;
   jk.out = pk ? static_cast<void*>(pk) : grad_k;
   jk.out_f32 = f32 || pk;
-  PGF_TRY(da::walk<da::MODE_OUT>(jk, da::TangentArgs{}, dtype, s));
+  PGF_TRY(da::f_call(jk, pl, dtype, s));
   if (grad_log_decay) {
     da::Job jt = job;
     jt.x = tq; jt.y = tk; jt.z = tv;
-    jt.start = S;
+    jt.start = S.p; jt.start_stride = S.stride;
     jt.z_scale = 1.f;
     da::TangentArgs t = {};
     t.g = tg;
-    t.behind = X;
-    t.behind_stride = job.start_stride;
+    t.behind = X.p;
+    t.behind_stride = X.stride;
     t.part = part;
     t.scale = scale;
     PGF_TRY(da::walk<da::MODE_TANGENT>(jt, t, dtype, s));
     da::decay_sum_kernel<<<unsigned(H), 256, 0, s>>>(part, grad_log_decay, Bsz * job.segs * ceil_div(Dv, da::E), accumulate);
     PGF_LAUNCH_CHECK();
   }
+  if (L == 0) return PGF_OK;
   struct { float* part; void* out; int64_t heads, d; } sums[3] = {{pq, grad_q, Hq, Dk}, {pk, grad_k, Hk, Dk}, {pv, grad_v, Hv, Dv}};
   for (auto& t : sums)
     if (t.part) {

@@ -43,7 +43,7 @@ struct Job {
   int out_f32;               // out is float32 (else the inputs' type)
   float* end;                // (B, H, x.d, z.d) the state after the walk, or NULL
   float scale;               // of out
-  float z_scale;             // of z in the state's update (the output gradient carries the scale there)
+  float z_scale;             // of z, in the output and in the state
   int64_t B, L;
   int H;
   int rev;                   // walk from the end
