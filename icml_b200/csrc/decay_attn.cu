@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(THREADS) walk_kernel(const Job job, const Tang
   float tsum = 0.f;
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
   // (the end state of the walk's last piece enters no other piece)
-  const bool idle = MODE == MODE_STATE && seg == (job.rev ? 0 : job.segs - 1);
+  const bool idle = MODE == MODE_STATE && !job.last_too && seg == (job.rev ? 0 : job.segs - 1);
   const int chunks = idle ? 0 : int((s1 - s0 + C - 1) / C);
   for (int ci = 0; ci < chunks; ++ci) {
     const int64_t t0 = s0 + int64_t(job.rev ? chunks - 1 - ci : ci) * C;
@@ -283,27 +283,39 @@ __global__ void __launch_bounds__(THREADS) walk_kernel(const Job job, const Tang
 }
 
 // The pieces' own end states (B, H, segs, n) become the states that enter each piece: one thread per
-// state element walks the pieces in the direction of time (or back).
-__global__ void __launch_bounds__(256) enter_kernel(float* pieces, const float* first, const float* log_decay,
-                                                    const int32_t* lengths, int64_t L, int H, int segs, int64_t seg_len,
-                                                    int rev, int64_t n, int blocks) {
+// state element walks the pieces in the direction of time (or back), eight loads ahead of their use.
+// last: the state behind the walk (the last piece's own end state has to be there), or NULL.
+__global__ void __launch_bounds__(128) enter_kernel(float* __restrict__ pieces, const float* __restrict__ first,
+                                                    float* __restrict__ last, const float* __restrict__ log_decay,
+                                                    const int32_t* __restrict__ lengths, int64_t L, int H, int segs,
+                                                    int64_t seg_len, int rev, int64_t n, int blocks) {
+  constexpr int U = 8;
   const int64_t bh = blockIdx.x / blocks, b = bh / H;
   const int h = int(bh % H);
   const float l2 = log2_decay(log_decay[h]);
   const int64_t len = row_length(lengths, b, L);
-  const int64_t i = int64_t(blockIdx.x % blocks) * 256 + threadIdx.x;
+  const int64_t i = int64_t(blockIdx.x % blocks) * 128 + threadIdx.x;
   if (i >= n) return;
   float cur = first ? first[bh * n + i] : 0.f;
   float* p = pieces + bh * segs * n + i;
-#pragma unroll 4
-  for (int k = 0; k + 1 < segs; ++k) {
-    const int s = rev ? segs - 1 - k : k;
-    const int64_t s0 = min(len, s * seg_len), s1 = min(len, s0 + seg_len);
-    const float own = p[s * n];
-    p[s * n] = cur;
-    cur = fmaf(exp2f(l2 * float(s1 - s0)), cur, own);
+  const int own_segs = last ? segs : segs - 1;
+  for (int k0 = 0; k0 < segs; k0 += U) {
+    float own[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u;
+      own[u] = k < own_segs ? p[int64_t(rev ? segs - 1 - k : k) * n] : 0.f;
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u, s = rev ? segs - 1 - k : k;
+      if (k >= segs) break;
+      const int64_t s0 = min(len, s * seg_len), s1 = min(len, s0 + seg_len);
+      p[int64_t(s) * n] = cur;
+      cur = fmaf(exp2f(l2 * float(s1 - s0)), cur, own[u]);
+    }
   }
-  p[(rev ? 0 : segs - 1) * n] = cur;
+  if (last) last[bh * n + i] = cur;
 }
 
 // out (tokens, heads, d) = sum over the H / heads operator heads that share each head of part (tokens, H, d)
@@ -523,19 +535,22 @@ static int f_call(const Job& job, const Plan& pl, int dtype, cudaStream_t s) {
   return walk<MODE_OUT>(job, TangentArgs{}, dtype, s);
 }
 
-// What enters the pieces of a walk that begins with `first`; `pieces` is scratch for them.
-static int entering(Job job, const Plan& pl, const float* first, float* pieces, Entering* e, int dtype, cudaStream_t s) {
+// What enters the pieces of a walk that begins with `first`; `pieces` is scratch for them.  last: where the
+// state behind a cut walk goes, or NULL (an uncut one gives it by itself).
+static int entering(Job job, const Plan& pl, const float* first, float* pieces, float* last, Entering* e, int dtype,
+                    cudaStream_t s) {
   const int64_t n = int64_t(job.y.d) * job.z.d;
   *e = {first, n};
   if (job.segs == 1) return PGF_OK;
   job.start = pieces;
   job.start_stride = job.segs * n;
   job.start_t = 0;
+  job.last_too = last != nullptr;
   if (pl.tc) PGF_TRY(tc_walk(job, true, s));
   else PGF_TRY(walk<MODE_STATE>(job, TangentArgs{}, dtype, s));
-  const int blocks = ceil_div(n, 256);
-  enter_kernel<<<unsigned(job.B * job.H * blocks), 256, 0, s>>>(pieces, first, job.log_decay, job.lengths, job.L, job.H,
-                                                                job.segs, job.seg_len, job.rev, n, blocks);
+  const int blocks = ceil_div(n, 128);
+  enter_kernel<<<unsigned(job.B * job.H * blocks), 128, 0, s>>>(pieces, first, last, job.log_decay, job.lengths, job.L,
+                                                                job.H, job.segs, job.seg_len, job.rev, n, blocks);
   PGF_LAUNCH_CHECK();
   *e = {pieces, job.segs * n};
   return PGF_OK;
@@ -621,7 +636,8 @@ extern "C" int pgf_decay_attn_fwd(const void* q, const pgf_strides* q_strides, c
     }
   }
   da::Entering S;
-  PGF_TRY(da::entering(job, pl, state, pieces, &S, dtype, s));
+  PGF_TRY(da::entering(job, pl, state, pieces, state_out, &S, dtype, s));
+  if (job.segs > 1) job.end = nullptr;
   job.start = S.p;
   job.start_stride = S.stride;
   return da::f_call(job, pl, dtype, s);
@@ -674,11 +690,11 @@ extern "C" int pgf_decay_attn_bwd(const void* q, const pgf_strides* q_strides, c
   da::Job js = job;
   js.x = js.y = tk; js.z = tv;
   js.z_scale = 1.f;
-  PGF_TRY(da::entering(js, pl, state, sp, &S, dtype, s));
+  PGF_TRY(da::entering(js, pl, state, sp, nullptr, &S, dtype, s));
   js.x = js.y = tq; js.z = tg;
   js.z_scale = scale;
   js.rev = 1;
-  PGF_TRY(da::entering(js, pl, g_state, xp, &X, dtype, s));
+  PGF_TRY(da::entering(js, pl, g_state, xp, grad_state, &X, dtype, s));
   const int f32 = dtype == PGF_DTYPE_F32;
   // grad q = scale F(g, v, k; S^T)
   da::Job jq = job;
@@ -695,7 +711,7 @@ extern "C" int pgf_decay_attn_bwd(const void* q, const pgf_strides* q_strides, c
   jv.z_scale = scale;
   jv.out = pv ? static_cast<void*>(pv) : grad_v;
   jv.out_f32 = f32 || pv;
-  jv.end = grad_state;
+  jv.end = job.segs > 1 ? nullptr : grad_state;
   PGF_TRY(da::f_call(jv, pl, dtype, s));
   // grad k = F(v, g, scale q; X^T) from the end
   da::Job jk = job;

@@ -49,6 +49,7 @@ struct Job {
   int rev;                   // walk from the end
   int segs;                  // pieces of the sequence walked in parallel
   int64_t seg_len;           // tokens of a piece, a multiple of the engine's chunk
+  int last_too;              // pieces' own end states: the walk's last piece as well
 };
 
 // a^e for the exponents of one head.  log2(a) is clamped so that e = 0 gives 1 for a decay of zero.

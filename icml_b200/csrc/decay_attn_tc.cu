@@ -20,11 +20,17 @@
 // hold hi's and lo's sum and lanes 64..127 mid's, D1 runs over both (K = 128, x used twice), and they are
 // added only where the state leaves the kernel.
 //
-// Roles (576 threads): warp 0 TMA, warp 1 MMA, warps 2..9 scores and output, warps 10..17 the weighted y and
-// the state.  Input tiles pass through a ring of slots in the order x, y, z: with four 32 KB slots x of the
-// next chunk is there when a chunk begins and y and z arrive while it is worked on.  hi overwrites y in its
-// slot once A is done.  Every wait is bounded.
+// Roles (640 threads): warp 0 TMA loads, warp 1 MMA, warps 2..9 scores and output ("X"), warps 10..17 the
+// weighted y and the state ("Y"), warp 18 the output's TMA stores.  The chunk's steps overlap with its
+// neighbours': X forms P of chunk c and then writes the output of c - 1, so that it never waits for a product;
+// Y weighs y of c, publishes S and only then waits for U.  Input tiles pass through a ring of slots in the order
+// x, y, z; hi overwrites y in its slot once A is done, and the output is staged in z's slot.  Every wait is
+// bounded.
+//
+// P takes two multiplications for 32 x 32 blocks off the diagonal (a^(i-j) as a row factor times a column factor,
+// both with exponents >= 0: no overflow for any decay), a table look-up for the four on it, nothing for the rest.
 #include "decay_attn_tc.cuh"
+#include "f32x2.cuh"
 
 namespace pgf {
 namespace da {
@@ -32,23 +38,27 @@ namespace da {
 namespace {
 
 constexpr int C = TC_CHUNK;
-constexpr int THREADS = 576;
+constexpr int THREADS = 640;
 constexpr uint32_t BLK = 16384;   // 128 rows x 64 bf16 columns, 128B swizzle
 constexpr uint32_t TMEM_COLS = 512;
 
-template <int DX, int DZ>
+// NT: bf16 terms of the weighted y.  3 keep the state to float32 accuracy; 2 (2^-17) are enough where the state
+// only feeds D1, which reads it in bf16, and leave room for a fifth slot.
+template <int DX, int DZ, int NT>
 struct Cfg {
   static constexpr uint32_t XB = DX / 64 * BLK, ZB = DZ / 64 * BLK;
   static constexpr uint32_t SLOT = XB > ZB ? XB : ZB;
-  static constexpr int NS = SLOT == BLK ? 8 : 4;
+  static constexpr int NS = SLOT == BLK ? 8 : NT == 2 ? 5 : 4;
+  static constexpr int NA = NS == 8 ? 2 : 1;                            // A buffers
   static constexpr uint32_t RING = NS * SLOT;
   static constexpr uint32_t MID = RING, LO = MID + XB, ZERO = LO + XB;  // ZERO only with 64-wide y
-  static constexpr uint32_t ST = ZERO + (DX == 64 ? BLK : 0);           // S: 128 rows x DZ bf16
-  static constexpr uint32_t TAB = ST + ZB;                              // 256 floats
-  static constexpr uint32_t BARS = TAB + 1024;
+  static constexpr uint32_t ST = NT == 2 ? LO : DX == 64 ? ZERO + BLK : ZERO;  // S: 128 rows x DZ bf16
+  static constexpr uint32_t TAB = ST + ZB;                              // 256 + 32 floats
+  static constexpr uint32_t BARS = TAB + 1152;
   static constexpr uint32_t BYTES = BARS + 256 + 1024;
   // TMEM columns
-  static constexpr uint32_t T_A = 0, T_D1 = 128, T_D2 = 128 + DZ, T_U = 128 + 2 * DZ;
+  static constexpr uint32_t T_A = 0, T_D1 = NA * 128, T_D2 = T_D1 + DZ, T_U = T_D2 + DZ;
+  static_assert(T_U + DZ <= TMEM_COLS && BYTES <= 232448, "fits an SM");
 };
 
 struct Params {
@@ -60,7 +70,7 @@ struct Params {
   float* end;
   float scale, z_scale;
   int64_t L, seg_len;
-  int H, segs, dx, dz, start_t, out_f32;
+  int H, segs, dx, dz, start_t, out_f32, last_too;
   int gx, gy, gz;              // operator heads per tensor head
 };
 
@@ -69,6 +79,19 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, u
       "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
       ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
       : "memory");
+}
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%1, %2, %3, %4}], [%5];"
+               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(src)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
 }
 __device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -79,88 +102,59 @@ __device__ __forceinline__ void lds128(uint32_t a, uint32_t (&v)[4]) {
 __device__ __forceinline__ void sts128(uint32_t a, const uint32_t (&v)[4]) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
 }
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
+}
+__device__ __forceinline__ uint32_t pack2(float2 v) { return pack_bf16(v.x, v.y); }
 
-template <int DX, int DZ, bool STATE_ONLY, bool REV>
-__global__ void __launch_bounds__(THREADS, 1)
-walk_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmY,
-               const __grid_constant__ CUtensorMap tmZ, const Params p) {
-  using G = Cfg<DX, DZ>;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* tab = reinterpret_cast<float*>(base + G::TAB);   // tab[127 + e] = a^e for e >= 0, 0 below
-  const float* pw = tab + 127;                            // a^0 .. a^128
-  uint64_t* full = reinterpret_cast<uint64_t*>(base + G::BARS);
-  uint64_t* empty = full + G::NS;
-  uint64_t* afull = empty + G::NS;
-  uint64_t* pready = afull + 1;
-  uint64_t* ofull = afull + 2;
-  uint64_t* dfree = afull + 3;
-  uint64_t* kready = afull + 4;
-  uint64_t* ufull = afull + 5;
-  uint64_t* sready = afull + 6;
-  uint64_t* aread = afull + 7;    // [4]: both halves of a quarter's rows of A are read
-  uint64_t* sumready = afull + 11;
-  uint32_t* tslot = reinterpret_cast<uint32_t*>(afull + 12);
+// Barriers behind full[NS] and empty[NS].  A and P take turns where there are two A buffers: X may be a chunk
+// ahead of the product that reads P.
+enum { B_A = 0, B_A1, B_P, B_P1, B_O, B_DFREE, B_K, B_U, B_S, B_OSTAGED, B_SUM, B_COUNT };
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int seg = int(blockIdx.x % p.segs);
-  const int64_t bh = blockIdx.x / p.segs, b = bh / p.H;
-  const int h = int(bh % p.H);
-  const int64_t len = row_length(p.lengths, b, p.L);
-  const int64_t s0 = min(len, int64_t(seg) * p.seg_len), s1 = min(len, s0 + p.seg_len);
-  // (the end state of the walk's last piece enters no other piece)
-  const bool idle = STATE_ONLY && seg == (REV ? 0 : p.segs - 1);
-  const int chunks = idle ? 0 : int((s1 - s0 + C - 1) / C);
-  const float l2 = log2_decay(p.log_decay[h]);
+template <int DX, int DZ, int NT, bool STATE_ONLY, bool REV>
+struct Walk {
+  using G = Cfg<DX, DZ, NT>;
+  static constexpr int PER = STATE_ONLY ? 2 : 3;      // tiles of a chunk
+  static constexpr int HC = DZ / 2;                   // columns of one X or Y warp
+  static constexpr int CONV = STATE_ONLY ? 512 : 256; // threads that weigh y
 
-  for (int i = threadIdx.x; i < 256; i += THREADS) tab[i] = i >= 127 ? exp2f(l2 * float(i - 127)) : 0.f;
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < G::NS; ++s) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-    }
-    mbar_init(afull, 1);
-    mbar_init(pready, 8);
-    mbar_init(ofull, 1);
-    mbar_init(dfree, 8);
-    mbar_init(kready, 8);
-    mbar_init(ufull, 1);
-    mbar_init(sready, 8);
-    for (int k = 0; k < 4; ++k) mbar_init(&aread[k], 2);
-    mbar_init(sumready, 8);
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    if (!STATE_ONLY) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmX)) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmY)) : "memory");
-    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmZ)) : "memory");
+  const Params& p;
+  uint8_t* base;
+  uint32_t sbase;
+  float* tab;          // tab[127 + e] = a^e for e >= 0, 0 below
+  const float* pw;     // a^0 .. a^128
+  const float* cf;     // column factors of a block off the diagonal: a^(31-k), from the end a^k
+  uint64_t* full;
+  uint64_t* empty;
+  uint64_t* bars;
+  uint32_t tmem;
+  int warp, lane, seg, h, chunks;
+  int64_t b, bh, len, s0, s1;
+
+  __device__ __forceinline__ int64_t first_token(int c) const { return s0 + int64_t(REV ? chunks - 1 - c : c) * C; }
+  __device__ __forceinline__ int tokens(int c) const { return int(min(int64_t(C), s1 - first_token(c))); }
+  __device__ __forceinline__ uint32_t slot(uint32_t n) const { return n % G::NS; }
+  __device__ __forceinline__ bool wait(int which, int c) const { return mbar_wait_warp(&bars[which], c & 1); }
+  __device__ __forceinline__ bool wait_turn(int which, int c) const {
+    return mbar_wait_warp(&bars[which + c % G::NA], (c / G::NA) & 1);
   }
-  if (DX == 64) {
-    for (uint32_t i = threadIdx.x * 16; i < BLK; i += THREADS * 16)
-      *reinterpret_cast<uint4*>(base + G::ZERO + i) = make_uint4(0, 0, 0, 0);
-    fence_async();
+  __device__ __forceinline__ bool wait_full(uint32_t n) const { return mbar_wait_warp(&full[n % G::NS], (n / G::NS) & 1); }
+  __device__ __forceinline__ void arrive(int which) const {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars[which]);
   }
-  if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tslot)), "r"(TMEM_COLS));
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-  }
-  tc_before();
-  __syncthreads();
-  tc_after();
-  const uint32_t tmem = *tslot;
-  constexpr int PER = STATE_ONLY ? 2 : 3;      // tiles of a chunk
-  auto first_token = [&](int c) { return s0 + int64_t(REV ? chunks - 1 - c : c) * C; };
 
-  if (warp == 0) {
-    // ---- TMA: x, y, z of each chunk through the ring
+  // ---- warp 0
+  __device__ void load(const CUtensorMap* mx, const CUtensorMap* my, const CUtensorMap* mz) const {
     const bool leader = elect_one();
-    bool ok = true;
     uint32_t n = 0;
-    for (int c = 0; c < chunks && ok; ++c) {
+    for (int c = 0; c < chunks; ++c) {
       const int t0 = int(first_token(c));
       for (int k = 3 - PER; k < 3; ++k, ++n) {
-        const uint32_t s = n % G::NS, r = n / G::NS;
-        if (r > 0 && !mbar_wait_warp(&empty[s], (r - 1) & 1)) { ok = false; break; }
+        const uint32_t s = slot(n), r = n / G::NS;
+        if (r > 0 && !mbar_wait_warp(&empty[s], (r - 1) & 1)) return;
         if (leader) {
-          const CUtensorMap* m = k == 0 ? &tmX : k == 1 ? &tmY : &tmZ;
+          const CUtensorMap* m = k == 0 ? mx : k == 1 ? my : mz;
           const int hh = h / (k == 0 ? p.gx : k == 1 ? p.gy : p.gz);
           const int blocks = (k == 2 ? DZ : DX) / 64;
           mbar_expect_tx(&full[s], uint32_t(blocks) * BLK);
@@ -170,310 +164,444 @@ walk_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
         __syncwarp();
       }
     }
-  } else if (warp == 1) {
-    // ---- MMA
+  }
+
+  // ---- warp 1.  A tile's slot is released by the last product that reads it (z's by the output's store), and
+  // the order keeps every wait behind products that do not need it: with two A buffers A of the next chunk goes
+  // first; with five slots D1 comes last, with four it comes before the next A, whose y takes x's slot.
+  __device__ void mma() const {
     const bool leader = elect_one();
     const uint32_t id_a = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(C >> 3) << 17) | (uint32_t(C >> 4) << 24);
     const uint32_t id_d = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (uint32_t(DZ >> 3) << 17) |
                           (uint32_t(C >> 4) << 24);
     const uint32_t id_u = id_d | (1u << 15);
-    const uint32_t sbase = smem_u32(base);
-    uint32_t n = 0;
-    for (int c = 0; c < chunks; ++c, n += PER) {
-      const uint32_t nx = n, ny = n + PER - 2, nz = n + PER - 1;
-      const uint32_t xs = nx % G::NS, ys = ny % G::NS, zs = nz % G::NS;
-      const uint32_t xb = sbase + xs * G::SLOT, yb = sbase + ys * G::SLOT, zb = sbase + zs * G::SLOT;
-      if (!STATE_ONLY) {
-        if (!mbar_wait_warp(&full[xs], (nx / G::NS) & 1)) break;
-        if (!mbar_wait_warp(&full[ys], (ny / G::NS) & 1)) break;
-        tc_after();
-        if (leader) {
+    auto at = [&](uint32_t n) { return sbase + slot(n) * G::SLOT; };
+    auto product_a = [&](int c) {
+      const uint32_t nx = uint32_t(c) * PER, ny = nx + 1;
+      if (!wait_full(nx) || !wait_full(ny)) return false;
+      tc_after();
+      if (leader) {
 #pragma unroll
-          for (int kk = 0; kk < DX / 16; ++kk) {
-            const uint32_t off = (kk >> 2) * BLK + (kk & 3) * 32;
-            umma_bf16(tmem + G::T_A, sdesc(xb + off, 16, 1024), sdesc(yb + off, 16, 1024), id_a, kk > 0);
-          }
-          umma_commit(afull);
+        for (int kk = 0; kk < DX / 16; ++kk) {
+          const uint32_t off = (kk >> 2) * BLK + (kk & 3) * 32;
+          umma_bf16(tmem + G::T_A + uint32_t(c % G::NA) * 128, sdesc(at(nx) + off, 16, 1024), sdesc(at(ny) + off, 16, 1024),
+                    id_a, kk > 0);
         }
-        __syncwarp();
-        if (!mbar_wait_warp(sready, c & 1)) break;
-        if (c > 0 && !mbar_wait_warp(dfree, (c - 1) & 1)) break;
-        tc_after();
-        if (leader) {
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk) {  // 128 rows of S: all of x, or x twice
-            const int xk = kk % (DX / 16);
-            const uint32_t off = (xk >> 2) * BLK + (xk & 3) * 32;
-            umma_bf16(tmem + G::T_D1, sdesc(xb + off, 16, 1024), sdesc(sbase + G::ST + kk * 2048, BLK, 1024), id_d, kk > 0);
-          }
-          umma_commit(&empty[xs]);
-        }
-        __syncwarp();
+        umma_commit(&bars[B_A + c % G::NA]);
       }
-      if (!mbar_wait_warp(&full[zs], (nz / G::NS) & 1)) break;
-      if (!mbar_wait_warp(kready, c & 1)) break;
+      __syncwarp();
+      return true;
+    };
+    auto product_d1 = [&](int c) {
+      const uint32_t nx = uint32_t(c) * PER;
+      if (!wait(B_S, c)) return false;
+      tc_after();
+      if (leader) {
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {  // 128 rows of S: all of x, or x twice
+          const int xk = kk % (DX / 16);
+          const uint32_t off = (xk >> 2) * BLK + (xk & 3) * 32;
+          umma_bf16(tmem + G::T_D1, sdesc(at(nx) + off, 16, 1024), sdesc(sbase + G::ST + kk * 2048, BLK, 1024), id_d, kk > 0);
+        }
+        umma_commit(&empty[slot(nx)]);
+      }
+      __syncwarp();
+      return true;
+    };
+    if (!STATE_ONLY && chunks > 0 && !product_a(0)) return;
+    for (int c = 0; c < chunks; ++c) {
+      const uint32_t ny = uint32_t(c) * PER + PER - 2, nz = ny + 1;
+      const bool more = c + 1 < chunks;
+      if (!STATE_ONLY && G::NA == 2 && more && !product_a(c + 1)) return;
+      if (!wait_full(nz) || !wait(B_K, c)) return;
       tc_after();
       if (leader) {
         // small terms first, so that the accumulator drops the least
         const uint32_t lo = sbase + G::LO, mid = sbase + G::MID;
+        if (NT == 3) {
 #pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-          const uint64_t bd = sdesc(zb + kk * 2048, BLK, 1024);
-          umma_bf16(tmem + G::T_U, sdesc(lo + kk * 2048, BLK, 1024), bd, id_u, kk > 0);
+          for (int kk = 0; kk < 8; ++kk)
+            umma_bf16(tmem + G::T_U, sdesc(lo + kk * 2048, BLK, 1024), sdesc(at(nz) + kk * 2048, BLK, 1024), id_u, kk > 0);
         }
         if (DX == 128) {
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
-            umma_bf16(tmem + G::T_U, sdesc(mid + kk * 2048, BLK, 1024), sdesc(zb + kk * 2048, BLK, 1024), id_u, 1);
+            umma_bf16(tmem + G::T_U, sdesc(mid + kk * 2048, BLK, 1024), sdesc(at(nz) + kk * 2048, BLK, 1024), id_u,
+                      NT == 3 || kk > 0);
         }
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
-          umma_bf16(tmem + G::T_U, sdesc(yb + kk * 2048, DX == 64 ? mid - yb : BLK, 1024), sdesc(zb + kk * 2048, BLK, 1024),
-                    id_u, 1);
-        umma_commit(ufull);
-        umma_commit(&empty[ys]);
-        if (STATE_ONLY) umma_commit(&empty[zs]);
+          umma_bf16(tmem + G::T_U, sdesc(at(ny) + kk * 2048, DX == 64 ? mid - at(ny) : BLK, 1024),
+                    sdesc(at(nz) + kk * 2048, BLK, 1024), id_u, NT == 3 || DX == 128 || kk > 0);
+        umma_commit(&bars[B_U]);
+        umma_commit(&empty[slot(ny)]);
+        if (STATE_ONLY) umma_commit(&empty[slot(nz)]);
       }
       __syncwarp();
-      if (!STATE_ONLY) {
-        if (!mbar_wait_warp(pready, c & 1)) break;
-        tc_after();
-        if (leader) {
+      if (STATE_ONLY) continue;
+      if (!wait_turn(B_P, c)) return;
+      if (c > 0 && !wait(B_DFREE, c - 1)) return;
+      if (G::NS == 4 && !product_d1(c)) return;
+      tc_after();
+      if (leader) {
+        const uint32_t pa = tmem + G::T_A + uint32_t(c % G::NA) * 128;
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
-            umma_bf16_ta(tmem + G::T_D2, tmem + G::T_A + 8 * kk, sdesc(zb + kk * 2048, BLK, 1024), id_d, kk > 0);
-          umma_commit(ofull);
-          umma_commit(&empty[zs]);
-        }
+        for (int kk = 0; kk < 8; ++kk)  // P of columns 0..63 and 64..127 lies where each half of A was
+          umma_bf16_ta(tmem + G::T_D2, pa + (kk >> 2) * 64 + (kk & 3) * 8, sdesc(at(nz) + kk * 2048, BLK, 1024), id_d, kk > 0);
+        if (G::NS == 4) umma_commit(&bars[B_O]);
+      }
+      __syncwarp();
+      if (G::NA == 1 && more && !product_a(c + 1)) return;
+      if (G::NS != 4) {
+        if (!product_d1(c)) return;
+        if (leader) umma_commit(&bars[B_O]);
         __syncwarp();
       }
     }
-  } else if (warp < 10) {
-    if (!STATE_ONLY) {
-      // ---- scores and output: row i of the chunk is TMEM lane i
-      const int q = warp & 3, half = (warp - 2) >> 2, i = q * 32 + lane;
-      const uint32_t row = uint32_t(q * 32) << 16;
-      const int64_t seg0 = int64_t(seg) * p.seg_len;
-      const int64_t pitch = int64_t(p.H) * p.dz;
-      const int64_t obase = (b * p.L * p.H + h) * p.dz;
-      for (int c = 0; c < chunks; ++c) {
-        const int64_t t0 = first_token(c);
-        const int n = int(min(int64_t(C), s1 - t0));
-        if (!mbar_wait_warp(afull, c & 1)) break;
-        tc_after();
-        {
-          uint32_t r0[32], r1[32];
-          tmem_ld32_nowait(tmem + G::T_A + row + half * 64, r0);
-          tmem_ld32_nowait(tmem + G::T_A + row + half * 64 + 32, r1);
-          tmem_wait_ld();
-          tc_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&aread[q]);
-          if (!mbar_wait_warp(&aread[q], c & 1)) break;  // both halves are read before P goes over them
-          tc_after();
-          uint32_t pk[16];
-          const int j0 = half * 64;
-          const float* t = tab + (REV ? 127 - i + j0 : 127 + i - j0);
+  }
+
+  // ---- X: row i of the chunk is TMEM lane i
+  __device__ __forceinline__ bool scores(int c) const {
+    const int q = warp & 3, half = (warp - 2) >> 2, i = q * 32 + lane;
+    const uint32_t ta = tmem + G::T_A + uint32_t(c % G::NA) * 128 + (uint32_t(q * 32) << 16) + half * 64;
+    const int n = tokens(c);
+    if (!wait_turn(B_A, c)) return false;
+    tc_after();
 #pragma unroll
-          for (int g = 0; g < 2; ++g) {
+    for (int g = 0; g < 2; ++g) {
+      const int cb = half * 2 + g;      // block of 32 columns
+      uint32_t pk[16];
+      if (REV ? cb < q : cb > q) {
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              float v[2];
+        for (int k = 0; k < 16; ++k) pk[k] = 0;
+      } else {
+        uint32_t r[32];
+        tmem_ld32(ta + g * 32, r);
+        const int lim = REV ? n - 32 * cb : 32;   // columns past the length
+        if (cb != q && lim >= 32) {
+          const float rf = REV ? pw[32 * cb - i] : pw[i - 32 * cb - 31];
+          const float2 rf2 = make_float2(rf, rf);
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                const int j = g * 32 + 2 * k + e;
-                const float w = REV ? t[j] : t[-j];
-                const float a = __uint_as_float(g ? r1[2 * k + e] : r0[2 * k + e]);
-                const bool in = REV ? j0 + j >= i && j0 + j < n : j0 + j <= i;
-                v[e] = in ? a * w : 0.f;
-              }
-              pk[k] = pack_bf16(v[0], v[1]);
-            }
-            tmem_st16(tmem + G::T_A + row + half * 32 + g * 16, pk);
+          for (int k = 0; k < 8; ++k) {
+            const float4 w = *reinterpret_cast<const float4*>(cf + 4 * k);
+            const float2 lo = __fmul2_rn(make_float2(w.x, w.y), rf2), hi = __fmul2_rn(make_float2(w.z, w.w), rf2);
+            pk[2 * k] = pack2(__fmul2_rn(make_float2(__uint_as_float(r[4 * k]), __uint_as_float(r[4 * k + 1])), lo));
+            pk[2 * k + 1] = pack2(__fmul2_rn(make_float2(__uint_as_float(r[4 * k + 2]), __uint_as_float(r[4 * k + 3])), hi));
           }
-          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-          tc_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(pready);
-        }
-        if (!mbar_wait_warp(ofull, c & 1)) break;
-        tc_after();
-        const float w = i < n ? p.scale * pw[REV ? n - 1 - i : i + 1] : 0.f, w2 = p.scale * p.z_scale;
-        const bool on = t0 + i < p.L && t0 + i < seg0 + p.seg_len;
-        constexpr int HC = DZ / 2;              // columns of this warp
+        } else {
+          const float* t = tab + 127 + (REV ? 32 * cb - i : i - 32 * cb);
 #pragma unroll
-        for (int g = 0; g < HC / 32; ++g) {
-          uint32_t d1[32], d2[32];
-          const int col = half * HC + g * 32;
-          tmem_ld32_nowait(tmem + G::T_D1 + row + col, d1);
-          tmem_ld32_nowait(tmem + G::T_D2 + row + col, d2);
-          tmem_wait_ld();
-          if (g == HC / 32 - 1) {
-            tc_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(dfree);
-          }
-          float o[32];
+          for (int k = 0; k < 16; ++k) {
+            float v[2];
 #pragma unroll
-          for (int k = 0; k < 32; ++k)
-            o[k] = i < n ? fmaf(w, __uint_as_float(d1[k]), w2 * __uint_as_float(d2[k])) : 0.f;
-          if (on) {
-            const int64_t at = obase + (t0 + i) * pitch + col;
-            if (p.out_f32) {
-              float* dst = static_cast<float*>(p.out) + at;
-#pragma unroll
-              for (int k = 0; k < 8; ++k)
-                if (col + 4 * k < p.dz)
-                  *reinterpret_cast<float4*>(dst + 4 * k) = make_float4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
-            } else {
-              __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + at;
-#pragma unroll
-              for (int k = 0; k < 4; ++k)
-                if (col + 8 * k < p.dz)
-                  *reinterpret_cast<uint4*>(dst + 8 * k) =
-                      make_uint4(pack_bf16(o[8 * k], o[8 * k + 1]), pack_bf16(o[8 * k + 2], o[8 * k + 3]),
-                                 pack_bf16(o[8 * k + 4], o[8 * k + 5]), pack_bf16(o[8 * k + 6], o[8 * k + 7]));
+            for (int e = 0; e < 2; ++e) {
+              const int j = 2 * k + e;
+              const bool in = REV ? 32 * cb + j >= i && j < lim : 32 * cb + j <= i;
+              v[e] = in ? __uint_as_float(r[j]) * t[REV ? j : -j] : 0.f;
             }
+            pk[k] = pack_bf16(v[0], v[1]);
           }
         }
       }
-      // whole chunks past the length are zeros
-      const int64_t z0 = max(seg0, s0 + int64_t(chunks) * C), z1 = min(p.L, seg0 + p.seg_len);
-      const int per = p.dz / 8;
-      for (int64_t k = threadIdx.x - 64; k < (z1 - z0) * per; k += 256) {
-        const int64_t at = obase + (z0 + k / per) * pitch + (k % per) * 8;
-        const uint4 z = make_uint4(0, 0, 0, 0);
-        if (p.out_f32) {
-          uint4* dst = reinterpret_cast<uint4*>(static_cast<float*>(p.out) + at);
-          dst[0] = z;
-          dst[1] = z;
-        } else {
-          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + at) = z;
+      tmem_st16(ta + g * 16, pk);
+    }
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+    tc_before();
+    arrive(B_P + c % G::NA);
+    return true;
+  }
+
+  __device__ __forceinline__ bool output(int c) const {
+    const int q = warp & 3, half = (warp - 2) >> 2, i = q * 32 + lane;
+    const uint32_t row = uint32_t(q * 32) << 16;
+    const int64_t t0 = first_token(c);
+    const int n = tokens(c);
+    if (!wait(B_O, c)) return false;
+    tc_after();
+    const float w = i < n ? p.scale * pw[REV ? n - 1 - i : i + 1] : 0.f, w2 = p.scale * p.z_scale;
+    const uint32_t stage = sbase + slot(uint32_t(c) * PER + 2) * G::SLOT;
+#pragma unroll
+    for (int g = 0; g < HC / 32; ++g) {
+      uint32_t d1[32], d2[32];
+      const int col = half * HC + g * 32;
+      tmem_ld32_nowait(tmem + G::T_D1 + row + col, d1);
+      tmem_ld32_nowait(tmem + G::T_D2 + row + col, d2);
+      tmem_wait_ld();
+      if (g == HC / 32 - 1) {
+        tc_before();
+        arrive(B_DFREE);
+      }
+      float2 o[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        o[k] = __ffma2_rn(make_float2(w, w), make_float2(__uint_as_float(d1[2 * k]), __uint_as_float(d1[2 * k + 1])),
+                          __fmul2_rn(make_float2(w2, w2), make_float2(__uint_as_float(d2[2 * k]), __uint_as_float(d2[2 * k + 1]))));
+        if (i >= n) o[k] = make_float2(0.f, 0.f);
+      }
+      if (p.out_f32) {
+        if (t0 + i < p.L) {
+          float* dst = static_cast<float*>(p.out) + ((b * p.L + t0 + i) * p.H + h) * p.dz + col;
+#pragma unroll
+          for (int k = 0; k < 8; ++k)
+            if (col + 4 * k < p.dz)
+              *reinterpret_cast<float4*>(dst + 4 * k) = make_float4(o[2 * k].x, o[2 * k].y, o[2 * k + 1].x, o[2 * k + 1].y);
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t v[4] = {pack2(o[4 * k]), pack2(o[4 * k + 1]), pack2(o[4 * k + 2]), pack2(o[4 * k + 3])};
+          // 128-wide: a 128-byte row of the half's block; 64-wide: a 64-byte row of the warp's own 2 KB
+          const uint32_t a = DZ == 128 ? half * BLK + uint32_t(i) * 128 + (uint32_t((g * 4 + k) ^ (i & 7)) << 4)
+                                       : uint32_t(q * 2 + half) * 2048 + uint32_t(lane) * 64 + (uint32_t(k ^ ((lane >> 1) & 3)) << 4);
+          sts128(stage + a, v);
         }
       }
     }
-  } else {
-    // ---- the weighted y and the state: lane i of TMEM is row i of the state (64-wide y: row i % 64)
+    fence_async();
+    arrive(B_OSTAGED);
+    return true;
+  }
+
+  // ---- X: whole chunks past the length are zeros
+  __device__ void zeros() const {
+    const int64_t seg0 = int64_t(seg) * p.seg_len;
+    const int64_t z0 = max(seg0, s0 + int64_t(chunks) * C), z1 = min(p.L, seg0 + p.seg_len);
+    const int per = p.dz / 8;
+    for (int64_t k = int(threadIdx.x) - 64; k < (z1 - z0) * per; k += 256) {
+      const int64_t at = ((b * p.L + z0 + k / per) * p.H + h) * p.dz + (k % per) * 8;
+      const uint4 z = make_uint4(0, 0, 0, 0);
+      if (p.out_f32) {
+        uint4* dst = reinterpret_cast<uint4*>(static_cast<float*>(p.out) + at);
+        dst[0] = z;
+        dst[1] = z;
+      } else {
+        *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + at) = z;
+      }
+    }
+  }
+
+  // ---- warp 18: stores the staged output and hands z's slot back
+  __device__ void store(const CUtensorMap* mo) const {
+    for (int c = 0; c < chunks; ++c) {
+      const uint32_t nz = uint32_t(c) * PER + 2;
+      if (!wait(B_OSTAGED, c)) return;
+      if (lane == 0) {
+        if (!p.out_f32) {
+          const int t0 = int(first_token(c));
+          const uint32_t src = sbase + slot(nz) * G::SLOT;
+          for (int k = 0; k < 8; ++k) {
+            const int q = k >> 1, half = k & 1;
+            if (t0 + q * 32 < p.L && half * HC < p.dz)
+              tma_store_4d(mo, src + (DZ == 128 ? half * BLK + q * 4096 : k * 2048), half * HC, h, t0 + q * 32, int(b));
+          }
+          asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+          asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+        }
+        mbar_arrive(&empty[slot(nz)]);
+      }
+      __syncwarp();
+    }
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+
+  // ---- the weighted y of chunk c as bf16 terms (this thread's 16-byte pieces); z's rows past the length
+  __device__ __forceinline__ bool weigh(int c, int tid) const {
+    const uint32_t ny = uint32_t(c) * PER + PER - 2, nz = ny + 1;
+    const int n = tokens(c);
+    const uint32_t yb = sbase + slot(ny) * G::SLOT;
+    if (STATE_ONLY ? !wait_full(ny) : !wait_turn(B_A, c)) return false;
+#pragma unroll
+    for (int k = 0; k < DX / 64 * 1024 / CONV; ++k) {
+      const uint32_t u = uint32_t(tid + CONV * k), off = u * 16;
+      const int j = int(u >> 3) & 127;       // token
+      uint32_t v[4], hi[4], mid[4], lo[4];
+      lds128(yb + off, v);
+      if (j >= n) v[0] = v[1] = v[2] = v[3] = 0;  // what lies there may be anything
+      const float w = j < n ? pw[REV ? j + 1 : n - 1 - j] : 0.f;
+      const float2 w2 = make_float2(w, w), minus = make_float2(-1.f, -1.f);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float2 a = __fmul2_rn(unpack2(v[e]), w2);
+        hi[e] = pack2(a);
+        a = __ffma2_rn(unpack2(hi[e]), minus, a);
+        mid[e] = pack2(a);
+        if (NT == 3) {
+          a = __ffma2_rn(unpack2(mid[e]), minus, a);
+          lo[e] = pack2(a);
+        }
+      }
+      sts128(yb + off, hi);
+      sts128(sbase + G::MID + off, mid);
+      if (NT == 3) sts128(sbase + G::LO + off, lo);
+    }
+    if (n < C) {
+      if (!wait_full(nz)) return false;
+      const uint32_t zero[4] = {0, 0, 0, 0};
+      for (uint32_t u = uint32_t(tid); u < G::ZB / 16; u += CONV)
+        if ((int(u >> 3) & 127) >= n) sts128(sbase + slot(nz) * G::SLOT + u * 16, zero);
+    }
+    fence_async();
+    arrive(B_K);
+    return true;
+  }
+
+  // ---- Y: lane i of TMEM is row i of the state (64-wide y: row i % 64)
+  __device__ void state() const {
     const int q = warp & 3, half = (warp - 10) >> 2, i = q * 32 + lane;
     const int tid = int(threadIdx.x) - 320;
     const uint32_t row = uint32_t(q * 32) << 16;
-    const uint32_t sbase = smem_u32(base);
-    constexpr int HC = DZ / 2;
     const int64_t n_state = int64_t(p.dx) * p.dz;
-    float s[HC];
+    float2 s[HC / 2];
     {
       const float* st = p.start && !STATE_ONLY ? p.start + bh * p.start_stride + int64_t(seg) * n_state : nullptr;
 #pragma unroll
       for (int k = 0; k < HC; ++k) {
         const int c = half * HC + k;
-        s[k] = st && i < p.dx && i < DX && c < p.dz ? (p.start_t ? st[int64_t(c) * p.dx + i] : st[int64_t(i) * p.dz + c]) : 0.f;
+        const float v = st && i < p.dx && i < DX && c < p.dz
+                            ? (p.start_t ? st[int64_t(c) * p.dx + i] : st[int64_t(i) * p.dz + c]) : 0.f;
+        if (k & 1) s[k / 2].y = v;
+        else s[k / 2].x = v;
       }
     }
-    auto publish = [&]() {  // S as the bf16 operand of D1
+    for (int c = 0; c < chunks; ++c) {
+      // STATE_ONLY: the terms' buffers are free again (this warp has waited for U of c - 1)
+      if (!weigh(c, STATE_ONLY ? tid + 256 : tid)) return;
+      if (!STATE_ONLY) {
+        // S as the bf16 operand of D1, once D1 of the chunk before has read its own
+        if (c > 0 && !wait(B_O, c - 1)) return;
 #pragma unroll
-      for (int k = 0; k < HC / 8; ++k) {
-        const uint32_t w[4] = {pack_bf16(s[8 * k], s[8 * k + 1]), pack_bf16(s[8 * k + 2], s[8 * k + 3]),
-                               pack_bf16(s[8 * k + 4], s[8 * k + 5]), pack_bf16(s[8 * k + 6], s[8 * k + 7])};
-        const int ch = half * (HC / 8) + k;  // 16-byte chunk of the row
-        sts128(sbase + G::ST + uint32_t(ch >> 3) * BLK + uint32_t(i) * 128 + (uint32_t((ch & 7) ^ (i & 7)) << 4), w);
-      }
-      fence_async();
-      tc_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(sready);
-    };
-    if (!STATE_ONLY && chunks > 0) publish();
-    uint32_t n_tile = 0;
-    bool ok = true;
-    for (int c = 0; c < chunks; ++c, n_tile += PER) {
-      const uint32_t ny = n_tile + PER - 2, nz = n_tile + PER - 1;
-      const uint32_t ys = ny % G::NS, zs = nz % G::NS;
-      const int64_t t0 = first_token(c);
-      const int n = int(min(int64_t(C), s1 - t0));
-      if (STATE_ONLY) {
-        if (!mbar_wait_warp(&full[ys], (ny / G::NS) & 1)) { ok = false; break; }
-      } else if (!mbar_wait_warp(afull, c & 1)) {
-        ok = false;
-        break;
-      }
-#pragma unroll
-      for (int k = 0; k < DX / 64 * 4; ++k) {
-        const uint32_t u = uint32_t(tid + 256 * k), off = u * 16;
-        const int j = int(u >> 3) & 127;       // token
-        uint32_t v[4], hi[4], mid[4], lo[4];
-        lds128(sbase + ys * G::SLOT + off, v);
-        const float w = j < n ? pw[REV ? j + 1 : n - 1 - j] : 0.f;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float a = __uint_as_float(v[e] << 16) * w, d = __uint_as_float(v[e] & 0xFFFF0000u) * w;
-          if (j >= n) a = d = 0.f;              // what lies there may be anything
-          hi[e] = pack_bf16(a, d);
-          a -= __uint_as_float(hi[e] << 16);
-          d -= __uint_as_float(hi[e] & 0xFFFF0000u);
-          mid[e] = pack_bf16(a, d);
-          a -= __uint_as_float(mid[e] << 16);
-          d -= __uint_as_float(mid[e] & 0xFFFF0000u);
-          lo[e] = pack_bf16(a, d);
+        for (int k = 0; k < HC / 8; ++k) {
+          const uint32_t w[4] = {pack2(s[4 * k]), pack2(s[4 * k + 1]), pack2(s[4 * k + 2]), pack2(s[4 * k + 3])};
+          const int ch = half * (HC / 8) + k;  // 16-byte piece of the row
+          sts128(sbase + G::ST + uint32_t(ch >> 3) * BLK + uint32_t(i) * 128 + (uint32_t((ch & 7) ^ (i & 7)) << 4), w);
         }
-        sts128(sbase + ys * G::SLOT + off, hi);
-        sts128(sbase + G::MID + off, mid);
-        sts128(sbase + G::LO + off, lo);
+        fence_async();
+        arrive(B_S);
       }
-      if (n < C) {
-        if (!mbar_wait_warp(&full[zs], (nz / G::NS) & 1)) { ok = false; break; }
-        const uint32_t zero[4] = {0, 0, 0, 0};
-        for (uint32_t u = uint32_t(tid); u < G::ZB / 16; u += 256)
-          if ((int(u >> 3) & 127) >= n) sts128(sbase + zs * G::SLOT + u * 16, zero);
-      }
-      fence_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(kready);
-      if (!mbar_wait_warp(ufull, c & 1)) { ok = false; break; }
+      if (!wait(B_U, c)) return;
       tc_after();
-      const float an = pw[n];
+      const float an = pw[tokens(c)];
+      const float2 an2 = make_float2(an, an), zs = make_float2(p.z_scale, p.z_scale);
 #pragma unroll
-      for (int g = 0; g < HC / 32; ++g) {
-        uint32_t u[32];
-        tmem_ld32(tmem + G::T_U + row + half * HC + g * 32, u);
+      for (int g = 0; g < HC / 16; ++g) {
+        uint32_t u[16];
+        tmem_ld16_nowait(tmem + G::T_U + row + half * HC + g * 16, u);
+        tmem_wait_ld();
 #pragma unroll
-        for (int k = 0; k < 32; ++k) s[g * 32 + k] = fmaf(an, s[g * 32 + k], p.z_scale * __uint_as_float(u[k]));
+        for (int k = 0; k < 8; ++k)
+          s[g * 8 + k] = __ffma2_rn(an2, s[g * 8 + k],
+                                    __fmul2_rn(zs, make_float2(__uint_as_float(u[2 * k]), __uint_as_float(u[2 * k + 1]))));
       }
-      if (STATE_ONLY) tc_before();
-      else if (c + 1 < chunks) publish();
+      tc_before();
     }
     // the state leaves: a piece's own (STATE_ONLY) or the whole walk's
     float* end = nullptr;
-    if (STATE_ONLY) end = idle ? nullptr : const_cast<float*>(p.start) + bh * p.start_stride + int64_t(seg) * n_state;
+    if (STATE_ONLY) end = chunks > 0 || p.last_too || seg != (REV ? 0 : p.segs - 1)
+                              ? const_cast<float*>(p.start) + bh * p.start_stride + int64_t(seg) * n_state : nullptr;
     else if (p.end && seg == (REV ? 0 : p.segs - 1)) end = p.end + bh * n_state;
-    if (end && ok) {
-      if (DX == 64) {
-        // rows 64..127 hold the middle terms' part
-        float* sum = reinterpret_cast<float*>(base + G::ST);
-        if (i >= 64) {
+    if (!end) return;
+    if (DX == 64) {
+      // rows 64..127 hold the middle terms' part; the ring is done with
+      float2* sum = reinterpret_cast<float2*>(base + G::MID);
+      static_assert(DX != 64 || G::MID + 64 * DZ * 4 <= G::TAB, "the sum fits");
+      if (i >= 64) {
 #pragma unroll
-          for (int k = 0; k < HC; ++k) sum[(i - 64) + (half * HC + k) * 64] = s[k];
-        }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(sumready);
-        if (!mbar_wait_warp(sumready, 0)) ok = false;
-        if (i < 64) {
-#pragma unroll
-          for (int k = 0; k < HC; ++k) s[k] += sum[i + (half * HC + k) * 64];
-        }
+        for (int k = 0; k < HC / 2; ++k) sum[(i - 64) + (half * (HC / 2) + k) * 64] = s[k];
       }
-      if (ok && i < DX && i < p.dx) {
+      arrive(B_SUM);
+      if (!mbar_wait_warp(&bars[B_SUM], 0)) return;
+      if (i < 64) {
 #pragma unroll
-        for (int k = 0; k < HC; k += 4) {
-          const int c = half * HC + k;
-          if (c < p.dz) *reinterpret_cast<float4*>(end + int64_t(i) * p.dz + c) = make_float4(s[k], s[k + 1], s[k + 2], s[k + 3]);
-        }
+        for (int k = 0; k < HC / 2; ++k) s[k] = __fadd2_rn(s[k], sum[i + (half * (HC / 2) + k) * 64]);
+      }
+    }
+    if (i < DX && i < p.dx) {
+#pragma unroll
+      for (int k = 0; k < HC; k += 4) {
+        const int c = half * HC + k;
+        if (c < p.dz)
+          *reinterpret_cast<float4*>(end + int64_t(i) * p.dz + c) = make_float4(s[k / 2].x, s[k / 2].y, s[k / 2 + 1].x, s[k / 2 + 1].y);
       }
     }
   }
+};
+
+template <int DX, int DZ, int NT, bool STATE_ONLY, bool REV>
+__global__ void __launch_bounds__(THREADS, 1)
+walk_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmY,
+               const __grid_constant__ CUtensorMap tmZ, const __grid_constant__ CUtensorMap tmO, const Params p) {
+  using W = Walk<DX, DZ, NT, STATE_ONLY, REV>;
+  using G = typename W::G;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* tab = reinterpret_cast<float*>(base + G::TAB);
+  uint64_t* full = reinterpret_cast<uint64_t*>(base + G::BARS);
+  uint64_t* bars = full + 2 * G::NS;
+  static_assert((2 * G::NS + B_COUNT) * 8 + 4 <= 256, "barriers fit");
+  uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + B_COUNT);
+  W w{p, base, smem_u32(base), tab, tab + 127, tab + 256, full, full + G::NS, bars, 0u, int(threadIdx.x >> 5),
+      int(threadIdx.x & 31)};
+  w.seg = int(blockIdx.x % p.segs);
+  w.bh = blockIdx.x / p.segs;
+  w.b = w.bh / p.H;
+  w.h = int(w.bh % p.H);
+  w.len = row_length(p.lengths, w.b, p.L);
+  w.s0 = min(w.len, int64_t(w.seg) * p.seg_len);
+  w.s1 = min(w.len, w.s0 + p.seg_len);
+  // the end state of the walk's last piece enters no other piece
+  const bool idle = STATE_ONLY && !p.last_too && w.seg == (REV ? 0 : p.segs - 1);
+  w.chunks = idle ? 0 : int((w.s1 - w.s0 + C - 1) / C);
+
+  const float l2 = log2_decay(p.log_decay[w.h]);
+  for (int i = threadIdx.x; i < 256; i += THREADS) tab[i] = i >= 127 ? exp2f(l2 * float(i - 127)) : 0.f;
+  if (threadIdx.x < 32) tab[256 + threadIdx.x] = exp2f(l2 * float(REV ? threadIdx.x : 31 - threadIdx.x));
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2 * G::NS; ++s) mbar_init(&full[s], 1);
+    for (int k = 0; k < B_COUNT; ++k) mbar_init(&bars[k], k == B_A || k == B_A1 || k == B_O || k == B_U ? 1 : k == B_K ? W::CONV / 32 : 8);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    if (!STATE_ONLY) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmX)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmY)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmZ)) : "memory");
+  }
+  if (DX == 64 && NT == 3) {
+    for (uint32_t i = threadIdx.x * 16; i < BLK; i += THREADS * 16)
+      *reinterpret_cast<uint4*>(base + G::ZERO + i) = make_uint4(0, 0, 0, 0);
+    fence_async();
+  }
+  if (w.warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tslot)), "r"(TMEM_COLS));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
   tc_before();
   __syncthreads();
-  if (warp == 0)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS));
+  tc_after();
+  w.tmem = *tslot;
+
+  if (w.warp == 0) {
+    w.load(&tmX, &tmY, &tmZ);
+  } else if (w.warp == 1) {
+    w.mma();
+  } else if (w.warp < 10) {
+    if (STATE_ONLY) {
+      for (int c = 0; c < w.chunks; ++c) {
+        if (c > 0 && !w.wait(B_U, c - 1)) break;
+        if (!w.weigh(c, int(threadIdx.x) - 64)) break;
+      }
+    } else {
+      bool ok = true;
+      for (int c = 0; c < w.chunks && ok; ++c) ok = w.scores(c) && (c == 0 || w.output(c - 1));
+      if (ok && w.chunks > 0) w.output(w.chunks - 1);
+      w.zeros();
+    }
+  } else if (w.warp < 18) {
+    w.state();
+  } else if (w.warp == 18) {
+    if (!STATE_ONLY) w.store(&tmO);
+  }
+  tc_before();
+  __syncthreads();
+  if (w.warp == 0)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(w.tmem), "r"(TMEM_COLS));
 }
 
 // (D, heads, L, B) with a box of 64 columns x 128 tokens of one head; zeros outside.
@@ -495,13 +623,26 @@ bool fits(const Tensor& t, int64_t B, int64_t L) {
   return t.d % 8 == 0 && t.d <= 128 && aligned(t.p, 16) && ok(t.heads, t.s.head) && ok(L, t.s.token) && ok(B, t.s.batch);
 }
 
-template <int DX, int DZ, bool STATE_ONLY, bool REV>
+// The output as (D, H, L, B), a box of 32 tokens and one X warp's columns, in the swizzle that it is staged in.
+bool make_store_map(CUtensorMap* m, const Job& j, int cols) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t d = cuuint64_t(j.z.d);
+  cuuint64_t dims[4] = {d, cuuint64_t(j.H), cuuint64_t(j.L), cuuint64_t(j.B)};
+  cuuint64_t st[3] = {d * 2, d * 2 * j.H, d * 2 * j.H * cuuint64_t(j.L)};
+  cuuint32_t box[4] = {cuuint32_t(cols), 1, 32, 1}, es[4] = {1, 1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, j.out, dims, st, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DX, int DZ, int NT, bool STATE_ONLY, bool REV>
 int launch(const Job& j, cudaStream_t s) {
   static int limit = 0;
-  using G = Cfg<DX, DZ>;
-  CUtensorMap mx = {}, my, mz;
+  using G = Cfg<DX, DZ, NT>;
+  CUtensorMap mx = {}, my, mz, mo = {};
   if ((!STATE_ONLY && !make_tensor_map(&mx, j.x, j.B, j.L)) || !make_tensor_map(&my, j.y, j.B, j.L) ||
-      !make_tensor_map(&mz, j.z, j.B, j.L)) {
+      !make_tensor_map(&mz, j.z, j.B, j.L) || (!STATE_ONLY && !j.out_f32 && !make_store_map(&mo, j, DZ / 2))) {
     set_error("decay_attn: tensor map");
     return PGF_ERR_CUDA;
   }
@@ -522,28 +663,30 @@ int launch(const Job& j, cudaStream_t s) {
   p.dz = j.z.d;
   p.start_t = j.start_t;
   p.out_f32 = j.out_f32;
+  p.last_too = j.last_too;
   p.gx = STATE_ONLY ? 1 : j.H / j.x.heads;
   p.gy = j.H / j.y.heads;
   p.gz = j.H / j.z.heads;
-  PGF_CUDA(ensure_dynamic_smem(walk_tc_kernel<DX, DZ, STATE_ONLY, REV>, G::BYTES, limit));
-  walk_tc_kernel<DX, DZ, STATE_ONLY, REV><<<unsigned(j.B * j.H * j.segs), THREADS, G::BYTES, s>>>(mx, my, mz, p);
+  PGF_CUDA(ensure_dynamic_smem(walk_tc_kernel<DX, DZ, NT, STATE_ONLY, REV>, G::BYTES, limit));
+  walk_tc_kernel<DX, DZ, NT, STATE_ONLY, REV><<<unsigned(j.B * j.H * j.segs), THREADS, G::BYTES, s>>>(mx, my, mz, mo, p);
   PGF_LAUNCH_CHECK();
   return PGF_OK;
 }
 
-template <bool STATE_ONLY, bool REV>
+template <int NT, bool STATE_ONLY, bool REV>
 int dispatch(const Job& j, cudaStream_t s) {
   if (j.y.d <= 64)
-    return j.z.d <= 64 ? launch<64, 64, STATE_ONLY, REV>(j, s) : launch<64, 128, STATE_ONLY, REV>(j, s);
-  return j.z.d <= 64 ? launch<128, 64, STATE_ONLY, REV>(j, s) : launch<128, 128, STATE_ONLY, REV>(j, s);
+    return j.z.d <= 64 ? launch<64, 64, NT, STATE_ONLY, REV>(j, s) : launch<64, 128, NT, STATE_ONLY, REV>(j, s);
+  return j.z.d <= 64 ? launch<128, 64, NT, STATE_ONLY, REV>(j, s) : launch<128, 128, NT, STATE_ONLY, REV>(j, s);
 }
 
 }  // namespace
 
 bool tc_fits(const Tensor& t, int64_t B, int64_t L) { return fits(t, B, L); }
 int tc_walk(const Job& j, bool state_only, cudaStream_t s) {
-  if (state_only) return j.rev ? dispatch<true, true>(j, s) : dispatch<true, false>(j, s);
-  return j.rev ? dispatch<false, true>(j, s) : dispatch<false, false>(j, s);
+  if (state_only) return j.rev ? dispatch<3, true, true>(j, s) : dispatch<3, true, false>(j, s);
+  if (j.end) return j.rev ? dispatch<3, false, true>(j, s) : dispatch<3, false, false>(j, s);
+  return j.rev ? dispatch<2, false, true>(j, s) : dispatch<2, false, false>(j, s);
 }
 
 }  // namespace da
