@@ -22,9 +22,9 @@
 //
 // Roles (640 threads): warp 0 TMA loads, warp 1 MMA, warps 2..9 scores and output ("X"), warps 10..17 the
 // weighted y and the state ("Y"), warp 18 the output's TMA stores.  The chunk's steps overlap with its
-// neighbours': X forms P of chunk c and then writes the output of c - 1, so that it never waits for a product;
+// neighbours': X forms P of chunk c beside the output of c - 1, so that it seldom waits for a product;
 // Y weighs y of c, publishes S and only then waits for U.  Input tiles pass through a ring of slots in the order
-// x, y, z; hi overwrites y in its slot once A is done, and the output is staged in z's slot.  Every wait is
+// y, x, z; hi overwrites y in its slot once A is done, and the output is staged in z's slot.  Every wait is
 // bounded.
 //
 // P takes two multiplications for 32 x 32 blocks off the diagonal (a^(i-j) as a row factor times a column factor,
@@ -107,6 +107,29 @@ __device__ __forceinline__ float2 unpack2(uint32_t v) {
 }
 __device__ __forceinline__ uint32_t pack2(float2 v) { return pack_bf16(v.x, v.y); }
 
+// Bounded warp-wide wait: one try before the clock is read (most waits find their phase complete).
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  if (__all_sync(0xffffffffu, done)) return true;
+  return mbar_wait_warp(bar, parity);
+}
+// A matrix descriptor (sdesc) whose start moves by whole 16-byte units: the address field is the low 14 bits
+// and shared memory ends below 2^18, so a step never carries out of it.
+struct Desc {
+  uint32_t lo, hi;
+  __device__ __forceinline__ Desc(uint32_t saddr, uint32_t lbo) {
+    const uint64_t d = sdesc(saddr, lbo, 1024);
+    lo = uint32_t(d);
+    hi = uint32_t(d >> 32);
+  }
+  __device__ __forceinline__ uint64_t at(uint32_t bytes) const { return uint64_t(hi) << 32 | (lo + (bytes >> 4)); }
+};
+
 // Barriers behind full[NS] and empty[NS].  A and P take turns where there are two A buffers: X may be a chunk
 // ahead of the product that reads P.
 enum { B_A = 0, B_A1, B_P, B_P1, B_O, B_DFREE, B_K, B_U, B_S, B_OSTAGED, B_SUM, B_COUNT };
@@ -134,15 +157,20 @@ struct Walk {
   __device__ __forceinline__ int64_t first_token(int c) const { return s0 + int64_t(REV ? chunks - 1 - c : c) * C; }
   __device__ __forceinline__ int tokens(int c) const { return int(min(int64_t(C), s1 - first_token(c))); }
   __device__ __forceinline__ uint32_t slot(uint32_t n) const { return n % G::NS; }
-  __device__ __forceinline__ bool wait(int which, int c) const { return mbar_wait_warp(&bars[which], c & 1); }
+  __device__ __forceinline__ bool wait(int which, int c) const { return warp_wait(&bars[which], c & 1); }
   __device__ __forceinline__ bool wait_turn(int which, int c) const {
-    return mbar_wait_warp(&bars[which + c % G::NA], (c / G::NA) & 1);
+    return warp_wait(&bars[which + c % G::NA], (c / G::NA) & 1);
   }
-  __device__ __forceinline__ bool wait_full(uint32_t n) const { return mbar_wait_warp(&full[n % G::NS], (n / G::NS) & 1); }
+  __device__ __forceinline__ bool wait_full(uint32_t n) const { return warp_wait(&full[n % G::NS], (n / G::NS) & 1); }
   __device__ __forceinline__ void arrive(int which) const {
     __syncwarp();
     if (lane == 0) mbar_arrive(&bars[which]);
   }
+
+  // Places of a chunk's tiles in the ring's order y, x, z (y, z).
+  __device__ __forceinline__ uint32_t tile_y(int c) const { return uint32_t(c) * PER; }
+  __device__ __forceinline__ uint32_t tile_x(int c) const { return uint32_t(c) * PER + 1; }
+  __device__ __forceinline__ uint32_t tile_z(int c) const { return uint32_t(c) * PER + PER - 1; }
 
   // ---- warp 0
   __device__ void load(const CUtensorMap* mx, const CUtensorMap* my, const CUtensorMap* mz) const {
@@ -150,113 +178,101 @@ struct Walk {
     uint32_t n = 0;
     for (int c = 0; c < chunks; ++c) {
       const int t0 = int(first_token(c));
-      for (int k = 3 - PER; k < 3; ++k, ++n) {
+      for (int i = 0; i < PER; ++i, ++n) {
+        const int k = i == 0 ? 1 : i == PER - 1 ? 2 : 0;
         const uint32_t s = slot(n), r = n / G::NS;
-        if (r > 0 && !mbar_wait_warp(&empty[s], (r - 1) & 1)) return;
+        if (r > 0 && !warp_wait(&empty[s], (r - 1) & 1)) return;
         if (leader) {
           const CUtensorMap* m = k == 0 ? mx : k == 1 ? my : mz;
           const int hh = h / (k == 0 ? p.gx : k == 1 ? p.gy : p.gz);
           const int blocks = (k == 2 ? DZ : DX) / 64;
           mbar_expect_tx(&full[s], uint32_t(blocks) * BLK);
-          for (int i = 0; i < blocks; ++i)
-            tma_load_4d(base + s * G::SLOT + i * BLK, m, &full[s], i * 64, hh, t0, int(b));
+          for (int blk = 0; blk < blocks; ++blk)
+            tma_load_4d(base + s * G::SLOT + blk * BLK, m, &full[s], blk * 64, hh, t0, int(b));
         }
         __syncwarp();
       }
     }
   }
 
-  // ---- warp 1.  A tile's slot is released by the last product that reads it (z's by the output's store), and
-  // the order keeps every wait behind products that do not need it: with two A buffers A of the next chunk goes
-  // first; with five slots D1 comes last, with four it comes before the next A, whose y takes x's slot.
+  // ---- warp 1.  A tile's slot is released by the last product that reads it (z's by the output's store).  With
+  // two A buffers A of the next chunk goes first; with one it follows the product that reads P, and D1 comes last.
   __device__ void mma() const {
     const bool leader = elect_one();
     const uint32_t id_a = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(C >> 3) << 17) | (uint32_t(C >> 4) << 24);
     const uint32_t id_d = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (uint32_t(DZ >> 3) << 17) |
                           (uint32_t(C >> 4) << 24);
     const uint32_t id_u = id_d | (1u << 15);
+    const Desc d_lo(sbase + G::LO, BLK), d_mid(sbase + G::MID, BLK), d_s(sbase + G::ST, BLK);
     auto at = [&](uint32_t n) { return sbase + slot(n) * G::SLOT; };
     auto product_a = [&](int c) {
-      const uint32_t nx = uint32_t(c) * PER, ny = nx + 1;
-      if (!wait_full(nx) || !wait_full(ny)) return false;
+      if (!wait_full(tile_y(c)) || !wait_full(tile_x(c))) return false;
       tc_after();
       if (leader) {
+        const Desc dx(at(tile_x(c)), 16), dy(at(tile_y(c)), 16);
 #pragma unroll
         for (int kk = 0; kk < DX / 16; ++kk) {
           const uint32_t off = (kk >> 2) * BLK + (kk & 3) * 32;
-          umma_bf16(tmem + G::T_A + uint32_t(c % G::NA) * 128, sdesc(at(nx) + off, 16, 1024), sdesc(at(ny) + off, 16, 1024),
-                    id_a, kk > 0);
+          umma_bf16(tmem + G::T_A + uint32_t(c % G::NA) * 128, dx.at(off), dy.at(off), id_a, kk > 0);
         }
         umma_commit(&bars[B_A + c % G::NA]);
       }
       __syncwarp();
       return true;
     };
-    auto product_d1 = [&](int c) {
-      const uint32_t nx = uint32_t(c) * PER;
-      if (!wait(B_S, c)) return false;
-      tc_after();
-      if (leader) {
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {  // 128 rows of S: all of x, or x twice
-          const int xk = kk % (DX / 16);
-          const uint32_t off = (xk >> 2) * BLK + (xk & 3) * 32;
-          umma_bf16(tmem + G::T_D1, sdesc(at(nx) + off, 16, 1024), sdesc(sbase + G::ST + kk * 2048, BLK, 1024), id_d, kk > 0);
-        }
-        umma_commit(&empty[slot(nx)]);
-      }
-      __syncwarp();
-      return true;
-    };
     if (!STATE_ONLY && chunks > 0 && !product_a(0)) return;
     for (int c = 0; c < chunks; ++c) {
-      const uint32_t ny = uint32_t(c) * PER + PER - 2, nz = ny + 1;
       const bool more = c + 1 < chunks;
       if (!STATE_ONLY && G::NA == 2 && more && !product_a(c + 1)) return;
-      if (!wait_full(nz) || !wait(B_K, c)) return;
+      if (!wait_full(tile_z(c)) || !wait(B_K, c)) return;
       tc_after();
+      const Desc dz(at(tile_z(c)), BLK);
       if (leader) {
         // small terms first, so that the accumulator drops the least
-        const uint32_t lo = sbase + G::LO, mid = sbase + G::MID;
+        const uint32_t yb = at(tile_y(c));
+        const Desc dy(yb, DX == 64 ? sbase + G::MID - yb : BLK);
         if (NT == 3) {
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
-            umma_bf16(tmem + G::T_U, sdesc(lo + kk * 2048, BLK, 1024), sdesc(at(nz) + kk * 2048, BLK, 1024), id_u, kk > 0);
+          for (int kk = 0; kk < 8; ++kk) umma_bf16(tmem + G::T_U, d_lo.at(kk * 2048), dz.at(kk * 2048), id_u, kk > 0);
         }
         if (DX == 128) {
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
-            umma_bf16(tmem + G::T_U, sdesc(mid + kk * 2048, BLK, 1024), sdesc(at(nz) + kk * 2048, BLK, 1024), id_u,
-                      NT == 3 || kk > 0);
+            umma_bf16(tmem + G::T_U, d_mid.at(kk * 2048), dz.at(kk * 2048), id_u, NT == 3 || kk > 0);
         }
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
-          umma_bf16(tmem + G::T_U, sdesc(at(ny) + kk * 2048, DX == 64 ? mid - at(ny) : BLK, 1024),
-                    sdesc(at(nz) + kk * 2048, BLK, 1024), id_u, NT == 3 || DX == 128 || kk > 0);
+          umma_bf16(tmem + G::T_U, dy.at(kk * 2048), dz.at(kk * 2048), id_u, NT == 3 || DX == 128 || kk > 0);
         umma_commit(&bars[B_U]);
-        umma_commit(&empty[slot(ny)]);
-        if (STATE_ONLY) umma_commit(&empty[slot(nz)]);
+        umma_commit(&empty[slot(tile_y(c))]);
+        if (STATE_ONLY) umma_commit(&empty[slot(tile_z(c))]);
       }
       __syncwarp();
       if (STATE_ONLY) continue;
       if (!wait_turn(B_P, c)) return;
       if (c > 0 && !wait(B_DFREE, c - 1)) return;
-      if (G::NS == 4 && !product_d1(c)) return;
       tc_after();
       if (leader) {
         const uint32_t pa = tmem + G::T_A + uint32_t(c % G::NA) * 128;
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)  // P of columns 0..63 and 64..127 lies where each half of A was
-          umma_bf16_ta(tmem + G::T_D2, pa + (kk >> 2) * 64 + (kk & 3) * 8, sdesc(at(nz) + kk * 2048, BLK, 1024), id_d, kk > 0);
-        if (G::NS == 4) umma_commit(&bars[B_O]);
+          umma_bf16_ta(tmem + G::T_D2, pa + (kk >> 2) * 64 + (kk & 3) * 8, dz.at(kk * 2048), id_d, kk > 0);
       }
       __syncwarp();
       if (G::NA == 1 && more && !product_a(c + 1)) return;
-      if (G::NS != 4) {
-        if (!product_d1(c)) return;
-        if (leader) umma_commit(&bars[B_O]);
-        __syncwarp();
+      if (!wait(B_S, c)) return;
+      tc_after();
+      if (leader) {
+        const Desc dx(at(tile_x(c)), 16);
+#pragma unroll
+        for (int kk = 0; kk < 8; ++kk) {  // 128 rows of S: all of x, or x twice
+          const int xk = kk % (DX / 16);
+          umma_bf16(tmem + G::T_D1, dx.at((xk >> 2) * BLK + (xk & 3) * 32), d_s.at(kk * 2048), id_d, kk > 0);
+        }
+        umma_commit(&empty[slot(tile_x(c))]);
+        umma_commit(&bars[B_O]);
       }
+      __syncwarp();
     }
   }
 
@@ -319,7 +335,7 @@ struct Walk {
     if (!wait(B_O, c)) return false;
     tc_after();
     const float w = i < n ? p.scale * pw[REV ? n - 1 - i : i + 1] : 0.f, w2 = p.scale * p.z_scale;
-    const uint32_t stage = sbase + slot(uint32_t(c) * PER + 2) * G::SLOT;
+    const uint32_t stage = sbase + slot(tile_z(c)) * G::SLOT;
 #pragma unroll
     for (int g = 0; g < HC / 32; ++g) {
       uint32_t d1[32], d2[32];
@@ -383,7 +399,7 @@ struct Walk {
   // ---- warp 18: stores the staged output and hands z's slot back
   __device__ void store(const CUtensorMap* mo) const {
     for (int c = 0; c < chunks; ++c) {
-      const uint32_t nz = uint32_t(c) * PER + 2;
+      const uint32_t nz = tile_z(c);
       if (!wait(B_OSTAGED, c)) return;
       if (lane == 0) {
         if (!p.out_f32) {
@@ -406,33 +422,39 @@ struct Walk {
 
   // ---- the weighted y of chunk c as bf16 terms (this thread's 16-byte pieces); z's rows past the length
   __device__ __forceinline__ bool weigh(int c, int tid) const {
-    const uint32_t ny = uint32_t(c) * PER + PER - 2, nz = ny + 1;
+    const uint32_t ny = tile_y(c), nz = tile_z(c);
     const int n = tokens(c);
     const uint32_t yb = sbase + slot(ny) * G::SLOT;
     if (STATE_ONLY ? !wait_full(ny) : !wait_turn(B_A, c)) return false;
+    constexpr int PIECES = DX / 64 * 1024 / CONV, BATCH = PIECES < 4 ? PIECES : 4;
 #pragma unroll
-    for (int k = 0; k < DX / 64 * 1024 / CONV; ++k) {
-      const uint32_t u = uint32_t(tid + CONV * k), off = u * 16;
-      const int j = int(u >> 3) & 127;       // token
-      uint32_t v[4], hi[4], mid[4], lo[4];
-      lds128(yb + off, v);
-      if (j >= n) v[0] = v[1] = v[2] = v[3] = 0;  // what lies there may be anything
-      const float w = j < n ? pw[REV ? j + 1 : n - 1 - j] : 0.f;
-      const float2 w2 = make_float2(w, w), minus = make_float2(-1.f, -1.f);
+    for (int k0 = 0; k0 < PIECES; k0 += BATCH) {
+      uint32_t v[BATCH][4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float2 a = __fmul2_rn(unpack2(v[e]), w2);
-        hi[e] = pack2(a);
-        a = __ffma2_rn(unpack2(hi[e]), minus, a);
-        mid[e] = pack2(a);
-        if (NT == 3) {
-          a = __ffma2_rn(unpack2(mid[e]), minus, a);
-          lo[e] = pack2(a);
+      for (int k = 0; k < BATCH; ++k) lds128(yb + uint32_t(tid + CONV * (k0 + k)) * 16, v[k]);
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        const uint32_t u = uint32_t(tid + CONV * (k0 + k)), off = u * 16;
+        const int j = int(u >> 3) & 127;       // token
+        uint32_t hi[4], mid[4], lo[4];
+        if (j >= n) v[k][0] = v[k][1] = v[k][2] = v[k][3] = 0;  // what lies there may be anything
+        const float w = j < n ? pw[REV ? j + 1 : n - 1 - j] : 0.f;
+        const float2 w2 = make_float2(w, w), minus = make_float2(-1.f, -1.f);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float2 a = __fmul2_rn(unpack2(v[k][e]), w2);
+          hi[e] = pack2(a);
+          a = __ffma2_rn(unpack2(hi[e]), minus, a);
+          mid[e] = pack2(a);
+          if (NT == 3) {
+            a = __ffma2_rn(unpack2(mid[e]), minus, a);
+            lo[e] = pack2(a);
+          }
         }
+        sts128(yb + off, hi);
+        sts128(sbase + G::MID + off, mid);
+        if (NT == 3) sts128(sbase + G::LO + off, lo);
       }
-      sts128(yb + off, hi);
-      sts128(sbase + G::MID + off, mid);
-      if (NT == 3) sts128(sbase + G::LO + off, lo);
     }
     if (n < C) {
       if (!wait_full(nz)) return false;
@@ -589,7 +611,12 @@ walk_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
       }
     } else {
       bool ok = true;
-      for (int c = 0; c < w.chunks && ok; ++c) ok = w.scores(c) && (c == 0 || w.output(c - 1));
+      // with one A buffer the output goes first: the product that reads P waits for its accumulators
+      for (int c = 0; c < w.chunks && ok; ++c) {
+        if (G::NA == 1 && c > 0) ok = w.output(c - 1);
+        ok = ok && w.scores(c);
+        if (G::NA == 2 && c > 0) ok = ok && w.output(c - 1);
+      }
       if (ok && w.chunks > 0) w.output(w.chunks - 1);
       w.zeros();
     }
