@@ -473,7 +473,8 @@ static Cut cut(int64_t ctas, int64_t L, int chunk, int resident) {
   Cut best = {1, (chunks ? chunks : 1) * chunk};
   if (ctas == 0) return best;
   double least = 0;
-  for (int64_t s = 1; s <= chunks && s <= 2 * slots; ++s) {
+  // (more than two waves of pieces never pay)
+  for (int64_t s = 1; s <= chunks && (s == 1 || ctas * s <= 2 * slots); ++s) {
     const int64_t per = (chunks + s - 1) / s, n = (chunks + per - 1) / per;
     if (n != s) continue;
     const double t = double((ctas * n + slots - 1) / slots) * (double(per) * (n > 1 ? 1.5 : 1.0) + 2.5) + (n > 1 ? 3.0 : 0.0);
@@ -562,7 +563,7 @@ static size_t workspace(const Shape& p, bool backward) {
   size_t pieces = 0;
   for (const Plan& q : {f, t})
     if (q.c.segs > 1 && q.c.segs * state > pieces) pieces = q.c.segs * state;
-  size_t n = 256;
+  size_t n = 0;
   if (pieces) n += (backward ? 2 : 1) * (Workspace::round(pieces) + 256);
   if (backward) {
     const int segs = f.c.segs > t.c.segs ? f.c.segs : t.c.segs;
@@ -676,12 +677,12 @@ extern "C" int pgf_decay_attn_bwd(const void* q, const pgf_strides* q_strides, c
   const size_t states = size_t(Bsz) * H * job.segs * Dk * Dv;
   float* sp = job.segs > 1 ? w.take<float>(states) : nullptr;
   float* xp = job.segs > 1 ? w.take<float>(states) : nullptr;
-  float* part = w.take<float>(size_t(H) * Bsz * job.segs * ceil_div(Dv, da::E));
+  float* part = grad_log_decay ? w.take<float>(size_t(H) * Bsz * job.segs * ceil_div(Dv, da::E)) : nullptr;
   const int64_t tokens = Bsz * L;
   float* pq = Hq < H ? w.take<float>(size_t(tokens) * H * Dk) : nullptr;
   float* pk = Hk < H ? w.take<float>(size_t(tokens) * H * Dk) : nullptr;
   float* pv = Hv < H ? w.take<float>(size_t(tokens) * H * Dv) : nullptr;
-  if (!ws || !part || (job.segs > 1 && (!sp || !xp)) || (Hq < H && !pq) || (Hk < H && !pk) || (Hv < H && !pv)) {
+  if ((grad_log_decay && !part) || (job.segs > 1 && (!sp || !xp)) || (Hq < H && !pq) || (Hk < H && !pk) || (Hv < H && !pv)) {
     set_error("decay_attn_bwd: workspace of %zu bytes is too small", ws_bytes);
     return PGF_ERR_WORKSPACE;
   }

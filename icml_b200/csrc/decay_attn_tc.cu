@@ -53,8 +53,9 @@ struct Cfg {
   static constexpr uint32_t RING = NS * SLOT;
   static constexpr uint32_t MID = RING, LO = MID + XB, ZERO = LO + XB;  // ZERO only with 64-wide y
   static constexpr uint32_t ST = NT == 2 ? LO : DX == 64 ? ZERO + BLK : ZERO;  // S: 128 rows x DZ bf16
-  static constexpr uint32_t TAB = ST + ZB;                              // 256 + 32 floats
-  static constexpr uint32_t BARS = TAB + 1152;
+  static constexpr uint32_t WTAB = ST + ZB;                             // 130 x 8 bytes
+  static constexpr uint32_t TAB = WTAB + 1040;                          // 132 + 32 floats
+  static constexpr uint32_t BARS = TAB + 656;
   static constexpr uint32_t BYTES = BARS + 256 + 1024;
   // TMEM columns
   static constexpr uint32_t T_A = 0, T_D1 = NA * 128, T_D2 = T_D1 + DZ, T_U = T_D2 + DZ;
@@ -70,7 +71,7 @@ struct Params {
   float* end;
   float scale, z_scale;
   int64_t L, seg_len;
-  int H, segs, dx, dz, start_t, out_f32, last_too;
+  int H, segs, dx, dz, start_t, out_f32, last_too, wide;
   int gx, gy, gz;              // operator heads per tensor head
 };
 
@@ -101,6 +102,23 @@ __device__ __forceinline__ void lds128(uint32_t a, uint32_t (&v)[4]) {
 }
 __device__ __forceinline__ void sts128(uint32_t a, const uint32_t (&v)[4]) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
+// Reads of the tables, which stay as they are once the CTA has written them (shared addresses: a load through a
+// generic pointer is a slower one).
+__device__ __forceinline__ float lds_f(uint32_t a) {
+  float v;
+  asm("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds_u2(uint32_t a) {
+  uint2 v;
+  asm("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ float4 lds_f4(uint32_t a) {
+  float4 v;
+  asm("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
+  return v;
 }
 __device__ __forceinline__ float2 unpack2(uint32_t v) {
   return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
@@ -144,15 +162,18 @@ struct Walk {
   const Params& p;
   uint8_t* base;
   uint32_t sbase;
-  float* tab;          // tab[127 + e] = a^e for e >= 0, 0 below
-  const float* pw;     // a^0 .. a^128
-  const float* cf;     // column factors of a block off the diagonal: a^(31-k), from the end a^k
   uint64_t* full;
   uint64_t* empty;
   uint64_t* bars;
   uint32_t tmem;
   int warp, lane, seg, h, chunks;
   int64_t b, bh, len, s0, s1;
+
+  // a^e; a^e as two bf16 terms, each twice; column factors of a block off the diagonal: a^(31-k), from the end a^k
+  __device__ __forceinline__ uint32_t pw_at(int e) const { return sbase + G::TAB + 4 * e; }
+  __device__ __forceinline__ float pw(int e) const { return lds_f(pw_at(e)); }
+  __device__ __forceinline__ uint2 wt(int e) const { return lds_u2(sbase + G::WTAB + 8 * e); }
+  __device__ __forceinline__ float4 cf4(int k) const { return lds_f4(sbase + G::TAB + 528 + 4 * k); }
 
   __device__ __forceinline__ int64_t first_token(int c) const { return s0 + int64_t(REV ? chunks - 1 - c : c) * C; }
   __device__ __forceinline__ int tokens(int c) const { return int(min(int64_t(C), s1 - first_token(c))); }
@@ -257,9 +278,9 @@ struct Walk {
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)  // P of columns 0..63 and 64..127 lies where each half of A was
           umma_bf16_ta(tmem + G::T_D2, pa + (kk >> 2) * 64 + (kk & 3) * 8, dz.at(kk * 2048), id_d, kk > 0);
+        if (G::NS == 5) umma_commit(&empty[slot(tile_z(c))]);
       }
       __syncwarp();
-      if (G::NA == 1 && more && !product_a(c + 1)) return;
       if (!wait(B_S, c)) return;
       tc_after();
       if (leader) {
@@ -273,6 +294,7 @@ struct Walk {
         umma_commit(&bars[B_O]);
       }
       __syncwarp();
+      if (G::NA == 1 && more && !product_a(c + 1)) return;
     }
   }
 
@@ -295,17 +317,17 @@ struct Walk {
         tmem_ld32(ta + g * 32, r);
         const int lim = REV ? n - 32 * cb : 32;   // columns past the length
         if (cb != q && lim >= 32) {
-          const float rf = REV ? pw[32 * cb - i] : pw[i - 32 * cb - 31];
+          const float rf = pw(REV ? 32 * cb - i : i - 32 * cb - 31);
           const float2 rf2 = make_float2(rf, rf);
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const float4 w = *reinterpret_cast<const float4*>(cf + 4 * k);
+            const float4 w = cf4(4 * k);
             const float2 lo = __fmul2_rn(make_float2(w.x, w.y), rf2), hi = __fmul2_rn(make_float2(w.z, w.w), rf2);
             pk[2 * k] = pack2(__fmul2_rn(make_float2(__uint_as_float(r[4 * k]), __uint_as_float(r[4 * k + 1])), lo));
             pk[2 * k + 1] = pack2(__fmul2_rn(make_float2(__uint_as_float(r[4 * k + 2]), __uint_as_float(r[4 * k + 3])), hi));
           }
         } else {
-          const float* t = tab + 127 + (REV ? 32 * cb - i : i - 32 * cb);
+          const uint32_t t = pw_at(REV ? 32 * cb - i : i - 32 * cb);  // masked lanes read what lies in front
 #pragma unroll
           for (int k = 0; k < 16; ++k) {
             float v[2];
@@ -313,7 +335,7 @@ struct Walk {
             for (int e = 0; e < 2; ++e) {
               const int j = 2 * k + e;
               const bool in = REV ? 32 * cb + j >= i && j < lim : 32 * cb + j <= i;
-              v[e] = in ? __uint_as_float(r[j]) * t[REV ? j : -j] : 0.f;
+              v[e] = in ? __uint_as_float(r[j]) * lds_f(t + (REV ? 4 * j : -4 * j)) : 0.f;
             }
             pk[k] = pack_bf16(v[0], v[1]);
           }
@@ -334,7 +356,7 @@ struct Walk {
     const int n = tokens(c);
     if (!wait(B_O, c)) return false;
     tc_after();
-    const float w = i < n ? p.scale * pw[REV ? n - 1 - i : i + 1] : 0.f, w2 = p.scale * p.z_scale;
+    const float w = i < n ? p.scale * pw(REV ? n - 1 - i : i + 1) : 0.f, w2 = p.scale * p.z_scale;
     const uint32_t stage = sbase + slot(tile_z(c)) * G::SLOT;
 #pragma unroll
     for (int g = 0; g < HC / 32; ++g) {
@@ -362,6 +384,25 @@ struct Walk {
             if (col + 4 * k < p.dz)
               *reinterpret_cast<float4*>(dst + 4 * k) = make_float4(o[2 * k].x, o[2 * k].y, o[2 * k + 1].x, o[2 * k + 1].y);
         }
+      } else if (G::NS == 5) {
+        if (t0 + i < p.L) {
+          __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + ((b * p.L + t0 + i) * p.H + h) * p.dz + col;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            const float2* v = o + 8 * k;
+            if (p.wide) {  // 32 bytes: the width is a multiple of 16
+              if (col + 16 * k < p.dz)
+                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + 16 * k), "r"(pack2(v[0])),
+                             "r"(pack2(v[1])), "r"(pack2(v[2])), "r"(pack2(v[3])), "r"(pack2(v[4])), "r"(pack2(v[5])),
+                             "r"(pack2(v[6])), "r"(pack2(v[7])) : "memory");
+            } else {
+              if (col + 16 * k < p.dz)
+                *reinterpret_cast<uint4*>(dst + 16 * k) = make_uint4(pack2(v[0]), pack2(v[1]), pack2(v[2]), pack2(v[3]));
+              if (col + 16 * k + 8 < p.dz)
+                *reinterpret_cast<uint4*>(dst + 16 * k + 8) = make_uint4(pack2(v[4]), pack2(v[5]), pack2(v[6]), pack2(v[7]));
+            }
+          }
+        }
       } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -373,8 +414,10 @@ struct Walk {
         }
       }
     }
+    if (G::NS != 5) {
     fence_async();
     arrive(B_OSTAGED);
+    }
     return true;
   }
 
@@ -437,18 +480,32 @@ struct Walk {
         const uint32_t u = uint32_t(tid + CONV * (k0 + k)), off = u * 16;
         const int j = int(u >> 3) & 127;       // token
         uint32_t hi[4], mid[4], lo[4];
+        const int e = REV ? j + 1 : n - 1 - j;
         if (j >= n) v[k][0] = v[k][1] = v[k][2] = v[k][3] = 0;  // what lies there may be anything
-        const float w = j < n ? pw[REV ? j + 1 : n - 1 - j] : 0.f;
-        const float2 w2 = make_float2(w, w), minus = make_float2(-1.f, -1.f);
+        if (NT == 2) {
+          // in packed bf16: hi = rn(y w1), its error y w1 - hi exactly, mid = rn(that + y w2)
+          const uint2 w = wt(j < n ? e : 0);
+          const __nv_bfloat162 w1 = *reinterpret_cast<const __nv_bfloat162*>(&w.x);
+          const __nv_bfloat162 w2 = *reinterpret_cast<const __nv_bfloat162*>(&w.y);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float2 a = __fmul2_rn(unpack2(v[k][e]), w2);
-          hi[e] = pack2(a);
-          a = __ffma2_rn(unpack2(hi[e]), minus, a);
-          mid[e] = pack2(a);
-          if (NT == 3) {
-            a = __ffma2_rn(unpack2(mid[e]), minus, a);
-            lo[e] = pack2(a);
+          for (int m = 0; m < 4; ++m) {
+            const __nv_bfloat162 y = *reinterpret_cast<const __nv_bfloat162*>(&v[k][m]);
+            const __nv_bfloat162 h = __hmul2_rn(y, w1);
+            const __nv_bfloat162 r = __hfma2(y, w2, __hfma2(y, w1, __hneg2(h)));
+            hi[m] = *reinterpret_cast<const uint32_t*>(&h);
+            mid[m] = *reinterpret_cast<const uint32_t*>(&r);
+          }
+        } else {
+          const float w = pw(j < n ? e : 0);
+          const float2 w2 = make_float2(w, w), minus = make_float2(-1.f, -1.f);
+#pragma unroll
+          for (int m = 0; m < 4; ++m) {
+            float2 a = __fmul2_rn(unpack2(v[k][m]), w2);
+            hi[m] = pack2(a);
+            a = __ffma2_rn(unpack2(hi[m]), minus, a);
+            mid[m] = pack2(a);
+            a = __ffma2_rn(unpack2(mid[m]), minus, a);
+            lo[m] = pack2(a);
           }
         }
         sts128(yb + off, hi);
@@ -502,7 +559,7 @@ struct Walk {
       }
       if (!wait(B_U, c)) return;
       tc_after();
-      const float an = pw[tokens(c)];
+      const float an = pw(tokens(c));
       const float2 an2 = make_float2(an, an), zs = make_float2(p.z_scale, p.z_scale);
 #pragma unroll
       for (int g = 0; g < HC / 16; ++g) {
@@ -556,12 +613,13 @@ walk_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
   using G = typename W::G;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint2* wt = reinterpret_cast<uint2*>(base + G::WTAB);
   float* tab = reinterpret_cast<float*>(base + G::TAB);
   uint64_t* full = reinterpret_cast<uint64_t*>(base + G::BARS);
   uint64_t* bars = full + 2 * G::NS;
   static_assert((2 * G::NS + B_COUNT) * 8 + 4 <= 256, "barriers fit");
   uint32_t* tslot = reinterpret_cast<uint32_t*>(bars + B_COUNT);
-  W w{p, base, smem_u32(base), tab, tab + 127, tab + 256, full, full + G::NS, bars, 0u, int(threadIdx.x >> 5),
+  W w{p, base, smem_u32(base), full, full + G::NS, bars, 0u, int(threadIdx.x >> 5),
       int(threadIdx.x & 31)};
   w.seg = int(blockIdx.x % p.segs);
   w.bh = blockIdx.x / p.segs;
@@ -575,8 +633,13 @@ walk_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
   w.chunks = idle ? 0 : int((w.s1 - w.s0 + C - 1) / C);
 
   const float l2 = log2_decay(p.log_decay[w.h]);
-  for (int i = threadIdx.x; i < 256; i += THREADS) tab[i] = i >= 127 ? exp2f(l2 * float(i - 127)) : 0.f;
-  if (threadIdx.x < 32) tab[256 + threadIdx.x] = exp2f(l2 * float(REV ? threadIdx.x : 31 - threadIdx.x));
+  if (threadIdx.x <= C) {
+    const float a = exp2f(l2 * float(threadIdx.x));
+    const float a1 = __bfloat162float(__float2bfloat16_rn(a));
+    tab[threadIdx.x] = a;
+    wt[threadIdx.x] = make_uint2(pack_bf16(a1, a1), pack_bf16(a - a1, a - a1));
+  }
+  if (threadIdx.x < 32) tab[132 + threadIdx.x] = exp2f(l2 * float(REV ? threadIdx.x : 31 - threadIdx.x));
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2 * G::NS; ++s) mbar_init(&full[s], 1);
     for (int k = 0; k < B_COUNT; ++k) mbar_init(&bars[k], k == B_A || k == B_A1 || k == B_O || k == B_U ? 1 : k == B_K ? W::CONV / 32 : 8);
@@ -623,7 +686,7 @@ walk_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
   } else if (w.warp < 18) {
     w.state();
   } else if (w.warp == 18) {
-    if (!STATE_ONLY) w.store(&tmO);
+    if (!STATE_ONLY && G::NS != 5) w.store(&tmO);
   }
   tc_before();
   __syncthreads();
@@ -691,6 +754,7 @@ int launch(const Job& j, cudaStream_t s) {
   p.start_t = j.start_t;
   p.out_f32 = j.out_f32;
   p.last_too = j.last_too;
+  p.wide = j.z.d % 16 == 0 && aligned(j.out, 32);
   p.gx = STATE_ONLY ? 1 : j.H / j.x.heads;
   p.gy = j.H / j.y.heads;
   p.gz = j.H / j.z.heads;

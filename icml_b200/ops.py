@@ -834,7 +834,10 @@ def mamba_mixer_bwd_finish(state, dh_end=None, dA_end=None, want_g_halo=False):
 
 
 # --------------------------------------------------------------------------- decay-attention layer
+# These calls are made once per layer and token when decoding, so the time of the call itself counts: each
+# attribute is read once, and what is already as the kernels want it is passed on without a copy.
 PAIRS = {"halves": 0, "neighbours": 1}
+_DT = {torch.float32: F32, torch.bfloat16: BF16}
 
 
 def rotary_turns(dim: int, base: float = 10000.0, device="cuda") -> torch.Tensor:
@@ -848,60 +851,94 @@ def rotary_turns(dim: int, base: float = 10000.0, device="cuda") -> torch.Tensor
     return (f * 2.0 ** 64).to(torch.int64).to(device)
 
 
+def _acts(name: str, *ts: torch.Tensor) -> Tuple[int, int]:
+    """(type code, device index) of activations that share both."""
+    first = ts[0]
+    dtype, dev = first.dtype, first.get_device()
+    if dev < 0:
+        raise RuntimeError("icml_b200 operators run on CUDA tensors only (no CPU path)")
+    for t in ts:
+        if t.dtype is not dtype or t.get_device() != dev:
+            raise TypeError(f"{name}: tensors of {dtype} on cuda:{dev} and {t.dtype} on {t.device}")
+    dt = _DT.get(dtype)
+    if dt is None:
+        raise TypeError(f"unsupported activation dtype {dtype} (float32 or bfloat16)")
+    return dt, dev
+
+
 def _view(t: torch.Tensor):
     """(tensor, its strides for the C boundary): any (B, L, heads, D) or (B, heads, D) view whose last
     dimension is contiguous goes as it is, anything else is copied."""
-    if t.stride(-1) != 1 and t.shape[-1] > 1:
+    st = t.stride()
+    if st[-1] != 1 and t.shape[-1] > 1:
         t = t.contiguous()
-    if t.dim() == 3:
-        return t, Strides(t.stride(0), 0, t.stride(1))
-    return t, Strides(t.stride(0), t.stride(1), t.stride(2))
+        st = t.stride()
+    return t, (Strides(st[0], st[1], st[2]) if len(st) == 4 else Strides(st[0], 0, st[1]))
 
 
-def _same(name: str, *ts: Optional[torch.Tensor]) -> None:
-    """One device and, for activations, one type."""
-    ts = [t for t in ts if t is not None]
-    for t in ts[1:]:
-        if t.device != ts[0].device:
-            raise ValueError(f"{name}: tensors on {ts[0].device} and {t.device}")
-        if t.dtype != ts[0].dtype:
-            raise TypeError(f"{name}: tensors of {ts[0].dtype} and {t.dtype}")
+def _param(name: str, t: torch.Tensor, shape, dev: int) -> torch.Tensor:
+    """A float32 tensor of this shape on this device, contiguous."""
+    if t.shape != shape or t.dtype is not torch.float32 or t.get_device() != dev:
+        raise ValueError(f"{name}: {t.dtype} {tuple(t.shape)} on {t.device}, want float32 {tuple(shape)} on cuda:{dev}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _whole(name: str, what: str, t: torch.Tensor, shape, dev: int, dtype) -> torch.Tensor:
+    """A tensor of whole numbers of this shape on this device as `dtype`, contiguous."""
+    if t.get_device() != dev or t.is_floating_point() or t.dtype is torch.bool or t.shape != shape:
+        raise ValueError(f"{name}: {what} {t.dtype} {tuple(t.shape)} on {t.device}, want whole numbers {tuple(shape)} "
+                         f"on cuda:{dev}")
+    if t.dtype is not dtype:
+        t = t.to(dtype)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _raw_stream(dev: int) -> int:
+    """The current stream of the tensors' device, which has to be the current device."""
+    if dev != torch._C._cuda_getDevice():
+        raise RuntimeError(f"icml_b200: tensors on cuda:{dev}, but the current device is cuda:{torch._C._cuda_getDevice()}")
+    return torch._C._cuda_getCurrentRawStream(dev)
 
 
 def _qk_args(name, q, k, wq, wk, turns, positions, pairs):
-    _cuda(q, k, wq, wk, turns, positions)
-    _same(name, q, k)
-    if q.dim() != 4 or k.dim() != 4 or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
-        raise ValueError(f"{name}: queries {tuple(q.shape)} and keys {tuple(k.shape)}, want (B, L, heads, D)")
-    B, L_, _, D = q.shape
-    for w in (wq, wk):
-        if w is not None and tuple(w.shape) != (D,):
-            raise ValueError(f"{name}: weight {tuple(w.shape)} for heads of {D}")
-    if turns is not None and (turns.dtype != torch.int64 or turns.dim() != 1 or 2 * turns.numel() > D):
-        raise ValueError(f"{name}: turns must be int64 of at most {D // 2} entries (rotary_turns)")
+    dt, dev = _acts(name, q, k)
+    qsh, ksh = q.shape, k.shape
+    if len(qsh) != 4 or len(ksh) != 4 or qsh[0] != ksh[0] or qsh[1] != ksh[1] or qsh[3] != ksh[3]:
+        raise ValueError(f"{name}: queries {tuple(qsh)} and keys {tuple(ksh)}, want (B, L, heads, D)")
+    B, L_, _, D = qsh
+    if wq is not None:
+        wq = _param(name, wq, (D,), dev)
+    if wk is not None:
+        wk = _param(name, wk, (D,), dev)
+    R = 0
+    if turns is not None:
+        R = 2 * turns.numel()
+        if turns.dtype is not torch.int64 or turns.dim() != 1 or R > D or turns.get_device() != dev:
+            raise ValueError(f"{name}: turns must be int64 of at most {D // 2} entries on cuda:{dev} (rotary_turns)")
+        turns = turns.contiguous()
     if positions is not None:
-        if positions.dtype.is_floating_point or tuple(positions.shape) not in ((B, L_), (L_,)):
-            raise ValueError(f"{name}: positions {positions.dtype} {tuple(positions.shape)} for {(B, L_)}")
-        positions = positions.long().expand(B, L_).contiguous()
-    if pairs not in PAIRS:
+        if positions.dim() == 1:
+            positions = positions.expand(B, positions.shape[0])
+        positions = _whole(name, "positions", positions, (B, L_), dev, torch.int64)
+    code = PAIRS.get(pairs)
+    if code is None:
         raise ValueError(f"{name}: pairs {pairs!r} (halves or neighbours)")
-    return _f32(wq), _f32(wk), _c(turns), positions, 0 if turns is None else 2 * turns.numel()
+    return dt, dev, B, L_, qsh[2], ksh[2], D, R, wq, wk, turns, positions, code
 
 
 def qk_norm_rotate_fwd(q, k, wq=None, wk=None, turns=None, *, positions=None, start: int = 0, eps: float = 1e-6,
                        pairs: str = "halves"):
-    """(queries, keys) normed for each head, weighted by wq / wk (D, None: ones) and rotated by position
-    in one pass.  q (B, L, Hq, D) and k (B, L, Hk, D) may be views of one projection's rows.  turns:
+    """(queries, keys) normed for each head, weighted by wq / wk (float32 (D), None: ones) and rotated by
+    position in one pass.  q (B, L, Hq, D) and k (B, L, Hk, D) may be views of one projection's rows.  turns:
     rotary_turns(R) for the first R elements of a head (None: no rotation); positions (B, L) or (L,),
     default start, start + 1, ...; pairs "halves" (i with i + R/2) or "neighbours" (2i with 2i + 1)."""
-    wq, wk, turns, positions, R = _qk_args("qk_norm_rotate_fwd", q, k, wq, wk, turns, positions, pairs)
+    dt, dev, B, L_, Hq, Hk, D, R, wq, wk, turns, positions, code = _qk_args("qk_norm_rotate_fwd", q, k, wq, wk, turns,
+                                                                            positions, pairs)
     (q, qs), (k, ks) = _view(q), _view(k)
-    B, L_, Hq, D = q.shape
-    qo = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    ko = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    check(lib().pgf_qk_norm_rotate_fwd(_p(q), qs, _p(k), ks, _p(wq), _p(wk), _p(turns), _p(positions), start, _p(qo),
-                                       _p(ko), B, L_, Hq, k.shape[2], D, R, PAIRS[pairs], eps, _dt(q), _stream()),
-          "qk_norm_rotate_fwd")
+    qo, ko = q.new_empty(q.shape), k.new_empty(k.shape)
+    check(lib().pgf_qk_norm_rotate_fwd(q.data_ptr(), qs, k.data_ptr(), ks, _p(wq), _p(wk), _p(turns), _p(positions),
+                                       start, qo.data_ptr(), ko.data_ptr(), B, L_, Hq, Hk, D, R, code, eps, dt,
+                                       _raw_stream(dev)), "qk_norm_rotate_fwd")
     return qo, ko
 
 
@@ -911,63 +948,40 @@ def qk_norm_rotate_bwd(q, k, gq, gk, wq=None, wk=None, turns=None, *, positions=
     and grad_wq, grad_wk (float32) where a weight was given.  acc: a dict of float32 grad_wq / grad_wk
     buffers to add into (both or none)."""
     name = "qk_norm_rotate_bwd"
-    has_q, has_k = wq is not None, wk is not None
-    wq, wk, turns, positions, R = _qk_args(name, q, k, wq, wk, turns, positions, pairs)
-    _cuda(gq, gk)
-    _same(name, q, gq, gk)
+    dt, dev, B, L_, Hq, Hk, D, R, wq, wk, turns, positions, code = _qk_args(name, q, k, wq, wk, turns, positions, pairs)
+    _acts(name, q, gq, gk)
     if gq.shape != q.shape or gk.shape != k.shape:
         raise ValueError(f"{name}: gradients {tuple(gq.shape)}, {tuple(gk.shape)} of {tuple(q.shape)}, {tuple(k.shape)}")
     (q, qs), (k, ks) = _view(q), _view(k)
-    gq, gk = _c(gq), _c(gk)
-    B, L_, Hq, D = q.shape
-    out = {"grad_q": torch.empty(q.shape, dtype=q.dtype, device=q.device),
-           "grad_k": torch.empty(k.shape, dtype=k.dtype, device=k.device)}
-    acc = acc or {}
+    gq, gk = gq.contiguous(), gk.contiguous()
+    out = {"grad_q": q.new_empty(q.shape), "grad_k": k.new_empty(k.shape)}
     flags = set()
-    for key, has in (("grad_wq", has_q), ("grad_wk", has_k)):
-        if has:
-            out[key], a = _acc_buffer(acc.get(key), (D,), q.device, name)
+    for key, w in (("grad_wq", wq), ("grad_wk", wk)):
+        if w is not None:
+            out[key], a = _acc_buffer(acc.get(key) if acc else None, (D,), q.device, name)
             flags.add(a)
     if len(flags) > 1:
         raise ValueError(f"{name}: give both accumulators or none")
     L = lib()
-    ws = _ws(L.pgf_qk_norm_rotate_bwd_workspace(D), q.device)
-    check(L.pgf_qk_norm_rotate_bwd(_p(q), qs, _p(k), ks, _p(gq), _p(gk), _p(wq), _p(wk), _p(turns), _p(positions), start,
-                                   _p(out["grad_q"]), _p(out["grad_k"]), _p(out.get("grad_wq")),
-                                   _p(out.get("grad_wk")), int(flags == {1}), B, L_, Hq, k.shape[2], D, R, PAIRS[pairs],
-                                   eps, _dt(q), _p(ws), ws.numel(), _stream()), name)
+    ws = q.new_empty(L.pgf_qk_norm_rotate_bwd_workspace(D), dtype=torch.uint8)
+    check(L.pgf_qk_norm_rotate_bwd(q.data_ptr(), qs, k.data_ptr(), ks, gq.data_ptr(), gk.data_ptr(), _p(wq), _p(wk),
+                                   _p(turns), _p(positions), start, out["grad_q"].data_ptr(), out["grad_k"].data_ptr(),
+                                   _p(out.get("grad_wq")), _p(out.get("grad_wk")), int(flags == {1}), B, L_, Hq, Hk, D, R,
+                                   code, eps, dt, ws.data_ptr(), ws.numel(), _raw_stream(dev)), name)
     return out
 
 
 def _decay_args(name, q, k, v, log_decay, dims):
-    """Checks what the decay-attention calls share; (B, L, H, Hq, Hk, Hv, Dk, Dv)."""
-    _cuda(q, k, v, log_decay)
-    _same(name, q, k, v)
-    if log_decay.dtype != torch.float32 or log_decay.dim() != 1 or log_decay.device != q.device:
-        raise ValueError(f"{name}: log_decay must be float32 of one entry per head on {q.device}")
-    if any(t.dim() != dims for t in (q, k, v)) or q.shape[:-2] != k.shape[:-2] or q.shape[:-2] != v.shape[:-2] \
-            or q.shape[-1] != k.shape[-1]:
-        raise ValueError(f"{name}: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, want "
+    """Checks what the decay-attention calls share; (type, device, B, L, H, Hq, Hk, Hv, Dk, Dv, log_decay)."""
+    dt, dev = _acts(name, q, k, v)
+    qsh, ksh, vsh = q.shape, k.shape, v.shape
+    if len(qsh) != dims or len(ksh) != dims or len(vsh) != dims or qsh[:-2] != ksh[:-2] or qsh[:-2] != vsh[:-2] \
+            or qsh[-1] != ksh[-1]:
+        raise ValueError(f"{name}: q {tuple(qsh)}, k {tuple(ksh)}, v {tuple(vsh)}, want "
                          f"({'B, L' if dims == 4 else 'B'}, heads, D)")
-    return (q.shape[0], q.shape[1] if dims == 4 else 1, log_decay.numel(), q.shape[-2], k.shape[-2], v.shape[-2],
-            q.shape[-1], v.shape[-1])
-
-
-def _state_arg(name, t, shape, device):
-    if t is None:
-        return None
-    if tuple(t.shape) != tuple(shape) or t.dtype != torch.float32 or t.device != device:
-        raise ValueError(f"{name}: state {t.dtype} {tuple(t.shape)} on {t.device}, want float32 {tuple(shape)} on {device}")
-    return t.contiguous()
-
-
-def _lengths_arg(name, lengths, B, device):
-    if lengths is None:
-        return None
-    _cuda(lengths)
-    if lengths.dtype.is_floating_point or tuple(lengths.shape) != (B,) or lengths.device != device:
-        raise ValueError(f"{name}: lengths {lengths.dtype} {tuple(lengths.shape)}, want whole numbers ({B},) on {device}")
-    return lengths.to(torch.int32).contiguous()
+    H = log_decay.numel()
+    log_decay = _param(f"{name}: log_decay", log_decay, (H,), dev)
+    return dt, dev, qsh[0], qsh[1] if dims == 4 else 1, H, qsh[-2], ksh[-2], vsh[-2], qsh[-1], vsh[-1], log_decay
 
 
 def decay_attn_fwd(q, k, v, log_decay, *, scale: Optional[float] = None, state=None, lengths=None,
@@ -978,49 +992,54 @@ def decay_attn_fwd(q, k, v, log_decay, *, scale: Optional[float] = None, state=N
     defaults to Dk^-0.5.  state: float32 (B, H, Dk, Dv) that came before (None: zeros); lengths (B):
     tokens past a row's length are not there."""
     name = "decay_attn_fwd"
-    B, L_, H, Hq, Hk, Hv, Dk, Dv = _decay_args(name, q, k, v, log_decay, 4)
-    state = _state_arg(name, state, (B, H, Dk, Dv), q.device)
-    lengths = _lengths_arg(name, lengths, B, q.device)
+    dt, dev, B, L_, H, Hq, Hk, Hv, Dk, Dv, log_decay = _decay_args(name, q, k, v, log_decay, 4)
+    if state is not None:
+        state = _param(f"{name}: state", state, (B, H, Dk, Dv), dev)
+    if lengths is not None:
+        lengths = _whole(name, "lengths", lengths, (B,), dev, torch.int32)
     (q, qs), (k, ks), (v, vs) = _view(q), _view(k), _view(v)
-    out = torch.empty(B, L_, H, Dv, dtype=q.dtype, device=q.device)
-    end = torch.empty(B, H, Dk, Dv, dtype=torch.float32, device=q.device) if want_state else None
+    out = v.new_empty((B, L_, H, Dv))
+    end = log_decay.new_empty((B, H, Dk, Dv)) if want_state else None
     L = lib()
-    ws = _ws(L.pgf_decay_attn_workspace(B, L_, H, Hq, Hk, Hv, Dk, Dv, _dt(q), 0), q.device)
-    check(L.pgf_decay_attn_fwd(_p(q), qs, _p(k), ks, _p(v), vs, _p(_c(log_decay)), _p(state), _p(lengths), _p(out),
-                               _p(end), B, L_, H, Hq, Hk, Hv, Dk, Dv, Dk ** -0.5 if scale is None else scale, _dt(q),
-                               _p(ws), ws.numel(), _stream()), name)
+    nws = L.pgf_decay_attn_workspace(B, L_, H, Hq, Hk, Hv, Dk, Dv, dt, 0)
+    ws = q.new_empty(nws, dtype=torch.uint8) if nws else None
+    check(L.pgf_decay_attn_fwd(q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, log_decay.data_ptr(), _p(state),
+                               _p(lengths), out.data_ptr(), _p(end), B, L_, H, Hq, Hk, Hv, Dk, Dv,
+                               Dk ** -0.5 if scale is None else scale, dt, _p(ws), nws, _raw_stream(dev)), name)
     return out, end
 
 
 def decay_attn_bwd(q, k, v, log_decay, g, *, scale: Optional[float] = None, state=None, g_state=None, lengths=None,
                    need_g_log_decay: bool = False, g_log_decay_acc=None) -> Dict[str, torch.Tensor]:
     """Gradients of decay_attn_fwd from its inputs, g (of out) and g_state (of the final state, None:
-    zeros): grad_q, grad_k, grad_v, grad_state (float32, of the state that came before; with `state`
-    or g_state given or not) and, when asked for, grad_log_decay (H) float32."""
+    zeros): grad_q, grad_k, grad_v, grad_state (float32, of the state that came before, given or not)
+    and, when asked for, grad_log_decay (H) float32 (added into g_log_decay_acc if that is given)."""
     name = "decay_attn_bwd"
-    B, L_, H, Hq, Hk, Hv, Dk, Dv = _decay_args(name, q, k, v, log_decay, 4)
-    _cuda(g)
-    _same(name, q, g)
-    if tuple(g.shape) != (B, L_, H, Dv):
+    dt, dev, B, L_, H, Hq, Hk, Hv, Dk, Dv, log_decay = _decay_args(name, q, k, v, log_decay, 4)
+    _acts(name, q, g)
+    if g.shape != (B, L_, H, Dv):
         raise ValueError(f"{name}: gradient {tuple(g.shape)} of an output {(B, L_, H, Dv)}")
-    state = _state_arg(name, state, (B, H, Dk, Dv), q.device)
-    g_state = _state_arg(name, g_state, (B, H, Dk, Dv), q.device)
-    lengths = _lengths_arg(name, lengths, B, q.device)
+    if state is not None:
+        state = _param(f"{name}: state", state, (B, H, Dk, Dv), dev)
+    if g_state is not None:
+        g_state = _param(f"{name}: g_state", g_state, (B, H, Dk, Dv), dev)
+    if lengths is not None:
+        lengths = _whole(name, "lengths", lengths, (B,), dev, torch.int32)
     (q, qs), (k, ks), (v, vs), (g, gs) = _view(q), _view(k), _view(v), _view(g)
-    dev = q.device
-    out = {"grad_q": torch.empty(q.shape, dtype=q.dtype, device=dev),
-           "grad_k": torch.empty(k.shape, dtype=q.dtype, device=dev),
-           "grad_v": torch.empty(v.shape, dtype=q.dtype, device=dev),
-           "grad_state": torch.empty(B, H, Dk, Dv, dtype=torch.float32, device=dev)}
-    accum = 0
+    gq, gk, gv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
+    g0 = log_decay.new_empty((B, H, Dk, Dv))
+    out = {"grad_q": gq, "grad_k": gk, "grad_v": gv, "grad_state": g0}
+    gl, accum = None, 0
     if need_g_log_decay or g_log_decay_acc is not None:
-        out["grad_log_decay"], accum = _acc_buffer(g_log_decay_acc, (H,), dev, name)
+        gl, accum = _acc_buffer(g_log_decay_acc, (H,), q.device, name)
+        out["grad_log_decay"] = gl
     L = lib()
-    ws = _ws(L.pgf_decay_attn_workspace(B, L_, H, Hq, Hk, Hv, Dk, Dv, _dt(q), 1), dev)
-    check(L.pgf_decay_attn_bwd(_p(q), qs, _p(k), ks, _p(v), vs, _p(_c(log_decay)), _p(state), _p(lengths), _p(g), gs,
-                               _p(g_state), _p(out["grad_q"]), _p(out["grad_k"]), _p(out["grad_v"]),
-                               _p(out.get("grad_log_decay")), _p(out["grad_state"]), accum, B, L_, H, Hq, Hk, Hv, Dk, Dv,
-                               Dk ** -0.5 if scale is None else scale, _dt(q), _p(ws), ws.numel(), _stream()), name)
+    nws = L.pgf_decay_attn_workspace(B, L_, H, Hq, Hk, Hv, Dk, Dv, dt, 1)
+    ws = q.new_empty(nws, dtype=torch.uint8) if nws else None
+    check(L.pgf_decay_attn_bwd(q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, log_decay.data_ptr(), _p(state),
+                               _p(lengths), g.data_ptr(), gs, _p(g_state), gq.data_ptr(), gk.data_ptr(), gv.data_ptr(),
+                               _p(gl), g0.data_ptr(), accum, B, L_, H, Hq, Hk, Hv, Dk, Dv,
+                               Dk ** -0.5 if scale is None else scale, dt, _p(ws), nws, _raw_stream(dev)), name)
     return out
 
 
@@ -1029,22 +1048,25 @@ def decay_attn_step(q, k, v, log_decay, state, *, scale: Optional[float] = None,
     rows (B): row b goes on from state row rows[b] (a beam's parent) instead of its own.  out_state:
     where the new state goes (`state` itself updates in place, without rows); default a new tensor."""
     name = "decay_attn_step"
-    B, _, H, Hq, Hk, Hv, Dk, Dv = _decay_args(name, q, k, v, log_decay, 3)
-    _cuda(state, rows, out_state)
-    n_src = B if rows is None else state.shape[0]
+    dt, dev, B, _, H, Hq, Hk, Hv, Dk, Dv, log_decay = _decay_args(name, q, k, v, log_decay, 3)
+    n_src = B
+    if rows is not None:
+        n_src = state.shape[0]
+        rows = _whole(name, "rows", rows, (B,), dev, torch.int64)
     if not state.is_contiguous():
         raise ValueError(f"{name}: state must be contiguous")
-    state = _state_arg(name, state, (n_src, H, Dk, Dv), q.device)
-    if rows is not None:
-        if rows.dtype.is_floating_point or tuple(rows.shape) != (B,):
-            raise ValueError(f"{name}: rows {rows.dtype} {tuple(rows.shape)}, want whole numbers ({B},)")
-        rows = rows.long().contiguous()
-    new = _out_buf(out_state, (B, H, Dk, Dv), torch.float32, q.device, name)
+    state = _param(f"{name}: state", state, (n_src, H, Dk, Dv), dev)
+    if out_state is None:
+        new = state.new_empty((B, H, Dk, Dv))
+    else:
+        new = _param(f"{name}: out_state", out_state, (B, H, Dk, Dv), dev)
+        if new is not out_state:
+            raise ValueError(f"{name}: out_state must be contiguous")
     (q, qs), (k, ks), (v, vs) = _view(q), _view(k), _view(v)
-    out = torch.empty(B, H, Dv, dtype=q.dtype, device=q.device)
-    check(lib().pgf_decay_attn_step(_p(q), qs, _p(k), ks, _p(v), vs, _p(_c(log_decay)), _p(state), _p(rows), n_src,
-                                    _p(out), _p(new), B, H, Hq, Hk, Hv, Dk, Dv, Dk ** -0.5 if scale is None else scale,
-                                    _dt(q), _stream()), name)
+    out = v.new_empty((B, H, Dv))
+    check(lib().pgf_decay_attn_step(q.data_ptr(), qs, k.data_ptr(), ks, v.data_ptr(), vs, log_decay.data_ptr(),
+                                    state.data_ptr(), _p(rows), n_src, out.data_ptr(), new.data_ptr(), B, H, Hq, Hk, Hv,
+                                    Dk, Dv, Dk ** -0.5 if scale is None else scale, dt, _raw_stream(dev)), name)
     return out, new
 
 
@@ -1056,22 +1078,23 @@ def beam_select(logits, scores, finished=None, *, end_id: Optional[int] = None):
     that each new beam goes on from (for beam_reorder and decay_attn_step).  finished (B, K) bool: such
     a beam's one candidate is end_id at its own score.  A NaN candidate counts as -inf."""
     name = "beam_select"
-    _cuda(logits, scores, finished)
-    if logits.dim() != 3 or tuple(scores.shape) != tuple(logits.shape[:2]):
-        raise ValueError(f"{name}: logits {tuple(logits.shape)} and scores {tuple(scores.shape)}, want (B, K, V), (B, K)")
-    if scores.dtype != torch.float32:
-        raise TypeError(f"{name}: scores must be float32, not {scores.dtype}")
-    if finished is not None and (finished.dtype != torch.bool or finished.shape != scores.shape):
-        raise ValueError(f"{name}: finished must be bool {tuple(scores.shape)}")
-    dt = _dt(logits)
-    B, K, V = logits.shape
-    logits, scores, finished = _c(logits), _c(scores), _c(finished)
-    so = torch.empty(B, K, dtype=torch.float32, device=logits.device)
-    rows = torch.empty(B, K, dtype=torch.int64, device=logits.device)
-    tokens = torch.empty_like(rows)
-    fo = torch.empty(B, K, dtype=torch.bool, device=logits.device)
-    check(lib().pgf_beam_select(_p(logits), _p(scores), _p(finished), _p(so), _p(rows), _p(tokens), _p(fo), B, K, V,
-                                -1 if end_id is None else end_id, dt, _stream()), name)
+    dt, dev = _acts(name, logits)
+    shape = logits.shape
+    if len(shape) != 3 or scores.shape != shape[:2]:
+        raise ValueError(f"{name}: logits {tuple(shape)} and scores {tuple(scores.shape)}, want (B, K, V), (B, K)")
+    B, K, V = shape
+    scores = _param(f"{name}: scores", scores, (B, K), dev)
+    if finished is not None:
+        if finished.dtype is not torch.bool or finished.shape != (B, K) or finished.get_device() != dev:
+            raise ValueError(f"{name}: finished must be bool {(B, K)} on cuda:{dev}")
+        finished = finished.contiguous()
+    logits = logits.contiguous()
+    so = scores.new_empty((B, K))
+    rows, tokens = scores.new_empty((2, B, K), dtype=torch.int64).unbind(0)
+    fo = scores.new_empty((B, K), dtype=torch.bool)
+    check(lib().pgf_beam_select(logits.data_ptr(), scores.data_ptr(), _p(finished), so.data_ptr(), rows.data_ptr(),
+                                tokens.data_ptr(), fo.data_ptr(), B, K, V, -1 if end_id is None else end_id, dt,
+                                _raw_stream(dev)), name)
     return so, rows, tokens, fo
 
 
@@ -1079,22 +1102,28 @@ def beam_reorder(states, rows, out=None):
     """[s[rows] for s in states], in one launch: states of any type, (n, ...) contiguous; rows of any
     shape (flattened).  out: contiguous tensors to write (not the states themselves)."""
     name = "beam_reorder"
-    states = list(states)
-    _cuda(rows, *states)
-    if rows.dtype.is_floating_point:
-        raise TypeError(f"{name}: rows must be whole numbers, not {rows.dtype}")
-    rows = rows.reshape(-1).long().contiguous()
-    if not states:
+    dev = rows.get_device()
+    if dev < 0:
+        raise RuntimeError("icml_b200 operators run on CUDA tensors only (no CPU path)")
+    rows = _whole(name, "rows", rows, rows.shape, dev, torch.int64)
+    n, c = rows.numel(), len(states)
+    if c == 0:
         return []
-    n_src, n = states[0].shape[0], rows.numel()
-    states = [_c(s) for s in states]
-    if any(s.shape[0] != n_src or s.device != rows.device for s in states):
-        raise ValueError(f"{name}: every state needs {n_src} rows on {rows.device}")
-    outs = [_out_buf(None if out is None else out[i], (n, *s.shape[1:]), s.dtype, s.device, name)
-            for i, s in enumerate(states)]
-    c = len(states)
-    src = (ctypes.c_void_p * c)(*[s.data_ptr() for s in states])
-    dst = (ctypes.c_void_p * c)(*[o.data_ptr() for o in outs])
-    nb = (ctypes.c_int64 * c)(*[math.prod(s.shape[1:]) * s.element_size() for s in states])
-    check(lib().pgf_beam_reorder(src, dst, nb, c, _p(rows), n, n_src, _stream()), name)
+    n_src = states[0].shape[0]
+    src, dst, nb = (ctypes.c_void_p * c)(), (ctypes.c_void_p * c)(), (ctypes.c_int64 * c)()
+    keep, outs = [], []
+    for i, s in enumerate(states):
+        shape = s.shape
+        if shape[0] != n_src or s.get_device() != dev:
+            raise ValueError(f"{name}: every state needs {n_src} rows on cuda:{dev}")
+        if not s.is_contiguous():
+            s = s.contiguous()
+            keep.append(s)
+        want = (n, *shape[1:])
+        o = s.new_empty(want) if out is None else out[i]
+        if out is not None and (o.shape != want or o.dtype is not s.dtype or o.get_device() != dev or not o.is_contiguous()):
+            raise ValueError(f"{name}: out must be contiguous {want} {s.dtype} on cuda:{dev}")
+        outs.append(o)
+        src[i], dst[i], nb[i] = s.data_ptr(), o.data_ptr(), math.prod(shape[1:]) * s.element_size()
+    check(lib().pgf_beam_reorder(src, dst, nb, c, rows.data_ptr(), n, n_src, _raw_stream(dev)), name)
     return outs
