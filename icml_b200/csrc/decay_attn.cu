@@ -567,7 +567,7 @@ static size_t workspace(const Shape& p, bool backward) {
   if (pieces) n += (backward ? 2 : 1) * (Workspace::round(pieces) + 256);
   if (backward) {
     const int segs = f.c.segs > t.c.segs ? f.c.segs : t.c.segs;
-    n += Workspace::round(size_t(p.H) * p.B * segs * ceil_div(p.Dv, E) * sizeof(float)) + 256;
+    n += Workspace::round(size_t(p.H) * p.B * segs * ceil_div(p.Dk, 64) * ceil_div(p.Dv, 64) * sizeof(float)) + 256;
     const size_t tok = size_t(p.B) * p.L * p.H * sizeof(float);
     if (p.Hq < p.H) n += Workspace::round(tok * p.Dk) + 256;
     if (p.Hk < p.H) n += Workspace::round(tok * p.Dk) + 256;
@@ -677,7 +677,7 @@ extern "C" int pgf_decay_attn_bwd(const void* q, const pgf_strides* q_strides, c
   const size_t states = size_t(Bsz) * H * job.segs * Dk * Dv;
   float* sp = job.segs > 1 ? w.take<float>(states) : nullptr;
   float* xp = job.segs > 1 ? w.take<float>(states) : nullptr;
-  float* part = grad_log_decay ? w.take<float>(size_t(H) * Bsz * job.segs * ceil_div(Dv, da::E)) : nullptr;
+  float* part = grad_log_decay ? w.take<float>(size_t(H) * Bsz * job.segs * ceil_div(Dk, 64) * ceil_div(Dv, 64)) : nullptr;
   const int64_t tokens = Bsz * L;
   float* pq = Hq < H ? w.take<float>(size_t(tokens) * H * Dk) : nullptr;
   float* pk = Hk < H ? w.take<float>(size_t(tokens) * H * Dk) : nullptr;
@@ -723,18 +723,35 @@ extern "C" int pgf_decay_attn_bwd(const void* q, const pgf_strides* q_strides, c
   jk.out_f32 = f32 || pk;
   PGF_TRY(da::f_call(jk, pl, dtype, s));
   if (grad_log_decay) {
-    da::Job jt = job;
-    jt.x = tq; jt.y = tk; jt.z = tv;
-    jt.start = S.p; jt.start_stride = S.stride;
-    jt.z_scale = 1.f;
-    da::TangentArgs t = {};
-    t.g = tg;
-    t.behind = X.p;
-    t.behind_stride = X.stride;
-    t.part = part;
-    t.scale = scale;
-    PGF_TRY(da::walk<da::MODE_TANGENT>(jt, t, dtype, s));
-    da::decay_sum_kernel<<<unsigned(H), 256, 0, s>>>(part, grad_log_decay, Bsz * job.segs * ceil_div(Dv, da::E), accumulate);
+    int parts;
+    if (tc) {
+      da::TangentJob t = {};
+      t.q = tq; t.k = tk; t.v = tv; t.g = tg;
+      t.log_decay = log_decay;
+      t.lengths = lengths;
+      t.start = S.p; t.start_stride = S.stride;
+      t.behind = X.p; t.behind_stride = X.stride;
+      t.part = part;
+      t.scale = scale;
+      t.B = Bsz; t.L = L; t.seg_len = job.seg_len;
+      t.H = int(H); t.segs = job.segs;
+      PGF_TRY(da::tc_tangent(t, s));
+      parts = da::tc_tangent_blocks(Dk, Dv);
+    } else {
+      da::Job jt = job;
+      jt.x = tq; jt.y = tk; jt.z = tv;
+      jt.start = S.p; jt.start_stride = S.stride;
+      jt.z_scale = 1.f;
+      da::TangentArgs t = {};
+      t.g = tg;
+      t.behind = X.p;
+      t.behind_stride = X.stride;
+      t.part = part;
+      t.scale = scale;
+      PGF_TRY(da::walk<da::MODE_TANGENT>(jt, t, dtype, s));
+      parts = ceil_div(Dv, da::E);
+    }
+    da::decay_sum_kernel<<<unsigned(H), 256, 0, s>>>(part, grad_log_decay, Bsz * job.segs * parts, accumulate);
     PGF_LAUNCH_CHECK();
   }
   if (L == 0) return PGF_OK;

@@ -30,7 +30,6 @@
 // P takes two multiplications for 32 x 32 blocks off the diagonal (a^(i-j) as a row factor times a column factor,
 // both with exponents >= 0: no overflow for any decay), a table look-up for the four on it, nothing for the rest.
 #include "decay_attn_tc.cuh"
-#include "f32x2.cuh"
 
 namespace pgf {
 namespace da {
@@ -39,7 +38,6 @@ namespace {
 
 constexpr int C = TC_CHUNK;
 constexpr int THREADS = 640;
-constexpr uint32_t BLK = 16384;   // 128 rows x 64 bf16 columns, 128B swizzle
 constexpr uint32_t TMEM_COLS = 512;
 
 // NT: bf16 terms of the weighted y.  3 keep the state to float32 accuracy; 2 (2^-17) are enough where the state
@@ -73,79 +71,6 @@ struct Params {
   int64_t L, seg_len;
   int H, segs, dx, dz, start_t, out_f32, last_too, wide;
   int gx, gy, gz;              // operator heads per tensor head
-};
-
-__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2, int c3) {
-  asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
-      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
-      : "memory");
-}
-__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2, int c3) {
-  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%1, %2, %3, %4}], [%5];"
-               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(src)
-               : "memory");
-}
-__device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-}
-__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void lds128(uint32_t a, uint32_t (&v)[4]) {
-  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a));
-}
-__device__ __forceinline__ void sts128(uint32_t a, const uint32_t (&v)[4]) {
-  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
-}
-// Reads of the tables, which stay as they are once the CTA has written them (shared addresses: a load through a
-// generic pointer is a slower one).
-__device__ __forceinline__ float lds_f(uint32_t a) {
-  float v;
-  asm("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ uint2 lds_u2(uint32_t a) {
-  uint2 v;
-  asm("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ float4 lds_f4(uint32_t a) {
-  float4 v;
-  asm("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
-  return v;
-}
-__device__ __forceinline__ float2 unpack2(uint32_t v) {
-  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
-}
-__device__ __forceinline__ uint32_t pack2(float2 v) { return pack_bf16(v.x, v.y); }
-
-// Bounded warp-wide wait: one try before the clock is read (most waits find their phase complete).
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
-  uint32_t done;
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-      "selp.u32 %0, 1, 0, p;\n\t}\n"
-      : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
-  if (__all_sync(0xffffffffu, done)) return true;
-  return mbar_wait_warp(bar, parity);
-}
-// A matrix descriptor (sdesc) whose start moves by whole 16-byte units: the address field is the low 14 bits
-// and shared memory ends below 2^18, so a step never carries out of it.
-struct Desc {
-  uint32_t lo, hi;
-  __device__ __forceinline__ Desc(uint32_t saddr, uint32_t lbo) {
-    const uint64_t d = sdesc(saddr, lbo, 1024);
-    lo = uint32_t(d);
-    hi = uint32_t(d >> 32);
-  }
-  __device__ __forceinline__ uint64_t at(uint32_t bytes) const { return uint64_t(hi) << 32 | (lo + (bytes >> 4)); }
 };
 
 // Barriers behind full[NS] and empty[NS].  A and P take turns where there are two A buffers: X may be a chunk
@@ -692,20 +617,6 @@ walk_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
   __syncthreads();
   if (w.warp == 0)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(w.tmem), "r"(TMEM_COLS));
-}
-
-// (D, heads, L, B) with a box of 64 columns x 128 tokens of one head; zeros outside.
-bool make_tensor_map(CUtensorMap* m, const Tensor& t, int64_t B, int64_t L) {
-  EncodeTiledFn fn = encode_fn();
-  if (!fn) return false;
-  cuuint64_t dims[4] = {cuuint64_t(t.d), cuuint64_t(t.heads), cuuint64_t(L), cuuint64_t(B)};
-  // the stride of a dimension of one entry is never used, but has to be a valid one
-  cuuint64_t st[3] = {cuuint64_t(t.heads > 1 ? t.s.head : t.d) * 2, cuuint64_t(L > 1 ? t.s.token : t.d) * 2,
-                      cuuint64_t(B > 1 ? t.s.batch : t.d) * 2};
-  cuuint32_t box[4] = {64, 1, C, 1}, es[4] = {1, 1, 1, 1};
-  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(t.p), dims, st, box, es,
-            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 bool fits(const Tensor& t, int64_t B, int64_t L) {

@@ -1,18 +1,123 @@
-// The tensor-core engine of the decay attention, as the entry points call it.
+// The tensor-core engine of the decay attention: its entry points and what its kernels share.
 #pragma once
 #include "decay_attn.cuh"
+#include "f32x2.cuh"
 #include "tc_common.cuh"
 
 namespace pgf {
 namespace da {
 
 constexpr int TC_CHUNK = 128;
+constexpr uint32_t BLK = 16384;   // a tile of 128 rows x 64 bf16 columns, 128B swizzle
 
 // Whether a bf16 tensor can be read by the engine's TMA loads: 16-byte aligned base, pitches and width, at
 // most 128 wide.
 bool tc_fits(const Tensor& t, int64_t B, int64_t L);
 // One F call, or only the pieces' own end states (into job.start).  job.seg_len: a multiple of TC_CHUNK.
 int tc_walk(const Job& job, bool state_only, cudaStream_t s);
+
+// grad ln a: partial sums (H, B, segs, blocks), blocks = tc_tangent_blocks(Dk, Dv).  start: the state that enters
+// each piece, behind: the adjoint (scaled) of the state behind it; NULL: zeros.
+struct TangentJob {
+  Tensor q, k, v, g;
+  const float* log_decay;
+  const int32_t* lengths;
+  const float *start, *behind;
+  int64_t start_stride, behind_stride;
+  float* part;
+  float scale;
+  int64_t B, L, seg_len;
+  int H, segs;
+};
+static inline int tc_tangent_blocks(int64_t dk, int64_t dv) { return ceil_div(dk, 64) * ceil_div(dv, 64); }
+int tc_tangent(const TangentJob& job, cudaStream_t s);
+
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2, int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+__device__ __forceinline__ void tma_store_4d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.bulk_group [%0, {%1, %2, %3, %4}], [%5];"
+               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(src)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_ld16_nowait(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void lds128(uint32_t a, uint32_t (&v)[4]) {
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]) : "r"(a));
+}
+__device__ __forceinline__ void sts128(uint32_t a, const uint32_t (&v)[4]) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+}
+// Reads of the tables, which stay as they are once the CTA has written them (shared addresses: a load through a
+// generic pointer is a slower one).
+__device__ __forceinline__ float lds_f(uint32_t a) {
+  float v;
+  asm("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ uint2 lds_u2(uint32_t a) {
+  uint2 v;
+  asm("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ float4 lds_f4(uint32_t a) {
+  float4 v;
+  asm("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ float2 unpack2(uint32_t v) {
+  return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
+}
+__device__ __forceinline__ uint32_t pack2(float2 v) { return pack_bf16(v.x, v.y); }
+
+// Bounded warp-wide wait: one try before the clock is read (most waits find their phase complete).
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(done) : "r"(smem_u32(bar)), "r"(parity) : "memory");
+  if (__all_sync(0xffffffffu, done)) return true;
+  return mbar_wait_warp(bar, parity);
+}
+// A matrix descriptor (sdesc) whose start moves by whole 16-byte units: the address field is the low 14 bits
+// and shared memory ends below 2^18, so a step never carries out of it.
+struct Desc {
+  uint32_t lo, hi;
+  __device__ __forceinline__ Desc(uint32_t saddr, uint32_t lbo) {
+    const uint64_t d = sdesc(saddr, lbo, 1024);
+    lo = uint32_t(d);
+    hi = uint32_t(d >> 32);
+  }
+  __device__ __forceinline__ uint64_t at(uint32_t bytes) const { return uint64_t(hi) << 32 | (lo + (bytes >> 4)); }
+};
+
+// (D, heads, L, B) with a box of 64 columns x 128 tokens of one head; zeros outside.
+static inline bool make_tensor_map(CUtensorMap* m, const Tensor& t, int64_t B, int64_t L) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  cuuint64_t dims[4] = {cuuint64_t(t.d), cuuint64_t(t.heads), cuuint64_t(L), cuuint64_t(B)};
+  // the stride of a dimension of one entry is never used, but has to be a valid one
+  cuuint64_t st[3] = {cuuint64_t(t.heads > 1 ? t.s.head : t.d) * 2, cuuint64_t(L > 1 ? t.s.token : t.d) * 2,
+                      cuuint64_t(B > 1 ? t.s.batch : t.d) * 2};
+  cuuint32_t box[4] = {64, 1, TC_CHUNK, 1}, es[4] = {1, 1, 1, 1};
+  return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(t.p), dims, st, box, es,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 
 }  // namespace da
 }  // namespace pgf
