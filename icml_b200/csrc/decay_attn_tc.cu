@@ -69,7 +69,7 @@ struct Params {
   float* end;
   float scale, z_scale;
   int64_t L, seg_len;
-  int H, segs, dx, dz, start_t, out_f32, last_too, wide;
+  int H, segs, dx, dz, start_t, out_f32, last_too;
   int gx, gy, gz;              // operator heads per tensor head
 };
 
@@ -142,7 +142,7 @@ struct Walk {
   }
 
   // ---- warp 1.  A tile's slot is released by the last product that reads it (z's by the output's store).  With
-  // two A buffers A of the next chunk goes first; with one it follows the product that reads P, and D1 comes last.
+  // two A buffers A of the next chunk goes first; with one it comes last.
   __device__ void mma() const {
     const bool leader = elect_one();
     const uint32_t id_a = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(C >> 3) << 17) | (uint32_t(C >> 4) << 24);
@@ -203,7 +203,6 @@ struct Walk {
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)  // P of columns 0..63 and 64..127 lies where each half of A was
           umma_bf16_ta(tmem + G::T_D2, pa + (kk >> 2) * 64 + (kk & 3) * 8, dz.at(kk * 2048), id_d, kk > 0);
-        if (G::NS == 5) umma_commit(&empty[slot(tile_z(c))]);
       }
       __syncwarp();
       if (!wait(B_S, c)) return;
@@ -309,25 +308,6 @@ struct Walk {
             if (col + 4 * k < p.dz)
               *reinterpret_cast<float4*>(dst + 4 * k) = make_float4(o[2 * k].x, o[2 * k].y, o[2 * k + 1].x, o[2 * k + 1].y);
         }
-      } else if (G::NS == 5) {
-        if (t0 + i < p.L) {
-          __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(p.out) + ((b * p.L + t0 + i) * p.H + h) * p.dz + col;
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float2* v = o + 8 * k;
-            if (p.wide) {  // 32 bytes: the width is a multiple of 16
-              if (col + 16 * k < p.dz)
-                asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + 16 * k), "r"(pack2(v[0])),
-                             "r"(pack2(v[1])), "r"(pack2(v[2])), "r"(pack2(v[3])), "r"(pack2(v[4])), "r"(pack2(v[5])),
-                             "r"(pack2(v[6])), "r"(pack2(v[7])) : "memory");
-            } else {
-              if (col + 16 * k < p.dz)
-                *reinterpret_cast<uint4*>(dst + 16 * k) = make_uint4(pack2(v[0]), pack2(v[1]), pack2(v[2]), pack2(v[3]));
-              if (col + 16 * k + 8 < p.dz)
-                *reinterpret_cast<uint4*>(dst + 16 * k + 8) = make_uint4(pack2(v[4]), pack2(v[5]), pack2(v[6]), pack2(v[7]));
-            }
-          }
-        }
       } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -339,10 +319,8 @@ struct Walk {
         }
       }
     }
-    if (G::NS != 5) {
     fence_async();
     arrive(B_OSTAGED);
-    }
     return true;
   }
 
@@ -611,7 +589,7 @@ walk_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
   } else if (w.warp < 18) {
     w.state();
   } else if (w.warp == 18) {
-    if (!STATE_ONLY && G::NS != 5) w.store(&tmO);
+    if (!STATE_ONLY) w.store(&tmO);
   }
   tc_before();
   __syncthreads();
@@ -665,7 +643,6 @@ int launch(const Job& j, cudaStream_t s) {
   p.start_t = j.start_t;
   p.out_f32 = j.out_f32;
   p.last_too = j.last_too;
-  p.wide = j.z.d % 16 == 0 && aligned(j.out, 32);
   p.gx = STATE_ONLY ? 1 : j.H / j.x.heads;
   p.gy = j.H / j.y.heads;
   p.gz = j.H / j.z.heads;
