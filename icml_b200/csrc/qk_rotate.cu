@@ -42,6 +42,7 @@ struct Args {
   int64_t start;
   int64_t tokens, L;
   int D, R;
+  int flat[2];             // token t of row b stands at (b L + t) times the token stride
   int tw[2], ctas[2];      // tokens of a warp's tile, CTAs
   float eps;
   float* part;             // (CTAs, D) of the queries, then of the keys, backward only
@@ -54,8 +55,9 @@ __device__ __forceinline__ float2 turn_of(int64_t turns, int64_t pos) {
   const uint64_t phase = uint64_t(pos) * uint64_t(turns);
   const uint32_t hi = uint32_t(phase >> 32) + 0x20000000u;
   const uint32_t quadrant = hi >> 30;
-  const int64_t rest = int64_t(phase - (uint64_t(quadrant) << 62));
-  const float x = __ll2float_rn(rest) * 3.4061215800304796e-19f;   // 2 pi / 2^64
+  // the rest, within an eighth of a turn, to 2^-34 of a turn
+  const int32_t rest = int32_t(uint32_t(phase >> 30));   // the quadrant's bits fall off
+  const float x = float(rest) * 3.6572952e-10f;          // 2 pi / 2^34
   const float z = x * x;
   float s = fmaf(z, -1.0f / 39916800.0f, 1.0f / 362880.0f);
   s = fmaf(s, z, -1.0f / 5040.0f);
@@ -80,6 +82,12 @@ __device__ __forceinline__ float inv_sqrt(float x) {
   const float r = rsqrtf(x);
   const float e = fmaf(-x * r, r, 1.0f);
   return x < INFINITY ? fmaf(0.5f * r, e, r) : r;
+}
+
+__device__ __forceinline__ float4 lds4(uint32_t at) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at));
+  return v;
 }
 
 template <class T> struct Vec;
@@ -180,12 +188,20 @@ __global__ void __launch_bounds__(THREADS, 2) rotate_kernel(const Args a, int G)
       i1 = i0 + W;
     }
   }
+  // the lane's weights: registers in the forward; the backward, whose registers are full, reads them for each row
+  // from shared memory (W / 2 fours, slots)
   float2 w[W];
 #pragma unroll
   for (int e = 0; e < W; ++e) {
     const int i = e < W / 2 ? i0 + 2 * e : i1 + 2 * e - W;
     w[e] = a.w[z] ? make_float2(a.w[z][i], a.w[z][i + 1]) : f2(1.f);
   }
+  float4* sw = reinterpret_cast<float4*>(st + (np + 1) / 2 * 2) + WARPS * tw * (W / 2) * slots;
+  if (BWD && warp == 0 && gi == 0 && live) {
+#pragma unroll
+    for (int e = 0; e < W / 2; ++e) sw[e * slots + slot] = make_float4(w[2 * e].x, w[2 * e].y, w[2 * e + 1].x, w[2 * e + 1].y);
+  }
+  const uint32_t w_at = static_cast<uint32_t>(__cvta_generic_to_shared(sw + place));
   for (int i = threadIdx.x; i < a.R / 2; i += THREADS) st[i] = a.turns[i];
   __syncthreads();
   float2 acc[BWD ? W : 1];
@@ -206,10 +222,9 @@ __global__ void __launch_bounds__(THREADS, 2) rotate_kernel(const Args a, int G)
     const int64_t tok = tile_a * tw + t;
     mine_a = live && tok < a.tokens;
     if (!mine_a) return;
-    int64_t b, l;
-    if (a.tokens <= 0x7fffffff) { b = uint32_t(tok) / uint32_t(a.L); l = uint32_t(tok) - uint32_t(b) * uint32_t(a.L); }
-    else { b = tok / a.L; l = tok % a.L; }
-    px = any + b * a.xs[z].batch + l * a.xs[z].token + h0 * a.xs[z].head + i0;
+    int64_t at = tok * a.xs[z].token;
+    if (!a.flat[z]) at += tok / a.L * (a.xs[z].batch - a.L * a.xs[z].token);
+    px = any + at + h0 * a.xs[z].head + i0;
     if (BWD) pg = static_cast<const T*>(a.g[z]) + (tok * H + h0) * D + i0;
   };
   auto copy = [&](int at, const T* src, bool on) {
@@ -245,15 +260,21 @@ __global__ void __launch_bounds__(THREADS, 2) rotate_kernel(const Args a, int G)
     return v;
   };
   int64_t tile = tile_a;
+  // lane tt < tw: the position of token tt of the next tile, a tile ahead of its use
+  auto position_at = [&](int64_t tl) {
+    const int64_t tk = tl * tw + lane;
+    return lane < tw && tl < tiles && tk < a.tokens ? position_of(a, tk) : 0;
+  };
+  int64_t pos_next = position_at(tile);
   if (tile < tiles) locate();
   for (int q = 0; q < STAGES - 1; ++q) issue(q);
   int stage = 0;
   for (; tile < tiles; tile += step) {
+    const int64_t pos_tile = pos_next;
+    pos_next = position_at(tile + step);
     __syncwarp();
     for (int tt = 0; tt < tw; ++tt) {
-      const int64_t tk = tile * tw + tt;
-      if (tk >= a.tokens) break;
-      const int64_t pos = position_of(a, tk);
+      const int64_t pos = __shfl_sync(0xffffffffu, pos_tile, tt);
       for (int j = lane; j < np; j += 32) {
         float2 v = make_float2(1.f, 0.f);
         if (2 * j < a.R) v = turn_of(st[j], pos);
@@ -289,9 +310,10 @@ __global__ void __launch_bounds__(THREADS, 2) rotate_kernel(const Args a, int G)
           Vec<T>::unpack(piece(stage, u * PER + 3), d + W / 2);
           rotate<W, HALVES, true>(d, c, sn);
 #pragma unroll
-          for (int e = 0; e < W; ++e) {
-            ss2 = fma2(v[e], v[e], ss2);
-            sg2 = fma2(mul2(d[e], w[e]), v[e], sg2);
+          for (int e = 0; e < W / 2; ++e) {
+            const float4 f = lds4(w_at + uint32_t(e * slots) * 16);
+            ss2 = fma2(v[2 * e], v[2 * e], fma2(v[2 * e + 1], v[2 * e + 1], ss2));
+            sg2 = fma2(mul2(d[2 * e], lo2(f)), v[2 * e], fma2(mul2(d[2 * e + 1], hi2(f)), v[2 * e + 1], sg2));
           }
           float ss = hsum2(ss2), sg = hsum2(sg2);
           for (int o = G >> 1; o > 0; o >>= 1) {
@@ -302,9 +324,10 @@ __global__ void __launch_bounds__(THREADS, 2) rotate_kernel(const Args a, int G)
           const float2 r2 = f2(rinv), mean = f2(-sg * rinv * inv_d);
 #pragma unroll
           for (int e = 0; e < W; ++e) {
+            const float4 f = lds4(w_at + uint32_t(e / 2 * slots) * 16);
             v[e] = mul2(v[e], r2);
             acc[e] = fma2(d[e], v[e], acc[e]);
-            v[e] = mul2(r2, fma2(v[e], mean, mul2(d[e], w[e])));
+            v[e] = mul2(r2, fma2(v[e], mean, mul2(d[e], e & 1 ? hi2(f) : lo2(f))));
           }
         } else {
 #pragma unroll
@@ -503,7 +526,8 @@ static int launch(Args& a, bool halves, cudaStream_t s) {
     PGF_LAUNCH_CHECK();
     return PGF_OK;
   }
-  const size_t smem = size_t(RING) + (size_t(a.D / 2) + 1) / 2 * 16 + size_t(THREADS / 32) * tw_most * (a.D / 2) * 8;
+  const size_t smem = size_t(RING) + (size_t(a.D / 2) + 1) / 2 * 16 + size_t(THREADS / 32) * tw_most * (a.D / 2) * 8 +
+                      size_t(a.D) * 4;
   static int limit[2] = {0, 0};
   if (halves) {
     PGF_CUDA(ensure_dynamic_smem(rotate_kernel<T, true, BWD>, smem, limit[0]));
@@ -544,6 +568,7 @@ static Args make(const void* q, const pgf_strides* qs, const void* k, const pgf_
   a.xs[0] = qs ? *qs : dq;
   a.xs[1] = ks ? *ks : dk;
   a.H[0] = int(Hq); a.H[1] = int(Hk);
+  for (int z = 0; z < 2; ++z) a.flat[z] = Bsz == 1 || a.xs[z].batch == L * a.xs[z].token;
   a.turns = turns; a.positions = positions; a.start = start;
   a.tokens = Bsz * L; a.L = L;
   a.D = int(D); a.R = int(R); a.eps = eps;
