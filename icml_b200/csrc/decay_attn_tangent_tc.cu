@@ -16,10 +16,11 @@
 // rows of one product: U over U' (lanes 0..63 and 64..127) and V1 over V2, so S stands in lanes 0..63 next to
 // V1 and S' in lanes 64..127 next to V2; only n S crosses over, through shared memory.
 //
-// Roles (640 threads): warp 0 TMA, warp 1 MMA, warps 2..17 work.  Per chunk a worker weighs its share of k,
-// adds its block of the pair sum, fetches U, weighs q, adds its part of <S, V1> + <S', V2> and steps its
-// 16 columns of the state.  Bound by shared memory: per chunk 1,500 wavefronts to write the weighted terms, 2,800
-// for the products to read them and 512 for the tiles.
+// Roles (640 threads): warp 0 TMA, warp 1 MMA, warps 2..17 work.  Per chunk a worker weighs its share of k and q
+// by halves of 64 tokens (k, q, k, q: two buffers, so that the products of one run while the other is weighed),
+// adds its block of the pair sum, adds its part of <S, V1> + <S', V2> and steps its 16 columns of the state.
+// Shared memory is what it needs most: per chunk 1,500 wavefronts to write the weighted terms, 2,800 for the
+// products to read them and 512 for the tiles.
 #include "decay_attn_tc.cuh"
 
 namespace pgf {
@@ -30,14 +31,15 @@ namespace {
 constexpr int C = TC_CHUNK;
 constexpr int THREADS = 640;
 constexpr int NS = 7;                                     // ring: k, v, q, g of a chunk, three of the next
-constexpr uint32_t BUF = NS * BLK;                        // three terms x two weights
+constexpr uint32_t HALF = BLK / 2;                        // 64 rows
+constexpr uint32_t BUF = NS * BLK;                        // k, q: three terms x two weights of 64 rows
 constexpr uint32_t XCH = BUF + 6 * BLK;                   // 64 x 64 float32
 constexpr uint32_t TAB = XCH + BLK;                       // 132 + 32 floats
 constexpr uint32_t BARS = TAB + 656 + 64;
 constexpr uint32_t BYTES = BARS + 256 + 1024;
 static_assert(BYTES <= 232448, "fits an SM");
 constexpr uint32_t T_A = 0, T_B = 128, T_U = 256, T_V = 320;
-enum { B_AB = 0, B_U, B_V, B_K, B_Q, B_COUNT };
+enum { B_AB = 0, B_U, B_V, B_K, B_Q, B_X, B_COUNT };      // B_U, B_V, B_K, B_Q: a phase per half
 
 struct Params {
   const float* log_decay;
@@ -82,7 +84,7 @@ tangent_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   if (threadIdx.x < 16) sums[threadIdx.x] = 0.f;
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2 * NS; ++s) mbar_init(&full[s], 1);
-    for (int k = 0; k < B_COUNT; ++k) mbar_init(&bars[k], k == B_K || k == B_Q ? 16 : 1);
+    for (int k = 0; k < B_COUNT; ++k) mbar_init(&bars[k], k == B_K || k == B_Q ? 16 : k == B_X ? 8 : 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 0) {
@@ -123,47 +125,52 @@ tangent_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const uint32_t id_a = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(C >> 3) << 17) | (uint32_t(C >> 4) << 24);
     const uint32_t id_u = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 15) | (1u << 16) | (uint32_t(64 >> 3) << 17) |
                           (uint32_t(C >> 4) << 24);
-    const Desc terms(sbase + BUF, BLK);
-    for (int c = 0; c < chunks; ++c) {
+    const Desc terms_k(sbase + BUF, HALF), terms_q(sbase + BUF + 6 * HALF, HALF);
+    bool ok = true;
+    for (int c = 0; c < chunks && ok; ++c) {
       const uint32_t n = uint32_t(c) * 4;
       if (!wait_full(n) || !wait_full(n + 1) || !wait_full(n + 2) || !wait_full(n + 3)) break;
-      // the pair sum of the chunk before has been taken from A and B (its q sets have arrived since)
-      tc_after();
-      if (leader) {
-        const Desc k(tile(n), 16), v(tile(n + 1), 16), q(tile(n + 2), 16), g(tile(n + 3), 16);
+      for (int half = 0; half < 2; ++half) {
+        const int t = 2 * c + half;
+        // (a worker weighs the next k when it is done with A, B, U and V of the chunk before)
+        if (!wait(B_K, t)) { ok = false; break; }
+        tc_after();
+        if (leader) {
+          const Desc v(tile(n + 1) + half * HALF, BLK);
+          for (int m = 2; m >= 0; --m)   // small terms first
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) umma_bf16(tmem + T_A, q.at(kk * 32), k.at(kk * 32), id_a, kk > 0);
+            for (int kk = 0; kk < 4; ++kk)
+              umma_bf16(tmem + T_U, terms_k.at(m * 2 * HALF + kk * 2048), v.at(kk * 2048), id_u, half || m < 2 || kk > 0);
+          umma_commit(&bars[B_U]);
+          if (half == 0) {
+            const Desc k(tile(n), 16), v1(tile(n + 1), 16), q(tile(n + 2), 16), g(tile(n + 3), 16);
 #pragma unroll
-        for (int kk = 0; kk < 4; ++kk) umma_bf16(tmem + T_B, g.at(kk * 32), v.at(kk * 32), id_a, kk > 0);
-        umma_commit(&bars[B_AB]);
+            for (int kk = 0; kk < 4; ++kk) umma_bf16(tmem + T_A, q.at(kk * 32), k.at(kk * 32), id_a, kk > 0);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) umma_bf16(tmem + T_B, g.at(kk * 32), v1.at(kk * 32), id_a, kk > 0);
+            umma_commit(&bars[B_AB]);
+          } else {
+            umma_commit(&empty[n % NS]);
+            umma_commit(&empty[(n + 1) % NS]);
+          }
+        }
+        __syncwarp();
+        if (!wait(B_Q, t)) { ok = false; break; }
+        tc_after();
+        if (leader) {
+          const Desc g(tile(n + 3) + half * HALF, BLK);
+          for (int m = 2; m >= 0; --m)
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_bf16(tmem + T_V, terms_q.at(m * 2 * HALF + kk * 2048), g.at(kk * 2048), id_u, half || m < 2 || kk > 0);
+          umma_commit(&bars[B_V]);
+          if (half) {
+            umma_commit(&empty[(n + 2) % NS]);
+            umma_commit(&empty[(n + 3) % NS]);
+          }
+        }
+        __syncwarp();
       }
-      __syncwarp();
-      if (!wait(B_K, c)) break;
-      tc_after();
-      if (leader) {
-        const Desc v(tile(n + 1), BLK);
-        for (int t = 2; t >= 0; --t)   // small terms first
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
-            umma_bf16(tmem + T_U, terms.at(t * 2 * BLK + kk * 2048), v.at(kk * 2048), id_u, t < 2 || kk > 0);
-        umma_commit(&bars[B_U]);
-        umma_commit(&empty[n % NS]);
-        umma_commit(&empty[(n + 1) % NS]);
-      }
-      __syncwarp();
-      if (!wait(B_Q, c)) break;
-      tc_after();
-      if (leader) {
-        const Desc g(tile(n + 3), BLK);
-        for (int t = 2; t >= 0; --t)
-#pragma unroll
-          for (int kk = 0; kk < 8; ++kk)
-            umma_bf16(tmem + T_V, terms.at(t * 2 * BLK + kk * 2048), g.at(kk * 2048), id_u, t < 2 || kk > 0);
-        umma_commit(&bars[B_V]);
-        umma_commit(&empty[(n + 2) % NS]);
-        umma_commit(&empty[(n + 3) % NS]);
-      }
-      __syncwarp();
     }
   } else if (warp < 18) {
     const int q = warp & 3, cg = (warp - 2) >> 2, i = q * 32 + lane, tid = int(threadIdx.x) - 64;
@@ -171,37 +178,35 @@ tangent_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const bool tangent = i >= 64;                          // these lanes hold S'
     const int64_t n_state = int64_t(p.dk) * p.dv;
     auto pw = [&](int e) { return lds_f(sbase + TAB + 4 * e); };
-    // The tile's rows times two weights of their token, each as three terms; rows past the length as zeros.
-    auto weigh = [&](uint32_t src, int n, bool keys) {
-      uint32_t v[2][4];
+    // A half of the tile's rows times two weights of their token, each as three terms; rows past the length as zeros.
+    auto weigh = [&](uint32_t src, int half, int n, bool keys) {
+      uint32_t v[4];
+      const uint32_t off = uint32_t(tid) * 16;
+      lds128(src + half * HALF + off, v);
+      const int j = half * 64 + (tid >> 3);
+      if (j >= n) v[0] = v[1] = v[2] = v[3] = 0;
+      const int e = j >= n ? 0 : keys ? n - 1 - j : j + 1;
+      const float w = pw(e), we = w * float(e);
+      const uint32_t dst = sbase + BUF + (keys ? 0 : 6 * HALF) + off;
 #pragma unroll
-      for (int k = 0; k < 2; ++k) lds128(src + uint32_t(tid + 512 * k) * 16, v[k]);
+      for (int z = 0; z < 2; ++z) {
+        // first 64 rows of the product: a^e of the keys (U), e a^e of the queries (V1)
+        const float2 w2 = f2((z == 0) == keys ? w : we), minus = f2(-1.f);
+        uint32_t t[3][4];
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const uint32_t u = uint32_t(tid + 512 * k), off = u * 16;
-        const int j = int(u >> 3);
-        if (j >= n) v[k][0] = v[k][1] = v[k][2] = v[k][3] = 0;
-        const int e = j >= n ? 0 : keys ? n - 1 - j : j + 1;
-        const float w = pw(e), we = w * float(e);
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          // first 64 rows of the product: a^e of the keys (U), e a^e of the queries (V1)
-          const float wz = (z == 0) == keys ? w : we;
-          const float2 w2 = f2(wz), minus = f2(-1.f);
-          uint32_t t[3][4];
-#pragma unroll
-          for (int m = 0; m < 4; ++m) {
-            float2 a = __fmul2_rn(unpack2(v[k][m]), w2);
-            t[0][m] = pack2(a);
-            a = __ffma2_rn(unpack2(t[0][m]), minus, a);
-            t[1][m] = pack2(a);
-            a = __ffma2_rn(unpack2(t[1][m]), minus, a);
-            t[2][m] = pack2(a);
-          }
-#pragma unroll
-          for (int m = 0; m < 3; ++m) sts128(sbase + BUF + uint32_t(m * 2 + z) * BLK + off, t[m]);
+        for (int m = 0; m < 4; ++m) {
+          float2 a = __fmul2_rn(unpack2(v[m]), w2);
+          t[0][m] = pack2(a);
+          a = __ffma2_rn(unpack2(t[0][m]), minus, a);
+          t[1][m] = pack2(a);
+          a = __ffma2_rn(unpack2(t[1][m]), minus, a);
+          t[2][m] = pack2(a);
         }
+#pragma unroll
+        for (int m = 0; m < 3; ++m) sts128(dst + uint32_t(m * 2 + z) * HALF, t[m]);
       }
+      fence_async();
+      arrive(keys ? B_K : B_Q);
     };
     auto clear_rows = [&](uint32_t dst, int n) {
       const uint32_t zero[4] = {0, 0, 0, 0};
@@ -224,66 +229,78 @@ tangent_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     for (int c = 0; c < chunks; ++c) {
       const uint32_t nt = uint32_t(c) * 4;
       const int n = int(min(int64_t(C), s1 - (s0 + int64_t(c) * C)));
-      // the terms' buffers are free: this warp has seen V of the chunk before
+      // the buffers are free: this warp has seen U and V of the chunk before
       if (!tangent) {
 #pragma unroll
         for (int k = 0; k < 16; ++k) xch[k * 64] = s[k];
+        arrive(B_X);
       }
+      const float an = pw(n), cross = an * float(n);
       if (!wait_full(nt)) { ok = false; break; }
-      weigh(tile(nt), n, true);
       if (n < C) {
         if (!wait_full(nt + 1) || !wait_full(nt + 3)) { ok = false; break; }
         clear_rows(tile(nt + 1), n);
         clear_rows(tile(nt + 3), n);
       }
-      fence_async();
-      arrive(B_K);
+      weigh(tile(nt), 0, n, true);
+      if (!wait_full(nt + 2)) { ok = false; break; }
+      weigh(tile(nt + 2), 0, n, false);
+      float u[16];
+      if (tangent) {                            // S of this chunk, before its place is written again
+        if (!wait(B_X, c)) { ok = false; break; }
+#pragma unroll
+        for (int k = 0; k < 16; ++k) u[k] = cross * xch[k * 64];
+      } else {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) u[k] = 0.f;
+      }
+      if (!wait(B_U, 2 * c)) { ok = false; break; }
+      weigh(tile(nt), 1, n, true);
+      if (!wait(B_V, 2 * c)) { ok = false; break; }
+      weigh(tile(nt + 2), 1, n, false);
       // the pair sum: this warp's rows, columns 32 cg .. + 31
-      if (!wait(B_AB, c)) { ok = false; break; }
-      tc_after();
       if (cg <= q) {
-        uint32_t a[32], g[32];
-        tmem_ld32_nowait(tmem + T_A + row + cg * 32, a);
-        tmem_ld32_nowait(tmem + T_B + row + cg * 32, g);
-        tmem_wait_ld();
+        if (!wait(B_AB, c)) { ok = false; break; }
+        tc_after();
         float t = 0.f;
-        if (cg < q) {
-          const int e0 = i - 32 * cg;
-          const float rf = pw(e0 - 31);
+        const float e0 = float(i - 32 * cg);
+        const float rf = cg < q ? pw(i - 32 * cg - 31) : 1.f;
 #pragma unroll
-          for (int k = 0; k < 32; ++k)
-            t = fmaf(__uint_as_float(a[k]) * __uint_as_float(g[k]), lds_f(sbase + TAB + 528 + 4 * k) * float(e0 - k), t);
-          t *= rf;
-        } else {
+        for (int z = 0; z < 2; ++z) {
+          uint32_t a[16], g[16];
+          tmem_ld16_nowait(tmem + T_A + row + cg * 32 + z * 16, a);
+          tmem_ld16_nowait(tmem + T_B + row + cg * 32 + z * 16, g);
+          tmem_wait_ld();
+          if (cg < q) {
 #pragma unroll
-          for (int k = 0; k < 32; ++k) {
-            const float w = pw(lane - k) * float(lane - k);   // masked lanes read what lies in front
-            t += k <= lane ? __uint_as_float(a[k]) * __uint_as_float(g[k]) * w : 0.f;
+            for (int k = 0; k < 16; k += 4) {
+              const float4 w = lds_f4(sbase + TAB + 528 + 4 * (z * 16 + k));
+              const float wf[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+              for (int m = 0; m < 4; ++m)
+                t = fmaf(__uint_as_float(a[k + m]) * __uint_as_float(g[k + m]), wf[m] * (e0 - float(z * 16 + k + m)), t);
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              const int j = z * 16 + k;
+              const float w = pw(lane - j) * (e0 - float(j));            // masked lanes read what lies in front
+              t += j <= lane ? __uint_as_float(a[k]) * __uint_as_float(g[k]) * w : 0.f;
+            }
           }
         }
+        t *= rf;
         if (i < n) acc += t;
       }
-      const float an = pw(n);
-      float u[16];
-      {
-        if (!wait(B_U, c)) { ok = false; break; }
-        tc_after();
-        uint32_t r[16];
-        tmem_ld16_nowait(tmem + T_U + row + cg * 16, r);
-        tmem_wait_ld();
-        if (!wait(B_K, c)) { ok = false; break; }           // every S of this chunk is there to be read
-        const float cross = tangent ? an * float(n) : 0.f;
-#pragma unroll
-        for (int k = 0; k < 16; ++k) u[k] = fmaf(cross, tangent ? xch[k * 64] : 0.f, __uint_as_float(r[k]));
-      }
-      if (!wait_full(nt + 2)) { ok = false; break; }
-      weigh(tile(nt + 2), n, false);
-      fence_async();
-      tc_before();
-      arrive(B_Q);
-      if (!wait(B_V, c)) { ok = false; break; }
-      tc_after();
       uint32_t r[16];
+      if (!wait(B_U, 2 * c + 1)) { ok = false; break; }
+      tc_after();
+      tmem_ld16_nowait(tmem + T_U + row + cg * 16, r);
+      tmem_wait_ld();
+#pragma unroll
+      for (int k = 0; k < 16; ++k) u[k] += __uint_as_float(r[k]);
+      if (!wait(B_V, 2 * c + 1)) { ok = false; break; }
+      tc_after();
       tmem_ld16_nowait(tmem + T_V + row + cg * 16, r);
       tmem_wait_ld();
       float t = 0.f;
