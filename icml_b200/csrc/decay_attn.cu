@@ -36,15 +36,57 @@ static size_t smem_bytes(int dx, int mode) {
 }
 
 // rows [t0, t0 + n) x columns [c0, c0 + w) of one head as float32 with row pitch `pitch`; zeros elsewhere
-// (to C rows and wpad columns), so nothing that a padded place holds is read.
+// (to C rows and wpad columns, a multiple of 4), so nothing that a padded place holds is read.  float32 goes by
+// asynchronous copies (16 bytes where the tensor allows, else 4), so that all of a chunk's tensors are on
+// their way together; bfloat16 through registers, eight pieces at a time.  The caller waits (staged()).
 template <class T>
 __device__ __forceinline__ void stage(float* dst, int pitch, const Tensor& t, int64_t b, int64_t t0, int n, int h, int c0,
-                                      int w, int wpad, int C, float mul) {
+                                      int w, int wpad, int C) {
   const T* p = static_cast<const T*>(t.p) + b * t.s.batch + t0 * t.s.token + int64_t(h) * t.s.head + c0;
-  for (int i = threadIdx.x; i < C * wpad; i += THREADS) {
-    const int r = i / wpad, c = i - r * wpad;
-    dst[r * pitch + c] = r < n && c < w ? ld(p, int64_t(r) * t.s.token + c) * mul : 0.f;
+  const int w4 = wpad / 4;
+  if constexpr (sizeof(T) == 4) {
+    const uint32_t d0 = static_cast<uint32_t>(__cvta_generic_to_shared(dst));
+    if (t.vec) {
+      for (int i = threadIdx.x; i < C * w4; i += THREADS) {
+        const int r = i / w4, c = (i - r * w4) * 4;
+        const int bytes = r < n && c < w ? min(16, (w - c) * 4) : 0;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d0 + uint32_t(r * pitch + c) * 4),
+                     "l"(bytes ? p + int64_t(r) * t.s.token + c : static_cast<const T*>(t.p)), "r"(bytes) : "memory");
+      }
+    } else {
+      for (int i = threadIdx.x; i < C * wpad; i += THREADS) {
+        const int r = i / wpad, c = i - r * wpad;
+        const bool in = r < n && c < w;
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d0 + uint32_t(r * pitch + c) * 4),
+                     "l"(in ? p + int64_t(r) * t.s.token + c : static_cast<const T*>(t.p)), "r"(in ? 4 : 0) : "memory");
+      }
+    }
+  } else {
+    constexpr int U = 8;
+    for (int i0 = threadIdx.x; i0 < C * w4; i0 += U * THREADS) {
+      float4 v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * THREADS, r = i / w4, c = (i - r * w4) * 4;
+        const T* q = p + int64_t(r) * t.s.token + c;
+        v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < n && r < C) {
+          if (c < w) v[u].x = ld(q, 0);
+          if (c + 1 < w) v[u].y = ld(q, 1);
+          if (c + 2 < w) v[u].z = ld(q, 2);
+          if (c + 3 < w) v[u].w = ld(q, 3);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * THREADS, r = i / w4, c = (i - r * w4) * 4;
+        if (r < C) *reinterpret_cast<float4*>(dst + r * pitch + c) = v[u];
+      }
+    }
   }
+}
+__device__ __forceinline__ void staged() {
+  asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
 }
 
 template <class T, int C, int MODE>
@@ -87,7 +129,7 @@ __global__ void __launch_bounds__(THREADS) walk_kernel(const Job job, const Tang
     sS[i] = v;
     if (MODE == MODE_TANGENT) sD[i] = 0.f;
   }
-  float tsum = 0.f;
+  float tsum = 0.f, tend = 0.f;
   const int ty = threadIdx.x >> 4, tx = threadIdx.x & 15;
   // (the end state of the walk's last piece enters no other piece)
   const bool idle = MODE == MODE_STATE && !job.last_too && seg == (job.rev ? 0 : job.segs - 1);
@@ -96,14 +138,15 @@ __global__ void __launch_bounds__(THREADS) walk_kernel(const Job job, const Tang
     const int64_t t0 = s0 + int64_t(job.rev ? chunks - 1 - ci : ci) * C;
     const int n = int(min(int64_t(C), s1 - t0));
     __syncthreads();
-    stage<T>(sY, px, job.y, b, t0, n, hy, 0, dx, dxp, C, 1.f);
-    stage<T>(sZ, E, job.z, b, t0, n, hz, c0, cw, E, C, job.z_scale);
-    if (MODE != MODE_STATE) stage<T>(sX, px, job.x, b, t0, n, hx, 0, dx, dxp, C, 1.f);
-    if (MODE == MODE_TANGENT) stage<T>(sG, E, tan.g, b, t0, n, h / (job.H / tan.g.heads), c0, cw, E, C, tan.scale);
+    stage<T>(sY, px, job.y, b, t0, n, hy, 0, dx, dxp, C);
+    stage<T>(sZ, E, job.z, b, t0, n, hz, c0, cw, E, C);
+    if (MODE != MODE_STATE) stage<T>(sX, px, job.x, b, t0, n, hx, 0, dx, dxp, C);
+    if (MODE == MODE_TANGENT) stage<T>(sG, E, tan.g, b, t0, n, h / (job.H / tan.g.heads), c0, cw, E, C);
     if (threadIdx.x < C) {
       const int j = threadIdx.x;
-      sUpd[j] = j < n ? sPow[job.rev ? j + 1 : n - 1 - j] : 0.f;
+      sUpd[j] = j < n ? sPow[job.rev ? j + 1 : n - 1 - j] * job.z_scale : 0.f;
     }
+    staged();
     __syncthreads();
     if (MODE != MODE_STATE) {
       // scores of the pairs inside the chunk: rows i = ty + 16 r, columns j = tx + 16 c
@@ -134,7 +177,7 @@ __global__ void __launch_bounds__(THREADS) walk_kernel(const Job job, const Tang
 #pragma unroll
         for (int c = 0; c < RT; ++c) {
           const int i = ty + 16 * r, j = tx + 16 * c, e = job.rev ? j - i : i - j;
-          float w = e >= 0 ? sPow[e] : 0.f;
+          float w = e >= 0 ? sPow[e] * job.z_scale : 0.f;
           if (MODE == MODE_TANGENT) w *= float(e);
           sP[i * (C + 4) + j] = e >= 0 ? acc[r][c] * w : 0.f;
         }
@@ -268,10 +311,10 @@ __global__ void __launch_bounds__(THREADS) walk_kernel(const Job job, const Tang
     if (tan.behind) {
       const float* x = tan.behind + (b * job.H + h) * tan.behind_stride + int64_t(seg) * dx * dz;
       for (int i = threadIdx.x; i < dx * cw; i += THREADS)
-        tsum = fmaf(x[int64_t(i / cw) * dz + c0 + i % cw], sD[(i / cw) * E + i % cw], tsum);
+        tend = fmaf(x[int64_t(i / cw) * dz + c0 + i % cw], sD[(i / cw) * E + i % cw], tend);
     }
     __shared__ float red[THREADS / 32];
-    tsum = warp_sum(tsum);
+    tsum = warp_sum(fmaf(tsum, tan.scale, tend));
     if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = tsum;
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -510,6 +553,7 @@ static Tensor tensor(const void* p, const pgf_strides* s, int64_t L, int64_t hea
   t.d = int(d);
   if (s) t.s = *s;
   else t.s = {L * heads * d, heads * d, d};
+  t.vec = aligned(p, 16) && t.s.batch % 4 == 0 && t.s.token % 4 == 0 && t.s.head % 4 == 0;
   return t;
 }
 
@@ -522,7 +566,8 @@ static Plan plan(const Shape& p, bool tc, bool backward) {
   if (tc) return {true, cut(p.B * p.H, p.L, TC_CHUNK, 1)};
   // a backward's calls have either width as columns and either as rows
   const int64_t cols = backward && p.Dk < p.Dv ? p.Dk : p.Dv, rows = backward && p.Dv > p.Dk ? p.Dv : p.Dk;
-  return {false, cut(p.B * p.H * ceil_div(cols, E), p.L, chunk_of(int(rows)), 1)};
+  const int resident = int(233472 / (smem_bytes((int(rows) + 3) & ~3, MODE_OUT) + 1024));
+  return {false, cut(p.B * p.H * ceil_div(cols, E), p.L, chunk_of(int(rows)), resident)};
 }
 
 // The state that enters each piece of a walk: (B, H, segs, rows, columns).

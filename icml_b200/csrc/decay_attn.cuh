@@ -29,6 +29,7 @@ struct Tensor {
   pgf_strides s;
   int heads;      // divides H: head h of the operator reads head h / (H / heads)
   int d;
+  int vec;        // base and strides are whole 16-byte units of float32
 };
 
 // One F call.
