@@ -17,6 +17,13 @@ constexpr int THREADS = 256;
 constexpr int E = 64;               // state columns of one CTA
 enum { MODE_OUT = 0, MODE_STATE = 1, MODE_TANGENT = 2 };
 
+// Walks that run side by side in one launch: CTAs [first[k], first[k + 1]) take job k.
+struct Jobs {
+  Job job[3];
+  int first[4];
+  int count;
+};
+
 struct TangentArgs {
   Tensor g;               // output gradients, slices like z
   const float* behind;    // (B, H, segs, x.d, z.d): adjoint of the state behind each piece, or NULL (zeros)
@@ -90,11 +97,13 @@ __device__ __forceinline__ void staged() {
 }
 
 template <class T, int C, int MODE>
-__global__ void __launch_bounds__(THREADS) walk_kernel(const Job job, const TangentArgs tan) {
+__global__ void __launch_bounds__(THREADS) walk_kernel(const __grid_constant__ Jobs jobs, const TangentArgs tan) {
   extern __shared__ __align__(16) float sm[];
+  const int which = int(blockIdx.x) >= jobs.first[2] ? 2 : int(blockIdx.x) >= jobs.first[1] ? 1 : 0;
+  const Job& job = jobs.job[which];
   const int dx = job.x.d, dz = job.z.d, dxp = (dx + 3) & ~3, px = dxp + 4;
   const int slices = (dz + E - 1) / E;
-  int64_t id = blockIdx.x;
+  int64_t id = int(blockIdx.x) - jobs.first[which];
   const int sl = int(id % slices);
   id /= slices;
   const int seg = int(id % job.segs);
@@ -328,20 +337,27 @@ __global__ void __launch_bounds__(THREADS) walk_kernel(const Job job, const Tang
 // The pieces' own end states (B, H, segs, n) become the states that enter each piece: one thread per
 // state element walks the pieces in the direction of time (or back), eight loads ahead of their use.
 // last: the state behind the walk (the last piece's own end state has to be there), or NULL.
-__global__ void __launch_bounds__(128) enter_kernel(float* __restrict__ pieces, const float* __restrict__ first,
-                                                    float* __restrict__ last, const float* __restrict__ log_decay,
-                                                    const int32_t* __restrict__ lengths, int64_t L, int H, int segs,
-                                                    int64_t seg_len, int rev, int64_t n, int blocks) {
+struct EnterSet {
+  float* pieces[2];
+  const float* first[2];
+  float* last[2];
+  int rev[2];
+  const float* log_decay;
+  const int32_t* lengths;
+  int64_t L, seg_len, n;
+  int H, segs, blocks;
+};
+__global__ void __launch_bounds__(128) enter_kernel(const __grid_constant__ EnterSet a) {
   constexpr int U = 8;
-  const int64_t bh = blockIdx.x / blocks, b = bh / H;
-  const int h = int(bh % H);
-  const float l2 = log2_decay(log_decay[h]);
-  const int64_t len = row_length(lengths, b, L);
-  const int64_t i = int64_t(blockIdx.x % blocks) * 128 + threadIdx.x;
+  const int w = blockIdx.y, rev = a.rev[w], segs = a.segs;
+  const int64_t bh = blockIdx.x / a.blocks, b = bh / a.H, n = a.n;
+  const float l2 = log2_decay(a.log_decay[bh % a.H]);
+  const int64_t len = row_length(a.lengths, b, a.L);
+  const int64_t i = int64_t(blockIdx.x % a.blocks) * 128 + threadIdx.x;
   if (i >= n) return;
-  float cur = first ? first[bh * n + i] : 0.f;
-  float* p = pieces + bh * segs * n + i;
-  const int own_segs = last ? segs : segs - 1;
+  float cur = a.first[w] ? a.first[w][bh * n + i] : 0.f;
+  float* __restrict__ p = a.pieces[w] + bh * segs * n + i;
+  const int own_segs = a.last[w] ? segs : segs - 1;
   for (int k0 = 0; k0 < segs; k0 += U) {
     float own[U];
 #pragma unroll
@@ -353,21 +369,30 @@ __global__ void __launch_bounds__(128) enter_kernel(float* __restrict__ pieces, 
     for (int u = 0; u < U; ++u) {
       const int k = k0 + u, s = rev ? segs - 1 - k : k;
       if (k >= segs) break;
-      const int64_t s0 = min(len, s * seg_len), s1 = min(len, s0 + seg_len);
+      const int64_t s0 = min(len, s * a.seg_len), s1 = min(len, s0 + a.seg_len);
       p[int64_t(s) * n] = cur;
       cur = fmaf(exp2f(l2 * float(s1 - s0)), cur, own[u]);
     }
   }
-  if (last) last[bh * n + i] = cur;
+  if (a.last[w]) a.last[w][bh * n + i] = cur;
 }
 
-// out (tokens, heads, d) = sum over the H / heads operator heads that share each head of part (tokens, H, d)
+// out (tokens, heads, d) = sum over the H / heads operator heads that share each head of part (tokens, H, d),
+// for up to three tensors (blockIdx.y)
+struct ShareSet {
+  const float* part[3];
+  void* out[3];
+  int64_t n[3];
+  int heads[3], group[3], d[3];
+};
 template <class T>
-__global__ void __launch_bounds__(256) share_sum_kernel(const float* part, T* out, int64_t n, int heads, int group, int d) {
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < n; i += int64_t(gridDim.x) * 256) {
+__global__ void __launch_bounds__(256) share_sum_kernel(const __grid_constant__ ShareSet a) {
+  const int w = blockIdx.y, heads = a.heads[w], group = a.group[w], d = a.d[w];
+  T* out = static_cast<T*>(a.out[w]);
+  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < a.n[w]; i += int64_t(gridDim.x) * 256) {
     const int64_t th = i / d;
     const int64_t t = th / heads, hh = th % heads;
-    const float* p = part + (t * heads * group + hh * group) * d + i % d;
+    const float* p = a.part[w] + (t * heads * group + hh * group) * d + i % d;
     float s = 0.f;
     for (int r = 0; r < group; ++r) s += p[int64_t(r) * d];
     st(out, i, s);
@@ -391,21 +416,34 @@ __global__ void __launch_bounds__(256) decay_sum_kernel(const float* part, float
 }
 
 template <class T, int C, int MODE>
-static int walk_as(const Job& job, const TangentArgs& tan, cudaStream_t s) {
+static int walk_as(const Jobs& jobs, int rows, const TangentArgs& tan, cudaStream_t s) {
   static int limit = 0;
-  const size_t smem = smem_bytes((job.x.d + 3) & ~3, MODE);
+  const size_t smem = smem_bytes((rows + 3) & ~3, MODE);
   PGF_CUDA(ensure_dynamic_smem(walk_kernel<T, C, MODE>, smem, limit));
-  const int64_t grid = job.B * job.H * job.segs * ceil_div(job.z.d, E);
-  walk_kernel<T, C, MODE><<<unsigned(grid), THREADS, smem, s>>>(job, tan);
+  walk_kernel<T, C, MODE><<<unsigned(jobs.first[3]), THREADS, smem, s>>>(jobs, tan);
   PGF_LAUNCH_CHECK();
   return PGF_OK;
 }
 
 template <int MODE>
-static int walk(const Job& job, const TangentArgs& tan, int dtype, cudaStream_t s) {
+static int walk(const Job* job, int count, const TangentArgs& tan, int dtype, cudaStream_t s) {
+  Jobs jobs = {};
+  int64_t ctas = 0;
+  int rows = 0;
+  for (int k = 0; k < 3; ++k) {
+    jobs.first[k] = int(ctas);
+    if (k >= count) continue;
+    jobs.job[k] = job[k];
+    ctas += job[k].B * job[k].H * job[k].segs * ceil_div(job[k].z.d, E);
+    if (job[k].x.d > rows) rows = job[k].x.d;
+  }
+  PGF_CHECK_ARG(ctas < 0x7fffffff, "decay_attn: too many pieces");
+  jobs.first[3] = int(ctas);
+  jobs.count = count;
   if (dtype == PGF_DTYPE_BF16)
-    return job.x.d > 128 ? walk_as<__nv_bfloat16, 32, MODE>(job, tan, s) : walk_as<__nv_bfloat16, 64, MODE>(job, tan, s);
-  return job.x.d > 128 ? walk_as<float, 32, MODE>(job, tan, s) : walk_as<float, 64, MODE>(job, tan, s);
+    return rows > 128 ? walk_as<__nv_bfloat16, 32, MODE>(jobs, rows, tan, s)
+                      : walk_as<__nv_bfloat16, 64, MODE>(jobs, rows, tan, s);
+  return rows > 128 ? walk_as<float, 32, MODE>(jobs, rows, tan, s) : walk_as<float, 64, MODE>(jobs, rows, tan, s);
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -576,29 +614,47 @@ struct Entering {
   int64_t stride;
 };
 
-static int f_call(const Job& job, const Plan& pl, int dtype, cudaStream_t s) {
-  if (pl.tc) return tc_walk(job, false, s);
-  return walk<MODE_OUT>(job, TangentArgs{}, dtype, s);
+static int f_calls(const Job* job, int count, const Plan& pl, int dtype, cudaStream_t s) {
+  if (!pl.tc) return walk<MODE_OUT>(job, count, TangentArgs{}, dtype, s);
+  for (int k = 0; k < count; ++k) PGF_TRY(tc_walk(job[k], false, s));
+  return PGF_OK;
 }
 
-// What enters the pieces of a walk that begins with `first`; `pieces` is scratch for them.  last: where the
-// state behind a cut walk goes, or NULL (an uncut one gives it by itself).
-static int entering(Job job, const Plan& pl, const float* first, float* pieces, float* last, Entering* e, int dtype,
-                    cudaStream_t s) {
-  const int64_t n = int64_t(job.y.d) * job.z.d;
-  *e = {first, n};
-  if (job.segs == 1) return PGF_OK;
-  job.start = pieces;
-  job.start_stride = job.segs * n;
-  job.start_t = 0;
-  job.last_too = last != nullptr;
-  if (pl.tc) PGF_TRY(tc_walk(job, true, s));
-  else PGF_TRY(walk<MODE_STATE>(job, TangentArgs{}, dtype, s));
-  const int blocks = ceil_div(n, 128);
-  enter_kernel<<<unsigned(job.B * job.H * blocks), 128, 0, s>>>(pieces, first, last, job.log_decay, job.lengths, job.L,
-                                                                job.H, job.segs, job.seg_len, job.rev, n, blocks);
+// What enters the pieces of one or two walks of the same shape that begin with `first`; `pieces` is scratch for
+// them.  last: where the state behind a cut walk goes, or NULL (an uncut one gives it by itself).
+static int entering(Job* job, int count, const Plan& pl, const float* const* first, float* const* pieces,
+                    float* const* last, Entering* e, int dtype, cudaStream_t s) {
+  const int64_t n = int64_t(job[0].y.d) * job[0].z.d;
+  const int segs = job[0].segs;
+  for (int k = 0; k < count; ++k) e[k] = {first[k], n};
+  if (segs == 1) return PGF_OK;
+  EnterSet set;
+  for (int k = 0; k < count; ++k) {
+    job[k].start = pieces[k];
+    job[k].start_stride = segs * n;
+    job[k].start_t = 0;
+    job[k].last_too = last[k] != nullptr;
+    set.pieces[k] = pieces[k];
+    set.first[k] = first[k];
+    set.last[k] = last[k];
+    set.rev[k] = job[k].rev;
+    e[k] = {pieces[k], segs * n};
+  }
+  if (pl.tc) {
+    for (int k = 0; k < count; ++k) PGF_TRY(tc_walk(job[k], true, s));
+  } else {
+    PGF_TRY(walk<MODE_STATE>(job, count, TangentArgs{}, dtype, s));
+  }
+  set.log_decay = job[0].log_decay;
+  set.lengths = job[0].lengths;
+  set.L = job[0].L;
+  set.seg_len = job[0].seg_len;
+  set.n = n;
+  set.H = job[0].H;
+  set.segs = segs;
+  set.blocks = ceil_div(n, 128);
+  enter_kernel<<<dim3(unsigned(job[0].B * job[0].H * set.blocks), unsigned(count)), 128, 0, s>>>(set);
   PGF_LAUNCH_CHECK();
-  *e = {pieces, job.segs * n};
   return PGF_OK;
 }
 
@@ -619,16 +675,6 @@ static size_t workspace(const Shape& p, bool backward) {
     if (p.Hv < p.H) n += Workspace::round(tok * p.Dv) + 256;
   }
   return n;
-}
-
-template <class T>
-static int share_sum(const float* part, void* out, int64_t tokens, int64_t heads, int64_t H, int64_t d, cudaStream_t s) {
-  const int64_t n = tokens * heads * d;
-  int64_t ctas = (n + 255) / 256;
-  if (ctas > 148 * 16) ctas = 148 * 16;
-  share_sum_kernel<T><<<unsigned(ctas), 256, 0, s>>>(part, static_cast<T*>(out), n, int(heads), int(H / heads), int(d));
-  PGF_LAUNCH_CHECK();
-  return PGF_OK;
 }
 
 }  // namespace da
@@ -682,11 +728,12 @@ extern "C" int pgf_decay_attn_fwd(const void* q, const pgf_strides* q_strides, c
     }
   }
   da::Entering S;
-  PGF_TRY(da::entering(job, pl, state, pieces, state_out, &S, dtype, s));
+  da::Job js = job;
+  PGF_TRY(da::entering(&js, 1, pl, &state, &pieces, &state_out, &S, dtype, s));
   if (job.segs > 1) job.end = nullptr;
   job.start = S.p;
   job.start_stride = S.stride;
-  return da::f_call(job, pl, dtype, s);
+  return da::f_calls(&job, 1, pl, dtype, s);
 }
 
 extern "C" int pgf_decay_attn_bwd(const void* q, const pgf_strides* q_strides, const void* k,
@@ -732,41 +779,42 @@ extern "C" int pgf_decay_attn_bwd(const void* q, const pgf_strides* q_strides, c
     return PGF_ERR_WORKSPACE;
   }
   // what enters the pieces from both ends; X carries the scale of g
-  da::Entering S, X;
-  da::Job js = job;
-  js.x = js.y = tk; js.z = tv;
-  js.z_scale = 1.f;
-  PGF_TRY(da::entering(js, pl, state, sp, nullptr, &S, dtype, s));
-  js.x = js.y = tq; js.z = tg;
-  js.z_scale = scale;
-  js.rev = 1;
-  PGF_TRY(da::entering(js, pl, g_state, xp, grad_state, &X, dtype, s));
+  da::Entering ends[2];
+  {
+    da::Job js[2] = {job, job};
+    js[0].x = js[0].y = tk; js[0].z = tv;
+    js[0].z_scale = 1.f;
+    js[1].x = js[1].y = tq; js[1].z = tg;
+    js[1].z_scale = scale;
+    js[1].rev = 1;
+    const float* first[2] = {state, g_state};
+    float *pieces[2] = {sp, xp}, *last[2] = {nullptr, grad_state};
+    PGF_TRY(da::entering(js, 2, pl, first, pieces, last, ends, dtype, s));
+  }
+  const da::Entering S = ends[0], X = ends[1];
   const int f32 = dtype == PGF_DTYPE_F32;
   // grad q = scale F(g, v, k; S^T)
-  da::Job jq = job;
+  da::Job calls[3] = {job, job, job};
+  da::Job &jq = calls[0], &jv = calls[1], &jk = calls[2];
   jq.x = tg; jq.y = tv; jq.z = tk;
   jq.start = S.p; jq.start_stride = S.stride; jq.start_t = 1;
   jq.scale = scale; jq.z_scale = 1.f;
   jq.out = pq ? static_cast<void*>(pq) : grad_q;
   jq.out_f32 = f32 || pq;
-  PGF_TRY(da::f_call(jq, pl, dtype, s));
   // grad v = F(k, q, scale g; X) from the end
-  da::Job jv = job;
   jv.x = tk; jv.y = tq; jv.z = tg;
   jv.start = X.p; jv.start_stride = X.stride; jv.rev = 1;
   jv.z_scale = scale;
   jv.out = pv ? static_cast<void*>(pv) : grad_v;
   jv.out_f32 = f32 || pv;
   jv.end = job.segs > 1 ? nullptr : grad_state;
-  PGF_TRY(da::f_call(jv, pl, dtype, s));
   // grad k = F(v, g, scale q; X^T) from the end
-  da::Job jk = job;
   jk.x = tv; jk.y = tg; jk.z = tq;
   jk.start = X.p; jk.start_stride = X.stride; jk.start_t = 1; jk.rev = 1;
   jk.z_scale = scale;
   jk.out = pk ? static_cast<void*>(pk) : grad_k;
   jk.out_f32 = f32 || pk;
-  PGF_TRY(da::f_call(jk, pl, dtype, s));
+  PGF_TRY(da::f_calls(calls, 3, pl, dtype, s));
   if (grad_log_decay) {
     int parts;
     if (tc) {
@@ -793,19 +841,35 @@ extern "C" int pgf_decay_attn_bwd(const void* q, const pgf_strides* q_strides, c
       t.behind_stride = X.stride;
       t.part = part;
       t.scale = scale;
-      PGF_TRY(da::walk<da::MODE_TANGENT>(jt, t, dtype, s));
+      PGF_TRY(da::walk<da::MODE_TANGENT>(&jt, 1, t, dtype, s));
       parts = ceil_div(Dv, da::E);
     }
     da::decay_sum_kernel<<<unsigned(H), 256, 0, s>>>(part, grad_log_decay, Bsz * job.segs * parts, accumulate);
     PGF_LAUNCH_CHECK();
   }
   if (L == 0) return PGF_OK;
-  struct { float* part; void* out; int64_t heads, d; } sums[3] = {{pq, grad_q, Hq, Dk}, {pk, grad_k, Hk, Dk}, {pv, grad_v, Hv, Dv}};
-  for (auto& t : sums)
-    if (t.part) {
-      if (f32) PGF_TRY(da::share_sum<float>(t.part, t.out, tokens, t.heads, H, t.d, s));
-      else PGF_TRY(da::share_sum<__nv_bfloat16>(t.part, t.out, tokens, t.heads, H, t.d, s));
-    }
+  const struct { float* part; void* out; int64_t heads, d; } sums[3] = {{pq, grad_q, Hq, Dk}, {pk, grad_k, Hk, Dk}, {pv, grad_v, Hv, Dv}};
+  da::ShareSet set;
+  int count = 0;
+  int64_t most = 0;
+  for (const auto& t : sums) {
+    if (!t.part) continue;
+    set.part[count] = t.part;
+    set.out[count] = t.out;
+    set.n[count] = tokens * t.heads * t.d;
+    set.heads[count] = int(t.heads);
+    set.group[count] = int(H / t.heads);
+    set.d[count] = int(t.d);
+    if (set.n[count] > most) most = set.n[count];
+    ++count;
+  }
+  if (count) {
+    int64_t ctas = (most + 255) / 256;
+    if (ctas > 148 * 16) ctas = 148 * 16;
+    if (f32) da::share_sum_kernel<float><<<dim3(unsigned(ctas), unsigned(count)), 256, 0, s>>>(set);
+    else da::share_sum_kernel<__nv_bfloat16><<<dim3(unsigned(ctas), unsigned(count)), 256, 0, s>>>(set);
+    PGF_LAUNCH_CHECK();
+  }
   return PGF_OK;
 }
 
