@@ -851,13 +851,12 @@ def rotary_turns(dim: int, base: float = 10000.0, device="cuda") -> torch.Tensor
     return (f * 2.0 ** 64).to(torch.int64).to(device)
 
 
-def _acts(name: str, *ts: torch.Tensor) -> Tuple[int, int]:
+def _acts(name: str, first: torch.Tensor, *others: torch.Tensor) -> Tuple[int, int]:
     """(type code, device index) of activations that share both."""
-    first = ts[0]
     dtype, dev = first.dtype, first.get_device()
     if dev < 0:
         raise RuntimeError("icml_b200 operators run on CUDA tensors only (no CPU path)")
-    for t in ts:
+    for t in others:
         if t.dtype is not dtype or t.get_device() != dev:
             raise TypeError(f"{name}: tensors of {dtype} on cuda:{dev} and {t.dtype} on {t.device}")
     dt = _DT.get(dtype)
@@ -867,12 +866,13 @@ def _acts(name: str, *ts: torch.Tensor) -> Tuple[int, int]:
 
 
 def _view(t: torch.Tensor):
-    """(tensor, its strides for the C boundary): any (B, L, heads, D) or (B, heads, D) view whose last
-    dimension is contiguous goes as it is, anything else is copied."""
+    """(tensor, its strides for the C boundary or None): any (B, L, heads, D) or (B, heads, D) view whose
+    last dimension is contiguous goes as it is, anything else is copied."""
+    if t.is_contiguous():
+        return t, None
     st = t.stride()
     if st[-1] != 1 and t.shape[-1] > 1:
-        t = t.contiguous()
-        st = t.stride()
+        return t.contiguous(), None
     return t, (Strides(st[0], st[1], st[2]) if len(st) == 4 else Strides(st[0], 0, st[1]))
 
 
@@ -902,10 +902,13 @@ def _raw_stream(dev: int) -> int:
 
 def _qk_args(name, q, k, wq, wk, turns, positions, pairs):
     dt, dev = _acts(name, q, k)
-    qsh, ksh = q.shape, k.shape
-    if len(qsh) != 4 or len(ksh) != 4 or qsh[0] != ksh[0] or qsh[1] != ksh[1] or qsh[3] != ksh[3]:
-        raise ValueError(f"{name}: queries {tuple(qsh)} and keys {tuple(ksh)}, want (B, L, heads, D)")
-    B, L_, _, D = qsh
+    try:
+        (B, L_, Hq, D), (Bk, Lk, Hk, Dk) = q.shape, k.shape
+        same = B == Bk and L_ == Lk and D == Dk
+    except ValueError:
+        same = False
+    if not same:
+        raise ValueError(f"{name}: queries {tuple(q.shape)} and keys {tuple(k.shape)}, want (B, L, heads, D)")
     if wq is not None:
         wq = _param(name, wq, (D,), dev)
     if wk is not None:
@@ -923,7 +926,7 @@ def _qk_args(name, q, k, wq, wk, turns, positions, pairs):
     code = PAIRS.get(pairs)
     if code is None:
         raise ValueError(f"{name}: pairs {pairs!r} (halves or neighbours)")
-    return dt, dev, B, L_, qsh[2], ksh[2], D, R, wq, wk, turns, positions, code
+    return dt, dev, B, L_, Hq, Hk, D, R, wq, wk, turns, positions, code
 
 
 def qk_norm_rotate_fwd(q, k, wq=None, wk=None, turns=None, *, positions=None, start: int = 0, eps: float = 1e-6,
@@ -935,7 +938,7 @@ def qk_norm_rotate_fwd(q, k, wq=None, wk=None, turns=None, *, positions=None, st
     dt, dev, B, L_, Hq, Hk, D, R, wq, wk, turns, positions, code = _qk_args("qk_norm_rotate_fwd", q, k, wq, wk, turns,
                                                                             positions, pairs)
     (q, qs), (k, ks) = _view(q), _view(k)
-    qo, ko = q.new_empty(q.shape), k.new_empty(k.shape)
+    qo, ko = q.new_empty((B, L_, Hq, D)), q.new_empty((B, L_, Hk, D))
     check(lib().pgf_qk_norm_rotate_fwd(q.data_ptr(), qs, k.data_ptr(), ks, _p(wq), _p(wk), _p(turns), _p(positions),
                                        start, qo.data_ptr(), ko.data_ptr(), B, L_, Hq, Hk, D, R, code, eps, dt,
                                        _raw_stream(dev)), "qk_norm_rotate_fwd")
@@ -975,13 +978,21 @@ def _decay_args(name, q, k, v, log_decay, dims):
     """Checks what the decay-attention calls share; (type, device, B, L, H, Hq, Hk, Hv, Dk, Dv, log_decay)."""
     dt, dev = _acts(name, q, k, v)
     qsh, ksh, vsh = q.shape, k.shape, v.shape
-    if len(qsh) != dims or len(ksh) != dims or len(vsh) != dims or qsh[:-2] != ksh[:-2] or qsh[:-2] != vsh[:-2] \
-            or qsh[-1] != ksh[-1]:
+    try:
+        if dims == 4:
+            (B, L_, Hq, Dk), (Bk, Lk, Hk, Dq), (Bv, Lv, Hv, Dv) = qsh, ksh, vsh
+        else:
+            (B, Hq, Dk), (Bk, Hk, Dq), (Bv, Hv, Dv) = qsh, ksh, vsh
+            L_ = Lk = Lv = 1
+        same = B == Bk == Bv and L_ == Lk == Lv and Dk == Dq
+    except ValueError:
+        same = False
+    if not same:
         raise ValueError(f"{name}: q {tuple(qsh)}, k {tuple(ksh)}, v {tuple(vsh)}, want "
                          f"({'B, L' if dims == 4 else 'B'}, heads, D)")
     H = log_decay.numel()
     log_decay = _param(f"{name}: log_decay", log_decay, (H,), dev)
-    return dt, dev, qsh[0], qsh[1] if dims == 4 else 1, H, qsh[-2], ksh[-2], vsh[-2], qsh[-1], vsh[-1], log_decay
+    return dt, dev, B, L_, H, Hq, Hk, Hv, Dk, Dv, log_decay
 
 
 def decay_attn_fwd(q, k, v, log_decay, *, scale: Optional[float] = None, state=None, lengths=None,
