@@ -9,16 +9,20 @@
 // own score.  A NaN (a NaN or +inf logit, a row of -inf) counts as -inf: such candidates come last, in
 // index order.
 //
-// Bound by latency and, for large batches, by reading the logits.  One cluster of eight CTAs takes one
-// sequence, so that the whole step is one launch: the K rows (cut into parts where K < 8) go to the CTAs;
-// pass 1 takes the running maximum and sum of exponentials of each part and the largest logit of each
-// group of lanes; the parts' statistics meet through distributed shared memory; pass 2 (its reads hit L2)
-// forms c and keeps what is not below c at the K-th largest group maximum, a bound that at least K
-// candidates reach: a short list, ranked by counting.  The parts' best K keys meet the same way in one
+// Bound by latency and, for large batches, by reading the logits.  One cluster of CTAs (16 for few sequences,
+// else 8) takes one sequence, so that the whole step is one launch: the K rows (cut into parts where K is less
+// than the cluster) go to the CTAs; pass 1 takes the maximum and sum of exponentials of each part and the
+// largest logit of each group of lanes; the parts' statistics meet through distributed shared memory; pass 2
+// forms c and keeps what is not below c at the K-th largest group maximum, a bound that at least K candidates
+// reach: a short list, ranked by counting.  A part of 64 to 208 KB is copied once into shared memory (bulk copies,
+// worked on as they arrive) and read from there in both passes (16 rows x 8 beams x 50257 in bf16: 16.6 us, 23
+// with two readings); shorter ones are read twice, the second time from L1 and L2 (4 beams x 50257 in float32 over
+// 16 CTAs: 9.2 us, 10.2 through shared memory), and so are longer ones.  The loops stay short on purpose: a part unrolled into
+// registers ran slower (29 us at the first of these sizes), fetching instructions that run once.  The parts' best K keys meet the same way in one
 // CTA, which ranks them and writes the step's outputs.  A key is the order-preserving image of c above
 // the complement of the flat index, so one 64-bit comparison is the whole order.  A list that does not
 // fit (rows of equal logits) falls back to K passes of a plain maximum.
-#include "common.cuh"
+#include "tc_common.cuh"
 
 #include <cooperative_groups.h>
 
@@ -27,11 +31,11 @@ namespace beam {
 
 namespace cg = cooperative_groups;
 
-constexpr int CS = 8;              // CTAs of a cluster: one sequence
 constexpr int THREADS = 512;
 constexpr int MAX_K = 32;
-constexpr int UNITS = MAX_K / CS;  // (row, part) units of one CTA at most
 constexpr int LIST = 1024;
+constexpr int CHUNKS = 4;          // a held part is copied in this many
+constexpr int HELD_LEAST = 64 * 1024, HELD_MOST = 208 * 1024;   // bytes of a part that is held
 
 struct Args {
   const void* logits;        // (B, K, V)
@@ -42,6 +46,26 @@ struct Args {
   int64_t* out_tokens;       // (B, K)
   uint8_t* out_finished;     // (B, K)
   int K, V, end, parts;
+};
+
+// A row's columns [lo, hi) for the CTA's threads: single elements up to a 16-byte boundary, 16-byte pieces, single
+// elements behind them (a row of an odd vocabulary starts anywhere).
+template <class T>
+struct Span {
+  static constexpr int W = 16 / int(sizeof(T));
+  const T* row;
+  int lo, hi, a0, nv;
+  __device__ __forceinline__ Span(const T* row, int lo, int hi) : row(row), lo(lo), hi(hi) {
+    const int mis = int((reinterpret_cast<uintptr_t>(row + lo) & 15) / sizeof(T));
+    a0 = min(hi, mis ? lo + W - mis : lo);
+    nv = (hi - a0) / W;
+  }
+  __device__ __forceinline__ const uint4* pieces() const { return reinterpret_cast<const uint4*>(row + a0); }
+  // this thread's single elements in front (0) and behind (1): the column, or -1
+  __device__ __forceinline__ int single(int which) const {
+    const int c = which ? a0 + nv * W + int(threadIdx.x) : lo + int(threadIdx.x);
+    return c < (which ? hi : a0) ? c : -1;
+  }
 };
 
 __device__ __forceinline__ float candidate(float x, float lse, float score) {
@@ -57,12 +81,10 @@ __device__ __forceinline__ float score_of(uint64_t key) {
   return __uint_as_float(u & 0x80000000u ? u & 0x7FFFFFFFu : ~u);
 }
 
-__device__ __forceinline__ void each16(const float* p, float (&f)[4]) {
-  const float4 t = __ldg(reinterpret_cast<const float4*>(p));
-  f[0] = t.x; f[1] = t.y; f[2] = t.z; f[3] = t.w;
+__device__ __forceinline__ void unpack(const uint4& t, float (&f)[4]) {
+  f[0] = __uint_as_float(t.x); f[1] = __uint_as_float(t.y); f[2] = __uint_as_float(t.z); f[3] = __uint_as_float(t.w);
 }
-__device__ __forceinline__ void each16(const __nv_bfloat16* p, float (&f)[8]) {
-  const uint4 t = __ldg(reinterpret_cast<const uint4*>(p));
+__device__ __forceinline__ void unpack(const uint4& t, float (&f)[8]) {
   const uint32_t w[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -71,34 +93,49 @@ __device__ __forceinline__ void each16(const __nv_bfloat16* p, float (&f)[8]) {
   }
 }
 
-// body(v, n, at): n consecutive elements from column `at`, for this thread's share of [lo, hi): 16-byte
-// loads where the address allows, single elements in front of and behind them (a row of an odd
-// vocabulary starts anywhere).
-template <class T, class Body>
-__device__ __forceinline__ void scan_row(const T* row, int lo, int hi, Body body) {
-  constexpr int W = 16 / int(sizeof(T));
-  const int mis = int((reinterpret_cast<uintptr_t>(row + lo) & 15) / sizeof(T));
-  const int a0 = min(hi, mis ? lo + W - mis : lo);
-  const int nv = (hi - a0) / W;
-  float f[W];
-  if (lo + int(threadIdx.x) < a0) {
-    f[0] = ld(row, lo + threadIdx.x);
-    body(f, 1, lo + int(threadIdx.x));
+// body(values, at): an array of consecutive elements from column `at`, for this thread's share of the span.
+// HELD: the pieces lie in shared memory from `at_smem` on; chunk c of them is there once bars[c] has completed.
+template <bool HELD, class T, class Body>
+__device__ __forceinline__ bool scan(const Span<T>& sp, uint32_t at_smem, uint64_t* bars, Body body) {
+  constexpr int W = Span<T>::W;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const int c = sp.single(e);
+    if (c >= 0) {
+      const float one[1] = {ld(sp.row, c)};
+      body(one, c);
+    }
   }
+  if (HELD) {
+    const int per = (sp.nv + CHUNKS - 1) / CHUNKS;
+    for (int c = 0; c < CHUNKS; ++c) {
+      if (bars && !mbar_wait_warp(&bars[c], 0)) return false;
+      const int end = min(sp.nv, (c + 1) * per);
+#pragma unroll 2
+      for (int i = c * per + threadIdx.x; i < end; i += THREADS) {
+        uint4 t;
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(t.x), "=r"(t.y), "=r"(t.z), "=r"(t.w)
+                     : "r"(at_smem + uint32_t(i) * 16));
+        float f[W];
+        unpack(t, f);
+        body(f, sp.a0 + i * W);
+      }
+    }
+  } else {
 #pragma unroll 4
-  for (int i = threadIdx.x; i < nv; i += THREADS) {
-    each16(row + a0 + i * W, f);
-    body(f, W, a0 + i * W);
+    for (int i = threadIdx.x; i < sp.nv; i += THREADS) {
+      float f[W];
+      unpack(__ldg(sp.pieces() + i), f);
+      body(f, sp.a0 + i * W);
+    }
   }
-  const int tail = a0 + nv * W + int(threadIdx.x);
-  if (tail < hi) {
-    f[0] = ld(row, tail);
-    body(f, 1, tail);
-  }
+  return true;
 }
 
-template <class T>
-__global__ void __cluster_dims__(CS, 1, 1) __launch_bounds__(THREADS) select_kernel(const Args a) {
+// HOLD: every CTA has one unit at most, and it fits shared memory.
+template <class T, int CS, bool HOLD>
+__global__ void __cluster_dims__(CS, 1, 1) __launch_bounds__(THREADS, 1) select_kernel(const Args a) {
+  constexpr int UNITS = MAX_K / CS;                  // (row, part) units of one CTA at most
   constexpr int WARPS = THREADS / 32;
   __shared__ float s_max[UNITS], s_sum[UNITS];       // a unit's maximum and sum, read by the cluster
   __shared__ float s_tau[UNITS];                     // the logit that at least K of the unit reach
@@ -106,6 +143,10 @@ __global__ void __cluster_dims__(CS, 1, 1) __launch_bounds__(THREADS) select_ker
   __shared__ uint64_t s_list[LIST];
   __shared__ float s_wm[WARPS], s_ws[WARPS], s_g[2 * WARPS];
   __shared__ int s_n;
+  __shared__ float s_lse;
+  __shared__ uint64_t s_bars[CHUNKS];
+  __shared__ float s_score[UNITS];
+  __shared__ bool s_done[UNITS], s_fixed[UNITS];
   __shared__ uint64_t s_wk[WARPS];
   cg::cluster_group cl = cg::this_cluster();
   const int rank = int(cl.block_rank());
@@ -115,23 +156,62 @@ __global__ void __cluster_dims__(CS, 1, 1) __launch_bounds__(THREADS) select_ker
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   constexpr float L2E = 1.4426950408889634f;
 
-  // a unit without candidates of its own scan: its row has finished, or cannot go on at all
-  auto fixed = [&](int k) { return (a.finished && a.finished[b * K + k]) || a.scores[b * K + k] == -INFINITY; };
+  // s_fixed: a unit without candidates of its own scan, as its row has finished or cannot go on at all
+  for (int u = rank + CS * int(threadIdx.x); u < U; u += CS * THREADS) {
+    const int n = u / CS, k = u / P;
+    const float score = a.scores[b * K + k];
+    const bool done = a.finished && a.finished[b * K + k];
+    s_score[n] = score;
+    s_done[n] = done;
+    s_fixed[n] = done || score == -INFINITY;
+  }
+  auto span = [&](int u) {
+    const int lo = min(V, (u % P) * len);
+    return Span<T>(static_cast<const T*>(a.logits) + (b * K + u / P) * V, lo, min(V, lo + len));
+  };
+  uint32_t held = 0;
+  if constexpr (HOLD) {
+    extern __shared__ __align__(128) uint8_t smem[];
+    held = smem_u32(smem);
+    if (threadIdx.x == 0) {
+      for (int c = 0; c < CHUNKS; ++c) mbar_init(&s_bars[c], 1);
+      asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+      if (rank < U) {
+        const Span<T> sp = span(rank);
+        const int per = (sp.nv + CHUNKS - 1) / CHUNKS;
+        for (int c = 0; c < CHUNKS; ++c) {
+          const int i = min(sp.nv, c * per), n = min(sp.nv, i + per) - i;
+          mbar_expect_tx(&s_bars[c], uint32_t(n) * 16);
+          if (n > 0)
+            asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                         ::"r"(held + uint32_t(i) * 16), "l"(sp.pieces() + i), "r"(uint32_t(n) * 16),
+                           "r"(smem_u32(&s_bars[c])) : "memory");
+        }
+      }
+    }
+  }
+  bool ok = true;
+  __syncthreads();
 
   // ---- pass 1: maximum, sum of exponentials, group maxima
   for (int u = rank, n = 0; u < U; u += CS, ++n) {
-    const int k = u / P, lo = min(V, (u % P) * len), hi = min(V, lo + len);
     float m = -INFINITY, s = 0.f;
-    if (!fixed(k)) {
-      scan_row(static_cast<const T*>(a.logits) + (b * K + k) * V, lo, hi, [&](const float* f, int cnt, int) {
-        float mm = m;
-        for (int e = 0; e < cnt; ++e) mm = fmaxf(mm, f[e]);
+    if (!s_fixed[n]) {
+      ok = scan<HOLD>(span(u), held, s_bars, [&](const auto& f, int) {
+        constexpr int n = int(sizeof(f) / sizeof(float));
+        float mm = f[0];
+#pragma unroll
+        for (int e = 1; e < n; ++e) mm = fmaxf(mm, f[e]);
         if (mm > m) {
-          s *= exp2f((m - mm) * L2E);
+          s *= ex2f((m - mm) * L2E);
           m = mm;
         }
-        if (m != -INFINITY)
-          for (int e = 0; e < cnt; ++e) s += exp2f((f[e] - m) * L2E);
+        if (m != -INFINITY) {
+          float q = 0.f;
+#pragma unroll
+          for (int e = 0; e < n; ++e) q += ex2f((f[e] - m) * L2E);
+          s += q;
+        }
       });
     }
     // the K-th largest of the maxima of 16 warps (K <= 16) or 32 half warps: that many candidates reach it
@@ -141,7 +221,7 @@ __global__ void __cluster_dims__(CS, 1, 1) __launch_bounds__(THREADS) select_ker
     const int groups = K <= WARPS ? WARPS : 2 * WARPS;
     if (K <= WARPS ? lane == 0 : (lane & 15) == 0) s_g[K <= WARPS ? warp : threadIdx.x >> 4] = gm;
     const float wm = warp_max(m);
-    s = wm == -INFINITY ? s : s * exp2f((m - wm) * L2E);
+    s = wm == -INFINITY ? s : s * ex2f((m - wm) * L2E);
     s = warp_sum(s);
     if (lane == 0) { s_wm[warp] = wm; s_ws[warp] = s; }
     __syncthreads();
@@ -151,12 +231,14 @@ __global__ void __cluster_dims__(CS, 1, 1) __launch_bounds__(THREADS) select_ker
       for (int g = 0; g < groups; ++g) before += s_g[g] > mine || (s_g[g] == mine && g < int(threadIdx.x));
       if (before == K - 1) s_tau[n] = mine;
     }
-    if (threadIdx.x == 0) {
-      float tm = -INFINITY, ts = 0.f;
-      for (int w = 0; w < WARPS; ++w) tm = fmaxf(tm, s_wm[w]);
-      for (int w = 0; w < WARPS; ++w) ts += s_wm[w] == -INFINITY ? s_ws[w] : s_ws[w] * exp2f((s_wm[w] - tm) * L2E);
-      s_max[n] = tm;
-      s_sum[n] = ts;
+    if (warp == 1) {  // (the first warps' threads find the group's bound)
+      const float pm = lane < WARPS ? s_wm[lane] : -INFINITY, ps = lane < WARPS ? s_ws[lane] : 0.f;
+      const float tm = warp_max(pm);
+      const float ts = warp_sum(pm == -INFINITY ? ps : ps * ex2f((pm - tm) * L2E));
+      if (lane == 0) {
+        s_max[n] = tm;
+        s_sum[n] = ts;
+      }
     }
     __syncthreads();
   }
@@ -164,15 +246,15 @@ __global__ void __cluster_dims__(CS, 1, 1) __launch_bounds__(THREADS) select_ker
 
   // ---- pass 2: the unit's first K keys
   for (int u = rank, n = 0; u < U; u += CS, ++n) {
-    const int k = u / P, lo = min(V, (u % P) * len), hi = min(V, lo + len);
-    const float score = a.scores[b * K + k];
+    const int k = u / P;
+    const float score = s_score[n];
     const uint32_t flat0 = uint32_t(k) * uint32_t(V);
     if (threadIdx.x < MAX_K) s_best[n][threadIdx.x] = 0;  // below every key
     if (threadIdx.x == 0) s_n = 0;
     __syncthreads();
-    if (fixed(k)) {
+    if (s_fixed[n]) {
       // the end token at the score (if it has finished), then -inf from the lowest index
-      const bool done = a.finished && a.finished[b * K + k] && score > -INFINITY;
+      const bool done = s_done[n] && score > -INFINITY;
       const int j = threadIdx.x;
       if (u % P == 0 && j < K) {
         if (done && j == 0) {
@@ -186,28 +268,34 @@ __global__ void __cluster_dims__(CS, 1, 1) __launch_bounds__(THREADS) select_ker
       __syncthreads();
       continue;
     }
-    float m = -INFINITY, s = 0.f;
-    for (int p = 0; p < P; ++p) {
-      const int v = k * P + p;
-      m = fmaxf(m, cl.map_shared_rank(s_max, v % CS)[v / CS]);
+    if (warp == 0) {  // the row's log sum from its parts' (at most CS of them)
+      const int v = k * P + lane;
+      const float pm = lane < P ? cl.map_shared_rank(s_max, v % CS)[v / CS] : -INFINITY;
+      const float ps = lane < P ? cl.map_shared_rank(s_sum, v % CS)[v / CS] : 0.f;
+      const float m = warp_max(pm);
+      const float s = warp_sum(pm == -INFINITY ? ps : ps * ex2f((pm - m) * L2E));
+      if (lane == 0) s_lse = m + logf(s);
     }
-    for (int p = 0; p < P; ++p) {
-      const int v = k * P + p;
-      const float pm = cl.map_shared_rank(s_max, v % CS)[v / CS], ps = cl.map_shared_rank(s_sum, v % CS)[v / CS];
-      s += pm == -INFINITY ? ps : ps * exp2f((pm - m) * L2E);
-    }
-    const float lse = m + logf(s);
+    __syncthreads();
+    const float lse = s_lse;
     const float bound = candidate(s_tau[n], lse, score);
-    const T* row = static_cast<const T*>(a.logits) + (b * K + k) * V;
-    scan_row(row, lo, hi, [&](const float* f, int cnt, int at) {
-      for (int e = 0; e < cnt; ++e) {
-        const float c = candidate(f[e], lse, score);
-        if (c >= bound) {
-          const int i = atomicAdd(&s_n, 1);
-          if (i < LIST) s_list[i] = key_of(c, flat0 + at + e);
+    const Span<T> sp = span(u);
+    auto keep = [&](const auto& f, int at) {
+      constexpr int n = int(sizeof(f) / sizeof(float));
+      float top = f[0];                       // c grows with the logit: the largest speaks for its piece
+#pragma unroll
+      for (int e = 1; e < n; ++e) top = fmaxf(top, f[e]);
+      if (candidate(top, lse, score) >= bound) {
+        for (int e = 0; e < n; ++e) {
+          const float c = candidate(f[e], lse, score);
+          if (c >= bound) {
+            const int i = atomicAdd(&s_n, 1);
+            if (i < LIST) s_list[i] = key_of(c, flat0 + at + e);
+          }
         }
       }
-    });
+    };
+    scan<HOLD>(sp, held, nullptr, keep);
     __syncthreads();
     const int cnt = s_n;
     if (cnt <= LIST) {
@@ -221,8 +309,9 @@ __global__ void __cluster_dims__(CS, 1, 1) __launch_bounds__(THREADS) select_ker
       uint64_t last = ~uint64_t(0);
       for (int j = 0; j < K; ++j) {
         uint64_t top = 0;
-        scan_row(row, lo, hi, [&](const float* f, int c, int at) {
-          for (int e = 0; e < c; ++e) {
+        scan<HOLD>(sp, held, nullptr, [&](const auto& f, int at) {
+#pragma unroll
+          for (int e = 0; e < int(sizeof(f) / sizeof(float)); ++e) {
             const uint64_t key = key_of(candidate(f[e], lse, score), flat0 + at + e);
             if (key < last && key > top) top = key;
           }
@@ -245,7 +334,7 @@ __global__ void __cluster_dims__(CS, 1, 1) __launch_bounds__(THREADS) select_ker
 
   // ---- the sequence's K: all units' keys ranked by counting
   if (rank == 0) {
-    static_assert(MAX_K * MAX_K <= LIST && CS * CS <= LIST, "the units' keys fit the list");
+    static_assert(MAX_K * MAX_K <= LIST && CS * MAX_K <= LIST, "the units' keys fit the list");
     for (int i = threadIdx.x; i < U * K; i += THREADS) {
       const int u = i / K;
       s_list[i] = cl.map_shared_rank(&s_best[0][0], u % CS)[(u / CS) * MAX_K + i % K];
@@ -267,6 +356,55 @@ __global__ void __cluster_dims__(CS, 1, 1) __launch_bounds__(THREADS) select_ker
     }
   }
   cl.sync();  // the others' shared memory stays until it has been read
+}
+
+template <class T, int CS>
+static int select_as(Args a, int64_t Bsz, cudaStream_t s) {
+  constexpr int W = Span<T>::W;
+  a.parts = a.K < CS ? CS / a.K : 1;
+  const int len = (a.V + a.parts - 1) / a.parts;
+  const size_t bytes = size_t(len) / W * 16;
+  const unsigned grid = unsigned(Bsz * CS);
+  if (a.K * a.parts <= CS && bytes >= HELD_LEAST && bytes <= HELD_MOST) {
+    static int limit = 0;
+    PGF_CUDA(ensure_dynamic_smem(select_kernel<T, CS, true>, bytes, limit));
+    select_kernel<T, CS, true><<<grid, THREADS, bytes, s>>>(a);
+  } else {
+    select_kernel<T, CS, false><<<grid, THREADS, 0, s>>>(a);
+  }
+  PGF_LAUNCH_CHECK();
+  return PGF_OK;
+}
+
+// Clusters of 16 are beyond the portable size: asked for once, and used if the device can place one.
+template <class T>
+static bool wide_clusters() {
+  static const bool ok = [] {
+    for (auto* k : {select_kernel<T, 16, true>, select_kernel<T, 16, false>})
+      if (cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return false;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = dim3(16);
+    c.blockDim = dim3(THREADS);
+    cudaLaunchAttribute at;
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = 16;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    c.attrs = &at;
+    c.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, select_kernel<T, 16, true>, &c) != cudaSuccess || n < 1) {
+      cudaGetLastError();
+      return false;
+    }
+    return true;
+  }();
+  return ok;
+}
+
+// 16 CTAs a sequence while all of them run at once (a GPC holds one such cluster).
+template <class T>
+static int select(const Args& a, int64_t Bsz, cudaStream_t s) {
+  return Bsz <= 4 && wide_clusters<T>() ? select_as<T, 16>(a, Bsz, s) : select_as<T, 8>(a, Bsz, s);
 }
 
 constexpr int MAX_T = 64;           // tensors of one reorder launch
@@ -310,6 +448,9 @@ __global__ void __launch_bounds__(256) reorder_kernel(const __grid_constant__ Ta
 }
 
 }  // namespace beam
+
+int beam_fault() { return take_tc_fault(); }
+
 }  // namespace pgf
 
 using namespace pgf;
@@ -329,14 +470,9 @@ extern "C" int pgf_beam_select(const void* logits, const float* scores, const ui
   PGF_CHECK_ARG(logits && scores && out_scores && out_rows && out_tokens, "beam_select: null pointer");
   PGF_CHECK_ARG(aligned(logits, dtype == PGF_DTYPE_BF16 ? 2 : 4), "beam_select: misaligned logits");
   beam::Args a = {logits, scores, finished, out_scores, out_rows, out_tokens, out_finished,
-                  int(K), int(V), int(end_id), K < beam::CS ? int(beam::CS / K) : 1};
-  const unsigned grid = unsigned(Bsz * beam::CS);
-  if (dtype == PGF_DTYPE_BF16)
-    beam::select_kernel<__nv_bfloat16><<<grid, beam::THREADS, 0, as_stream(stream)>>>(a);
-  else
-    beam::select_kernel<float><<<grid, beam::THREADS, 0, as_stream(stream)>>>(a);
-  PGF_LAUNCH_CHECK();
-  return PGF_OK;
+                  int(K), int(V), int(end_id), 1};
+  if (dtype == PGF_DTYPE_BF16) return beam::select<__nv_bfloat16>(a, Bsz, as_stream(stream));
+  return beam::select<float>(a, Bsz, as_stream(stream));
 }
 
 extern "C" int pgf_beam_reorder(const void* const* src, void* const* dst, const int64_t* row_bytes, int count,

@@ -989,7 +989,7 @@ int tc_ce_bwd(const Gemm& g, const int64_t* targets, const float* lse, float sca
 extern "C" int pgf_tc_fault(void) {
   const int a = pgf::take_tc_fault();
   const int b = pgf::lmhead_tc_fault();
-  const int c = pgf::decay_tc_fault(), d = pgf::decay_tangent_tc_fault();
-  if (a < 0 || b < 0 || c < 0 || d < 0) return -1;
-  return (a || b || c || d) ? 1 : 0;
+  const int c = pgf::decay_tc_fault(), d = pgf::decay_tangent_tc_fault(), e = pgf::beam_fault();
+  if (a < 0 || b < 0 || c < 0 || d < 0 || e < 0) return -1;
+  return (a || b || c || d || e) ? 1 : 0;
 }
