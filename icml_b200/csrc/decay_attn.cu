@@ -616,7 +616,7 @@ struct Entering {
 
 static int f_calls(const Job* job, int count, const Plan& pl, int dtype, cudaStream_t s) {
   if (!pl.tc) return walk<MODE_OUT>(job, count, TangentArgs{}, dtype, s);
-  for (int k = 0; k < count; ++k) PGF_TRY(tc_walk(job[k], false, s));
+  for (int k = 0; k < count; ++k) PGF_TRY(tc_walk(job[k], s));
   return PGF_OK;
 }
 
@@ -641,7 +641,7 @@ static int entering(Job* job, int count, const Plan& pl, const float* const* fir
     e[k] = {pieces[k], segs * n};
   }
   if (pl.tc) {
-    for (int k = 0; k < count; ++k) PGF_TRY(tc_walk(job[k], true, s));
+    for (int k = 0; k < count; ++k) PGF_TRY(tc_pieces(job[k], s));
   } else {
     PGF_TRY(walk<MODE_STATE>(job, count, TangentArgs{}, dtype, s));
   }

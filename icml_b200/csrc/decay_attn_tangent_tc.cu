@@ -39,7 +39,7 @@ constexpr uint32_t BARS = TAB + 656 + 64;
 constexpr uint32_t BYTES = BARS + 256 + 1024;
 static_assert(BYTES <= 232448, "fits an SM");
 constexpr uint32_t T_A = 0, T_B = 128, T_U = 256, T_V = 320;
-enum { B_AB = 0, B_U, B_V, B_K, B_Q, B_X, B_COUNT };      // B_U, B_V, B_K, B_Q: a phase per half
+enum { B_AB = 0, B_U, B_V, B_K, B_Q, B_X, B_DONE, B_COUNT };      // B_U, B_V, B_K, B_Q: a phase per half
 
 struct Params {
   const float* log_decay;
@@ -120,6 +120,7 @@ tangent_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         __syncwarp();
       }
     }
+    copies_landed<NS>(full, n);
   } else if (warp == 1) {
     const bool leader = elect_one();
     const uint32_t id_a = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(C >> 3) << 17) | (uint32_t(C >> 4) << 24);
@@ -172,6 +173,7 @@ tangent_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         __syncwarp();
       }
     }
+    products_done(&bars[B_DONE], leader);
   } else if (warp < 18) {
     const int q = warp & 3, cg = (warp - 2) >> 2, i = q * 32 + lane, tid = int(threadIdx.x) - 64;
     const uint32_t row = uint32_t(q * 32) << 16;

@@ -69,20 +69,20 @@ struct Params {
   float* end;
   float scale, z_scale;
   int64_t L, seg_len;
-  int H, segs, dx, dz, start_t, out_f32, last_too;
+  int H, segs, dx, dz, start_t, out_f32;
   int gx, gy, gz;              // operator heads per tensor head
 };
 
 // Barriers behind full[NS] and empty[NS].  A and P take turns where there are two A buffers: X may be a chunk
 // ahead of the product that reads P.
-enum { B_A = 0, B_A1, B_P, B_P1, B_O, B_DFREE, B_K, B_U, B_S, B_OSTAGED, B_SUM, B_COUNT };
+enum { B_A = 0, B_A1, B_P, B_P1, B_O, B_DFREE, B_K, B_U, B_S, B_OSTAGED, B_SUM, B_DONE, B_COUNT };
 
-template <int DX, int DZ, int NT, bool STATE_ONLY, bool REV>
+template <int DX, int DZ, int NT, bool REV>
 struct Walk {
   using G = Cfg<DX, DZ, NT>;
-  static constexpr int PER = STATE_ONLY ? 2 : 3;      // tiles of a chunk
+  static constexpr int PER = 3;                       // tiles of a chunk
   static constexpr int HC = DZ / 2;                   // columns of one X or Y warp
-  static constexpr int CONV = STATE_ONLY ? 512 : 256; // threads that weigh y
+  static constexpr int CONV = 256;                    // threads that weigh y
 
   const Params& p;
   uint8_t* base;
@@ -113,7 +113,7 @@ struct Walk {
     if (lane == 0) mbar_arrive(&bars[which]);
   }
 
-  // Places of a chunk's tiles in the ring's order y, x, z (y, z).
+  // Places of a chunk's tiles in the ring's order y, x, z.
   __device__ __forceinline__ uint32_t tile_y(int c) const { return uint32_t(c) * PER; }
   __device__ __forceinline__ uint32_t tile_x(int c) const { return uint32_t(c) * PER + 1; }
   __device__ __forceinline__ uint32_t tile_z(int c) const { return uint32_t(c) * PER + PER - 1; }
@@ -122,12 +122,13 @@ struct Walk {
   __device__ void load(const CUtensorMap* mx, const CUtensorMap* my, const CUtensorMap* mz) const {
     const bool leader = elect_one();
     uint32_t n = 0;
-    for (int c = 0; c < chunks; ++c) {
+    bool ok = true;
+    for (int c = 0; c < chunks && ok; ++c) {
       const int t0 = int(first_token(c));
       for (int i = 0; i < PER; ++i, ++n) {
         const int k = i == 0 ? 1 : i == PER - 1 ? 2 : 0;
         const uint32_t s = slot(n), r = n / G::NS;
-        if (r > 0 && !warp_wait(&empty[s], (r - 1) & 1)) return;
+        if (r > 0 && !warp_wait(&empty[s], (r - 1) & 1)) { ok = false; break; }
         if (leader) {
           const CUtensorMap* m = k == 0 ? mx : k == 1 ? my : mz;
           const int hh = h / (k == 0 ? p.gx : k == 1 ? p.gy : p.gz);
@@ -139,12 +140,12 @@ struct Walk {
         __syncwarp();
       }
     }
+    copies_landed<G::NS>(full, n);
   }
 
   // ---- warp 1.  A tile's slot is released by the last product that reads it (z's by the output's store).  With
   // two A buffers A of the next chunk goes first; with one it comes last.
-  __device__ void mma() const {
-    const bool leader = elect_one();
+  __device__ void mma(const bool leader) const {
     const uint32_t id_a = (1u << 4) | (1u << 7) | (1u << 10) | (uint32_t(C >> 3) << 17) | (uint32_t(C >> 4) << 24);
     const uint32_t id_d = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (uint32_t(DZ >> 3) << 17) |
                           (uint32_t(C >> 4) << 24);
@@ -166,10 +167,10 @@ struct Walk {
       __syncwarp();
       return true;
     };
-    if (!STATE_ONLY && chunks > 0 && !product_a(0)) return;
+    if (chunks > 0 && !product_a(0)) return;
     for (int c = 0; c < chunks; ++c) {
       const bool more = c + 1 < chunks;
-      if (!STATE_ONLY && G::NA == 2 && more && !product_a(c + 1)) return;
+      if (G::NA == 2 && more && !product_a(c + 1)) return;
       if (!wait_full(tile_z(c)) || !wait(B_K, c)) return;
       tc_after();
       const Desc dz(at(tile_z(c)), BLK);
@@ -191,10 +192,8 @@ struct Walk {
           umma_bf16(tmem + G::T_U, dy.at(kk * 2048), dz.at(kk * 2048), id_u, NT == 3 || DX == 128 || kk > 0);
         umma_commit(&bars[B_U]);
         umma_commit(&empty[slot(tile_y(c))]);
-        if (STATE_ONLY) umma_commit(&empty[slot(tile_z(c))]);
       }
       __syncwarp();
-      if (STATE_ONLY) continue;
       if (!wait_turn(B_P, c)) return;
       if (c > 0 && !wait(B_DFREE, c - 1)) return;
       tc_after();
@@ -371,7 +370,7 @@ struct Walk {
     const uint32_t ny = tile_y(c), nz = tile_z(c);
     const int n = tokens(c);
     const uint32_t yb = sbase + slot(ny) * G::SLOT;
-    if (STATE_ONLY ? !wait_full(ny) : !wait_turn(B_A, c)) return false;
+    if (!wait_turn(B_A, c)) return false;
     constexpr int PIECES = DX / 64 * 1024 / CONV, BATCH = PIECES < 4 ? PIECES : 4;
 #pragma unroll
     for (int k0 = 0; k0 < PIECES; k0 += BATCH) {
@@ -435,7 +434,7 @@ struct Walk {
     const int64_t n_state = int64_t(p.dx) * p.dz;
     float2 s[HC / 2];
     {
-      const float* st = p.start && !STATE_ONLY ? p.start + bh * p.start_stride + int64_t(seg) * n_state : nullptr;
+      const float* st = p.start ? p.start + bh * p.start_stride + int64_t(seg) * n_state : nullptr;
 #pragma unroll
       for (int k = 0; k < HC; ++k) {
         const int c = half * HC + k;
@@ -446,9 +445,8 @@ struct Walk {
       }
     }
     for (int c = 0; c < chunks; ++c) {
-      // STATE_ONLY: the terms' buffers are free again (this warp has waited for U of c - 1)
-      if (!weigh(c, STATE_ONLY ? tid + 256 : tid)) return;
-      if (!STATE_ONLY) {
+      if (!weigh(c, tid)) return;
+      {
         // S as the bf16 operand of D1, once D1 of the chunk before has read its own
         if (c > 0 && !wait(B_O, c - 1)) return;
 #pragma unroll
@@ -476,11 +474,8 @@ struct Walk {
       }
       tc_before();
     }
-    // the state leaves: a piece's own (STATE_ONLY) or the whole walk's
-    float* end = nullptr;
-    if (STATE_ONLY) end = chunks > 0 || p.last_too || seg != (REV ? 0 : p.segs - 1)
-                              ? const_cast<float*>(p.start) + bh * p.start_stride + int64_t(seg) * n_state : nullptr;
-    else if (p.end && seg == (REV ? 0 : p.segs - 1)) end = p.end + bh * n_state;
+    // the state behind the whole walk leaves
+    float* end = p.end && seg == (REV ? 0 : p.segs - 1) ? p.end + bh * n_state : nullptr;
     if (!end) return;
     if (DX == 64) {
       // rows 64..127 hold the middle terms' part; the ring is done with
@@ -508,11 +503,11 @@ struct Walk {
   }
 };
 
-template <int DX, int DZ, int NT, bool STATE_ONLY, bool REV>
+template <int DX, int DZ, int NT, bool REV>
 __global__ void __launch_bounds__(THREADS, 1)
 walk_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmY,
                const __grid_constant__ CUtensorMap tmZ, const __grid_constant__ CUtensorMap tmO, const Params p) {
-  using W = Walk<DX, DZ, NT, STATE_ONLY, REV>;
+  using W = Walk<DX, DZ, NT, REV>;
   using G = typename W::G;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -531,9 +526,7 @@ walk_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
   w.len = row_length(p.lengths, w.b, p.L);
   w.s0 = min(w.len, int64_t(w.seg) * p.seg_len);
   w.s1 = min(w.len, w.s0 + p.seg_len);
-  // the end state of the walk's last piece enters no other piece
-  const bool idle = STATE_ONLY && !p.last_too && w.seg == (REV ? 0 : p.segs - 1);
-  w.chunks = idle ? 0 : int((w.s1 - w.s0 + C - 1) / C);
+  w.chunks = int((w.s1 - w.s0 + C - 1) / C);
 
   const float l2 = log2_decay(p.log_decay[w.h]);
   if (threadIdx.x <= C) {
@@ -545,9 +538,9 @@ walk_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
   if (threadIdx.x < 32) tab[132 + threadIdx.x] = exp2f(l2 * float(REV ? threadIdx.x : 31 - threadIdx.x));
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2 * G::NS; ++s) mbar_init(&full[s], 1);
-    for (int k = 0; k < B_COUNT; ++k) mbar_init(&bars[k], k == B_A || k == B_A1 || k == B_O || k == B_U ? 1 : k == B_K ? W::CONV / 32 : 8);
+    for (int k = 0; k < B_COUNT; ++k) mbar_init(&bars[k], k == B_A || k == B_A1 || k == B_O || k == B_U || k == B_DONE ? 1 : k == B_K ? W::CONV / 32 : 8);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    if (!STATE_ONLY) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmX)) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmX)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmY)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmZ)) : "memory");
   }
@@ -568,14 +561,11 @@ walk_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
   if (w.warp == 0) {
     w.load(&tmX, &tmY, &tmZ);
   } else if (w.warp == 1) {
-    w.mma();
+    const bool leader = elect_one();
+    w.mma(leader);
+    products_done(&bars[B_DONE], leader);
   } else if (w.warp < 10) {
-    if (STATE_ONLY) {
-      for (int c = 0; c < w.chunks; ++c) {
-        if (c > 0 && !w.wait(B_U, c - 1)) break;
-        if (!w.weigh(c, int(threadIdx.x) - 64)) break;
-      }
-    } else {
+    {
       bool ok = true;
       // with one A buffer the output goes first: the product that reads P waits for its accumulators
       for (int c = 0; c < w.chunks && ok; ++c) {
@@ -589,7 +579,7 @@ walk_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
   } else if (w.warp < 18) {
     w.state();
   } else if (w.warp == 18) {
-    if (!STATE_ONLY) w.store(&tmO);
+    w.store(&tmO);
   }
   tc_before();
   __syncthreads();
@@ -615,13 +605,13 @@ bool make_store_map(CUtensorMap* m, const Job& j, int cols) {
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DX, int DZ, int NT, bool STATE_ONLY, bool REV>
+template <int DX, int DZ, int NT, bool REV>
 int launch(const Job& j, cudaStream_t s) {
   static int limit = 0;
   using G = Cfg<DX, DZ, NT>;
-  CUtensorMap mx = {}, my, mz, mo = {};
-  if ((!STATE_ONLY && !make_tensor_map(&mx, j.x, j.B, j.L)) || !make_tensor_map(&my, j.y, j.B, j.L) ||
-      !make_tensor_map(&mz, j.z, j.B, j.L) || (!STATE_ONLY && !j.out_f32 && !make_store_map(&mo, j, DZ / 2))) {
+  CUtensorMap mx, my, mz, mo = {};
+  if (!make_tensor_map(&mx, j.x, j.B, j.L) || !make_tensor_map(&my, j.y, j.B, j.L) ||
+      !make_tensor_map(&mz, j.z, j.B, j.L) || (!j.out_f32 && !make_store_map(&mo, j, DZ / 2))) {
     set_error("decay_attn: tensor map");
     return PGF_ERR_CUDA;
   }
@@ -642,30 +632,27 @@ int launch(const Job& j, cudaStream_t s) {
   p.dz = j.z.d;
   p.start_t = j.start_t;
   p.out_f32 = j.out_f32;
-  p.last_too = j.last_too;
-  p.gx = STATE_ONLY ? 1 : j.H / j.x.heads;
+  p.gx = j.H / j.x.heads;
   p.gy = j.H / j.y.heads;
   p.gz = j.H / j.z.heads;
-  PGF_CUDA(ensure_dynamic_smem(walk_tc_kernel<DX, DZ, NT, STATE_ONLY, REV>, G::BYTES, limit));
-  walk_tc_kernel<DX, DZ, NT, STATE_ONLY, REV><<<unsigned(j.B * j.H * j.segs), THREADS, G::BYTES, s>>>(mx, my, mz, mo, p);
+  PGF_CUDA(ensure_dynamic_smem(walk_tc_kernel<DX, DZ, NT, REV>, G::BYTES, limit));
+  walk_tc_kernel<DX, DZ, NT, REV><<<unsigned(j.B * j.H * j.segs), THREADS, G::BYTES, s>>>(mx, my, mz, mo, p);
   PGF_LAUNCH_CHECK();
   return PGF_OK;
 }
 
-template <int NT, bool STATE_ONLY, bool REV>
+template <int NT, bool REV>
 int dispatch(const Job& j, cudaStream_t s) {
-  if (j.y.d <= 64)
-    return j.z.d <= 64 ? launch<64, 64, NT, STATE_ONLY, REV>(j, s) : launch<64, 128, NT, STATE_ONLY, REV>(j, s);
-  return j.z.d <= 64 ? launch<128, 64, NT, STATE_ONLY, REV>(j, s) : launch<128, 128, NT, STATE_ONLY, REV>(j, s);
+  if (j.y.d <= 64) return j.z.d <= 64 ? launch<64, 64, NT, REV>(j, s) : launch<64, 128, NT, REV>(j, s);
+  return j.z.d <= 64 ? launch<128, 64, NT, REV>(j, s) : launch<128, 128, NT, REV>(j, s);
 }
 
 }  // namespace
 
 bool tc_fits(const Tensor& t, int64_t B, int64_t L) { return fits(t, B, L); }
-int tc_walk(const Job& j, bool state_only, cudaStream_t s) {
-  if (state_only) return j.rev ? dispatch<3, true, true>(j, s) : dispatch<3, true, false>(j, s);
-  if (j.end) return j.rev ? dispatch<3, false, true>(j, s) : dispatch<3, false, false>(j, s);
-  return j.rev ? dispatch<2, false, true>(j, s) : dispatch<2, false, false>(j, s);
+int tc_walk(const Job& j, cudaStream_t s) {
+  if (j.end) return j.rev ? dispatch<3, true>(j, s) : dispatch<3, false>(j, s);
+  return j.rev ? dispatch<2, true>(j, s) : dispatch<2, false>(j, s);
 }
 
 }  // namespace da

@@ -13,8 +13,10 @@ constexpr uint32_t BLK = 16384;   // a tile of 128 rows x 64 bf16 columns, 128B 
 // Whether a bf16 tensor can be read by the engine's TMA loads: 16-byte aligned base, pitches and width, at
 // most 128 wide.
 bool tc_fits(const Tensor& t, int64_t B, int64_t L);
-// One F call, or only the pieces' own end states (into job.start).  job.seg_len: a multiple of TC_CHUNK.
-int tc_walk(const Job& job, bool state_only, cudaStream_t s);
+// One F call.  job.seg_len: a multiple of TC_CHUNK.
+int tc_walk(const Job& job, cudaStream_t s);
+// The pieces' own end states from zero, into job.start.
+int tc_pieces(const Job& job, cudaStream_t s);
 
 // grad ln a: partial sums (H, B, segs, blocks), blocks = tc_tangent_blocks(Dk, Dv).  start: the state that enters
 // each piece, behind: the adjoint (scaled) of the state behind it; NULL: zeros.
@@ -93,6 +95,17 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) {
   if (__all_sync(0xffffffffu, done)) return true;
   return mbar_wait_warp(bar, parity);
 }
+// Ends of the copying and the multiplying warp, after a wait that ran out too: no copy of the ring's first n tiles
+// and no product is in flight when the block leaves.
+template <int NS>
+__device__ __forceinline__ void copies_landed(uint64_t* full, uint32_t n) {
+  for (uint32_t k = n > NS ? n - NS : 0; k < n; ++k) warp_wait(&full[k % NS], (k / NS) & 1);
+}
+__device__ __forceinline__ void products_done(uint64_t* done, bool leader) {
+  if (leader) umma_commit(done);
+  __syncwarp();
+  warp_wait(done, 0);
+}
 // A matrix descriptor (sdesc) whose start moves by whole 16-byte units: the address field is the low 14 bits
 // and shared memory ends below 2^18, so a step never carries out of it.
 struct Desc {
@@ -105,15 +118,15 @@ struct Desc {
   __device__ __forceinline__ uint64_t at(uint32_t bytes) const { return uint64_t(hi) << 32 | (lo + (bytes >> 4)); }
 };
 
-// (D, heads, L, B) with a box of 64 columns x 128 tokens of one head; zeros outside.
-static inline bool make_tensor_map(CUtensorMap* m, const Tensor& t, int64_t B, int64_t L) {
+// (D, heads, L, B) with a box of 64 columns x `rows` tokens of one head; zeros outside.
+static inline bool make_tensor_map(CUtensorMap* m, const Tensor& t, int64_t B, int64_t L, int rows = TC_CHUNK) {
   EncodeTiledFn fn = encode_fn();
   if (!fn) return false;
   cuuint64_t dims[4] = {cuuint64_t(t.d), cuuint64_t(t.heads), cuuint64_t(L), cuuint64_t(B)};
   // the stride of a dimension of one entry is never used, but has to be a valid one
   cuuint64_t st[3] = {cuuint64_t(t.heads > 1 ? t.s.head : t.d) * 2, cuuint64_t(L > 1 ? t.s.token : t.d) * 2,
                       cuuint64_t(B > 1 ? t.s.batch : t.d) * 2};
-  cuuint32_t box[4] = {64, 1, TC_CHUNK, 1}, es[4] = {1, 1, 1, 1};
+  cuuint32_t box[4] = {64, 1, cuuint32_t(rows), 1}, es[4] = {1, 1, 1, 1};
   return fn(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(t.p), dims, st, box, es,
             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;

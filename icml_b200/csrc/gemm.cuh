@@ -85,6 +85,7 @@ int lmhead_tc_fault();
 int decay_tc_fault();
 int decay_tangent_tc_fault();
 int beam_fault();
+int decay_pieces_tc_fault();
 // Fused CE backward over M rows (lmhead_tc.cu): G = (softmax(h W^T) - onehot) * scale as bf16 (rows x
 // ldg, for grad W) and dh = G W (bf16, M x d) in one pass, G never re-read for dh.  d % 64 == 0,
 // d <= 256, 16-byte aligned operands; PGF_ERR_UNSUPPORTED otherwise.

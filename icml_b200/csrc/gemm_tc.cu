@@ -990,6 +990,7 @@ extern "C" int pgf_tc_fault(void) {
   const int a = pgf::take_tc_fault();
   const int b = pgf::lmhead_tc_fault();
   const int c = pgf::decay_tc_fault(), d = pgf::decay_tangent_tc_fault(), e = pgf::beam_fault();
-  if (a < 0 || b < 0 || c < 0 || d < 0 || e < 0) return -1;
-  return (a || b || c || d || e) ? 1 : 0;
+  const int f = pgf::decay_pieces_tc_fault();
+  if (a < 0 || b < 0 || c < 0 || d < 0 || e < 0 || f < 0) return -1;
+  return (a || b || c || d || e || f) ? 1 : 0;
 }
