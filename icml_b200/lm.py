@@ -103,9 +103,12 @@ class PGFLanguageModel:
                  weight_decay: float = 0.01, tie_embeddings: bool = False, init_std: float = 0.02,
                  variant: str = "reference", final_norm: bool = False, expand: int = 2, d_conv: int = 4,
                  dt_rank: Optional[int] = None, optimizer: Optional[str] = None,
-                 max_grad_norm: Optional[float] = None, stash: str = "device"):
+                 max_grad_norm: Optional[float] = None, stash: str = "device",
+                 n_heads: Optional[int] = None, n_kv_heads: Optional[int] = None):
         """variant "reference": the reference's PGFMambaBlock; "std": the Mamba-standard block
-        (pgf_mamba_std.PGFMambaStdBlock).  final_norm adds an RMSNorm before the LM head.
+        (pgf_mamba_std.PGFMambaStdBlock); "decay": decay attention (pgf_decay.PGFDecayBlock, with n_heads heads
+        over n_kv_heads keys and values, d_state wide queries and keys; generate.beam_search decodes with it).
+        final_norm adds an RMSNorm before the LM head.
         optimizer "flat" (default on a GPU): AdamW over one flat parameter buffer on libpgf's kernels
         (icml_b200.optim.FlatAdamW); "torch": torch.optim.AdamW (fused on a GPU).  max_grad_norm
         clips the global gradient norm first (flat optimizer only).  stash: where the layer inputs wait
@@ -126,6 +129,9 @@ class PGFLanguageModel:
             from .pgf_mamba_std import PGFMambaStdBlock
             blocks = [PGFMambaStdBlock(d_model, d_state, d_ff, block_size, expand, d_conv, dt_rank)
                       for _ in range(n_layers)]
+        elif variant == "decay":
+            from .pgf_decay import PGFDecayBlock
+            blocks = [PGFDecayBlock(d_model, d_state, d_ff, block_size, n_heads, n_kv_heads) for _ in range(n_layers)]
         else:
             raise ValueError(variant)
         self.variant = variant
