@@ -21,7 +21,7 @@ enum { MODE_OUT = 0, MODE_STATE = 1, MODE_TANGENT = 2 };
 struct Jobs {
   Job job[3];
   int first[4];
-  int count;
+  Link link;
 };
 
 struct TangentArgs {
@@ -123,6 +123,7 @@ __global__ void __launch_bounds__(THREADS) walk_kernel(const __grid_constant__ J
   float* sG = sP + (MODE != MODE_STATE ? C * (C + 4) : 0);
   float* sD = sG + (MODE == MODE_TANGENT ? C * E : 0);  // (dxp, E): d state / d ln a
 
+  chain_begin(jobs.link);
   const float l2 = log2_decay(job.log_decay[h]);
   for (int e = threadIdx.x; e <= C; e += THREADS) sPow[e] = exp2f(l2 * float(e));
   const int64_t len = row_length(job.lengths, b, job.L);
@@ -134,7 +135,7 @@ __global__ void __launch_bounds__(THREADS) walk_kernel(const __grid_constant__ J
     const int r = i / E, c = i % E;
     float v = 0.f;
     if (start && r < dx && c < cw)
-      v = job.start_t ? start[int64_t(c0 + c) * dx + r] : start[int64_t(r) * dz + c0 + c];
+      v = __ldcg(job.start_t ? start + int64_t(c0 + c) * dx + r : start + int64_t(r) * dz + c0 + c);
     sS[i] = v;
     if (MODE == MODE_TANGENT) sD[i] = 0.f;
   }
@@ -320,7 +321,7 @@ __global__ void __launch_bounds__(THREADS) walk_kernel(const __grid_constant__ J
     if (tan.behind) {
       const float* x = tan.behind + (b * job.H + h) * tan.behind_stride + int64_t(seg) * dx * dz;
       for (int i = threadIdx.x; i < dx * cw; i += THREADS)
-        tend = fmaf(x[int64_t(i / cw) * dz + c0 + i % cw], sD[(i / cw) * E + i % cw], tend);
+        tend = fmaf(__ldcg(x + int64_t(i / cw) * dz + c0 + i % cw), sD[(i / cw) * E + i % cw], tend);
     }
     __shared__ float red[THREADS / 32];
     tsum = warp_sum(fmaf(tsum, tan.scale, tend));
@@ -332,6 +333,7 @@ __global__ void __launch_bounds__(THREADS) walk_kernel(const __grid_constant__ J
       tan.part[((int64_t(h) * job.B + b) * job.segs + seg) * slices + sl] = s;
     }
   }
+  chain_end();
 }
 
 // The pieces' own end states (B, H, segs, n) become the states that enter each piece: one thread per
@@ -346,9 +348,11 @@ struct EnterSet {
   const int32_t* lengths;
   int64_t L, seg_len, n;
   int H, segs, blocks;
+  Link link;
 };
 __global__ void __launch_bounds__(128) enter_kernel(const __grid_constant__ EnterSet a) {
   constexpr int U = 8;
+  chain_begin(a.link);
   const int w = blockIdx.y, rev = a.rev[w], segs = a.segs;
   const int64_t bh = blockIdx.x / a.blocks, b = bh / a.H, n = a.n;
   const float l2 = log2_decay(a.log_decay[bh % a.H]);
@@ -384,9 +388,11 @@ struct ShareSet {
   void* out[3];
   int64_t n[3];
   int heads[3], group[3], d[3];
+  Link link;
 };
 template <class T>
 __global__ void __launch_bounds__(256) share_sum_kernel(const __grid_constant__ ShareSet a) {
+  chain_begin(a.link);
   const int w = blockIdx.y, heads = a.heads[w], group = a.group[w], d = a.d[w];
   T* out = static_cast<T*>(a.out[w]);
   for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < a.n[w]; i += int64_t(gridDim.x) * 256) {
@@ -394,13 +400,15 @@ __global__ void __launch_bounds__(256) share_sum_kernel(const __grid_constant__ 
     const int64_t t = th / heads, hh = th % heads;
     const float* p = a.part[w] + (t * heads * group + hh * group) * d + i % d;
     float s = 0.f;
-    for (int r = 0; r < group; ++r) s += p[int64_t(r) * d];
+    for (int r = 0; r < group; ++r) s += __ldcg(p + int64_t(r) * d);
     st(out, i, s);
   }
 }
 
 // grad ln a of head h: its partials in order
-__global__ void __launch_bounds__(256) decay_sum_kernel(const float* part, float* out, int64_t n, int accumulate) {
+__global__ void __launch_bounds__(256) decay_sum_kernel(const float* part, float* out, int64_t n, int accumulate,
+                                                        const Link link) {
+  chain_begin(link);
   __shared__ float red[8];
   const float* p = part + int64_t(blockIdx.x) * n;
   float s = 0.f;
@@ -420,13 +428,13 @@ static int walk_as(const Jobs& jobs, int rows, const TangentArgs& tan, cudaStrea
   static int limit = 0;
   const size_t smem = smem_bytes((rows + 3) & ~3, MODE);
   PGF_CUDA(ensure_dynamic_smem(walk_kernel<T, C, MODE>, smem, limit));
-  walk_kernel<T, C, MODE><<<unsigned(jobs.first[3]), THREADS, smem, s>>>(jobs, tan);
+  PGF_CUDA(launch_link(jobs.link, walk_kernel<T, C, MODE>, unsigned(jobs.first[3]), THREADS, smem, s, jobs, tan));
   PGF_LAUNCH_CHECK();
   return PGF_OK;
 }
 
 template <int MODE>
-static int walk(const Job* job, int count, const TangentArgs& tan, int dtype, cudaStream_t s) {
+static int walk(const Job* job, int count, const TangentArgs& tan, const Link& link, int dtype, cudaStream_t s) {
   Jobs jobs = {};
   int64_t ctas = 0;
   int rows = 0;
@@ -439,7 +447,7 @@ static int walk(const Job* job, int count, const TangentArgs& tan, int dtype, cu
   }
   PGF_CHECK_ARG(ctas < 0x7fffffff, "decay_attn: too many pieces");
   jobs.first[3] = int(ctas);
-  jobs.count = count;
+  jobs.link = link;
   if (dtype == PGF_DTYPE_BF16)
     return rows > 128 ? walk_as<__nv_bfloat16, 32, MODE>(jobs, rows, tan, s)
                       : walk_as<__nv_bfloat16, 64, MODE>(jobs, rows, tan, s);
@@ -614,16 +622,16 @@ struct Entering {
   int64_t stride;
 };
 
-static int f_calls(const Job* job, int count, const Plan& pl, int dtype, cudaStream_t s) {
-  if (!pl.tc) return walk<MODE_OUT>(job, count, TangentArgs{}, dtype, s);
-  for (int k = 0; k < count; ++k) PGF_TRY(tc_walk(job[k], s));
+static int f_calls(const Job* job, int count, const Plan& pl, Chain& chain, int dtype, cudaStream_t s) {
+  if (!pl.tc) return walk<MODE_OUT>(job, count, TangentArgs{}, chain.next(), dtype, s);
+  for (int k = 0; k < count; ++k) PGF_TRY(tc_walk(job[k], chain.next(), s));
   return PGF_OK;
 }
 
 // What enters the pieces of one or two walks of the same shape that begin with `first`; `pieces` is scratch for
 // them.  last: where the state behind a cut walk goes, or NULL (an uncut one gives it by itself).
 static int entering(Job* job, int count, const Plan& pl, const float* const* first, float* const* pieces,
-                    float* const* last, Entering* e, int dtype, cudaStream_t s) {
+                    float* const* last, Entering* e, Chain& chain, int dtype, cudaStream_t s) {
   const int64_t n = int64_t(job[0].y.d) * job[0].z.d;
   const int segs = job[0].segs;
   for (int k = 0; k < count; ++k) e[k] = {first[k], n};
@@ -641,9 +649,9 @@ static int entering(Job* job, int count, const Plan& pl, const float* const* fir
     e[k] = {pieces[k], segs * n};
   }
   if (pl.tc) {
-    for (int k = 0; k < count; ++k) PGF_TRY(tc_pieces(job[k], s));
+    for (int k = 0; k < count; ++k) PGF_TRY(tc_pieces(job[k], chain.next(), s));
   } else {
-    PGF_TRY(walk<MODE_STATE>(job, count, TangentArgs{}, dtype, s));
+    PGF_TRY(walk<MODE_STATE>(job, count, TangentArgs{}, chain.next(), dtype, s));
   }
   set.log_decay = job[0].log_decay;
   set.lengths = job[0].lengths;
@@ -653,8 +661,12 @@ static int entering(Job* job, int count, const Plan& pl, const float* const* fir
   set.H = job[0].H;
   set.segs = segs;
   set.blocks = ceil_div(n, 128);
-  enter_kernel<<<dim3(unsigned(job[0].B * job[0].H * set.blocks), unsigned(count)), 128, 0, s>>>(set);
+  chain.wait = 1;
+  set.link = chain.next();
+  PGF_CUDA(launch_link(set.link, enter_kernel, dim3(unsigned(job[0].B * job[0].H * set.blocks), unsigned(count)), 128, 0, s,
+                       set));
   PGF_LAUNCH_CHECK();
+  chain.wait = 1;
   return PGF_OK;
 }
 
@@ -728,12 +740,13 @@ extern "C" int pgf_decay_attn_fwd(const void* q, const pgf_strides* q_strides, c
     }
   }
   da::Entering S;
+  da::Chain chain;
   da::Job js = job;
-  PGF_TRY(da::entering(&js, 1, pl, &state, &pieces, &state_out, &S, dtype, s));
+  PGF_TRY(da::entering(&js, 1, pl, &state, &pieces, &state_out, &S, chain, dtype, s));
   if (job.segs > 1) job.end = nullptr;
   job.start = S.p;
   job.start_stride = S.stride;
-  return da::f_calls(&job, 1, pl, dtype, s);
+  return da::f_calls(&job, 1, pl, chain, dtype, s);
 }
 
 extern "C" int pgf_decay_attn_bwd(const void* q, const pgf_strides* q_strides, const void* k,
@@ -780,6 +793,7 @@ extern "C" int pgf_decay_attn_bwd(const void* q, const pgf_strides* q_strides, c
   }
   // what enters the pieces from both ends; X carries the scale of g
   da::Entering ends[2];
+  da::Chain chain;
   {
     da::Job js[2] = {job, job};
     js[0].x = js[0].y = tk; js[0].z = tv;
@@ -789,7 +803,7 @@ extern "C" int pgf_decay_attn_bwd(const void* q, const pgf_strides* q_strides, c
     js[1].rev = 1;
     const float* first[2] = {state, g_state};
     float *pieces[2] = {sp, xp}, *last[2] = {nullptr, grad_state};
-    PGF_TRY(da::entering(js, 2, pl, first, pieces, last, ends, dtype, s));
+    PGF_TRY(da::entering(js, 2, pl, first, pieces, last, ends, chain, dtype, s));
   }
   const da::Entering S = ends[0], X = ends[1];
   const int f32 = dtype == PGF_DTYPE_F32;
@@ -814,7 +828,7 @@ extern "C" int pgf_decay_attn_bwd(const void* q, const pgf_strides* q_strides, c
   jk.z_scale = scale;
   jk.out = pk ? static_cast<void*>(pk) : grad_k;
   jk.out_f32 = f32 || pk;
-  PGF_TRY(da::f_calls(calls, 3, pl, dtype, s));
+  PGF_TRY(da::f_calls(calls, 3, pl, chain, dtype, s));
   if (grad_log_decay) {
     int parts;
     if (tc) {
@@ -828,7 +842,7 @@ extern "C" int pgf_decay_attn_bwd(const void* q, const pgf_strides* q_strides, c
       t.scale = scale;
       t.B = Bsz; t.L = L; t.seg_len = job.seg_len;
       t.H = int(H); t.segs = job.segs;
-      PGF_TRY(da::tc_tangent(t, s));
+      PGF_TRY(da::tc_tangent(t, chain.next(), s));
       parts = da::tc_tangent_blocks(Dk, Dv);
     } else {
       da::Job jt = job;
@@ -841,10 +855,13 @@ extern "C" int pgf_decay_attn_bwd(const void* q, const pgf_strides* q_strides, c
       t.behind_stride = X.stride;
       t.part = part;
       t.scale = scale;
-      PGF_TRY(da::walk<da::MODE_TANGENT>(&jt, 1, t, dtype, s));
+      PGF_TRY(da::walk<da::MODE_TANGENT>(&jt, 1, t, chain.next(), dtype, s));
       parts = ceil_div(Dv, da::E);
     }
-    da::decay_sum_kernel<<<unsigned(H), 256, 0, s>>>(part, grad_log_decay, Bsz * job.segs * parts, accumulate);
+    chain.wait = 1;
+    const da::Link sum = chain.next();
+    PGF_CUDA(da::launch_link(sum, da::decay_sum_kernel, unsigned(H), 256, 0, s, part, grad_log_decay,
+                             int64_t(Bsz * job.segs * parts), accumulate, sum));
     PGF_LAUNCH_CHECK();
   }
   if (L == 0) return PGF_OK;
@@ -866,8 +883,10 @@ extern "C" int pgf_decay_attn_bwd(const void* q, const pgf_strides* q_strides, c
   if (count) {
     int64_t ctas = (most + 255) / 256;
     if (ctas > 148 * 16) ctas = 148 * 16;
-    if (f32) da::share_sum_kernel<float><<<dim3(unsigned(ctas), unsigned(count)), 256, 0, s>>>(set);
-    else da::share_sum_kernel<__nv_bfloat16><<<dim3(unsigned(ctas), unsigned(count)), 256, 0, s>>>(set);
+    chain.wait = 1;
+    set.link = chain.next();
+    PGF_CUDA(da::launch_link(set.link, f32 ? da::share_sum_kernel<float> : da::share_sum_kernel<__nv_bfloat16>,
+                             dim3(unsigned(ctas), unsigned(count)), 256, 0, s, set));
     PGF_LAUNCH_CHECK();
   }
   return PGF_OK;

@@ -40,6 +40,7 @@ struct Params {
   int64_t stride, L, seg_len;
   float z_scale;
   int H, segs, dx, dz, last_too, gy, gz;
+  Link link;
 };
 
 template <int DX, int DZ, bool REV>
@@ -67,7 +68,11 @@ pieces_tc_kernel(const __grid_constant__ CUtensorMap tmY, const __grid_constant_
   const int64_t len = row_length(p.lengths, b, p.L);
   const int64_t s0 = min(len, int64_t(seg) * p.seg_len), s1 = min(len, s0 + p.seg_len);
   // the end state of the walk's last piece enters no other piece
-  if (!p.last_too && seg == (REV ? 0 : p.segs - 1)) return;
+  chain_begin(p.link);
+  if (!p.last_too && seg == (REV ? 0 : p.segs - 1)) {
+    chain_end();
+    return;
+  }
   const int chunks = int((s1 - s0 + C - 1) / C);
   auto first_token = [&](int c) { return s0 + int64_t(REV ? chunks - 1 - c : c) * C; };
   auto tokens = [&](int c) { return int(min(int64_t(C), s1 - first_token(c))); };
@@ -240,10 +245,11 @@ pieces_tc_kernel(const __grid_constant__ CUtensorMap tmY, const __grid_constant_
   __syncthreads();
   if (warp == 0)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(uint32_t(2 * DZ)));
+  chain_end();
 }
 
 template <int DX, int DZ, bool REV>
-int launch(const Job& j, cudaStream_t s) {
+int launch(const Job& j, const Link& link, cudaStream_t s) {
   static int limit = 0;
   using G = Cfg<DX, DZ>;
   CUtensorMap my, mz;
@@ -252,22 +258,23 @@ int launch(const Job& j, cudaStream_t s) {
     return PGF_ERR_CUDA;
   }
   const Params p = {j.log_decay, j.lengths, const_cast<float*>(j.start), j.start_stride, j.L, j.seg_len, j.z_scale, j.H,
-                    j.segs, j.y.d, j.z.d, j.last_too, j.H / j.y.heads, j.H / j.z.heads};
+                    j.segs, j.y.d, j.z.d, j.last_too, j.H / j.y.heads, j.H / j.z.heads,
+                    link};
   PGF_CUDA(ensure_dynamic_smem(pieces_tc_kernel<DX, DZ, REV>, G::BYTES, limit));
-  pieces_tc_kernel<DX, DZ, REV><<<unsigned(j.B * j.H * j.segs), THREADS, G::BYTES, s>>>(my, mz, p);
+  PGF_CUDA(launch_link(link, pieces_tc_kernel<DX, DZ, REV>, unsigned(j.B * j.H * j.segs), THREADS, G::BYTES, s, my, mz, p));
   PGF_LAUNCH_CHECK();
   return PGF_OK;
 }
 
 template <bool REV>
-int dispatch(const Job& j, cudaStream_t s) {
-  if (j.y.d <= 64) return j.z.d <= 64 ? launch<64, 64, REV>(j, s) : launch<64, 128, REV>(j, s);
-  return j.z.d <= 64 ? launch<128, 64, REV>(j, s) : launch<128, 128, REV>(j, s);
+int dispatch(const Job& j, const Link& l, cudaStream_t s) {
+  if (j.y.d <= 64) return j.z.d <= 64 ? launch<64, 64, REV>(j, l, s) : launch<64, 128, REV>(j, l, s);
+  return j.z.d <= 64 ? launch<128, 64, REV>(j, l, s) : launch<128, 128, REV>(j, l, s);
 }
 
 }  // namespace
 
-int tc_pieces(const Job& j, cudaStream_t s) { return j.rev ? dispatch<true>(j, s) : dispatch<false>(j, s); }
+int tc_pieces(const Job& j, const Link& l, cudaStream_t s) { return j.rev ? dispatch<true>(j, l, s) : dispatch<false>(j, l, s); }
 
 }  // namespace da
 

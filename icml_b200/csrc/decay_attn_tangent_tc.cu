@@ -50,6 +50,7 @@ struct Params {
   float scale;
   int64_t B, L, seg_len;
   int H, segs, dk, dv, gq, gk, gv, gg;
+  Link link;
 };
 
 __global__ void __launch_bounds__(THREADS, 1)
@@ -78,6 +79,7 @@ tangent_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   const int64_t s0 = min(len, int64_t(seg) * p.seg_len), s1 = min(len, s0 + p.seg_len);
   const int chunks = int((s1 - s0 + C - 1) / C);
 
+  chain_begin(p.link);
   const float l2 = log2_decay(p.log_decay[h]);
   if (threadIdx.x <= C) tab[threadIdx.x] = exp2f(l2 * float(threadIdx.x));
   if (threadIdx.x < 32) tab[132 + threadIdx.x] = exp2f(l2 * float(31 - threadIdx.x));
@@ -222,7 +224,7 @@ tangent_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
         const int cc = c0 + cg * 16 + k;
-        s[k] = st && sr < p.dk && cc < p.dv ? st[cc] : 0.f;
+        s[k] = st && sr < p.dk && cc < p.dv ? __ldcg(st + cc) : 0.f;
       }
     }
     float* xch = reinterpret_cast<float*>(base + XCH) + cg * 16 * 64 + (i & 63);
@@ -319,7 +321,7 @@ tangent_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
       for (int k = 0; k < 16; ++k) {
         const int cc = c0 + cg * 16 + k;
-        if (cc < p.dv) acc_end = fmaf(x[cc], s[k], acc_end);
+        if (cc < p.dv) acc_end = fmaf(__ldcg(x + cc), s[k], acc_end);
       }
     }
     const float sum = warp_sum(fmaf(acc, p.scale, acc_end));
@@ -334,11 +336,12 @@ tangent_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     for (int k = 0; k < 16; ++k) s += sums[k];
     p.part[((int64_t(h) * p.B + b) * p.segs + seg) * blocks + blk] = s;
   }
+  chain_end();
 }
 
 }  // namespace
 
-int tc_tangent(const TangentJob& j, cudaStream_t s) {
+int tc_tangent(const TangentJob& j, const Link& link, cudaStream_t s) {
   static int limit = 0;
   CUtensorMap mq, mk, mv, mg;
   if (!make_tensor_map(&mq, j.q, j.B, j.L) || !make_tensor_map(&mk, j.k, j.B, j.L) || !make_tensor_map(&mv, j.v, j.B, j.L) ||
@@ -362,13 +365,14 @@ int tc_tangent(const TangentJob& j, cudaStream_t s) {
   p.segs = j.segs;
   p.dk = j.q.d;
   p.dv = j.v.d;
+  p.link = link;
   p.gq = j.H / j.q.heads;
   p.gk = j.H / j.k.heads;
   p.gv = j.H / j.v.heads;
   p.gg = j.H / j.g.heads;
   PGF_CUDA(ensure_dynamic_smem(tangent_tc_kernel, BYTES, limit));
   const int64_t grid = j.B * j.H * j.segs * tc_tangent_blocks(j.q.d, j.v.d);
-  tangent_tc_kernel<<<unsigned(grid), THREADS, BYTES, s>>>(mq, mk, mv, mg, p);
+  PGF_CUDA(launch_link(link, tangent_tc_kernel, unsigned(grid), THREADS, BYTES, s, mq, mk, mv, mg, p));
   PGF_LAUNCH_CHECK();
   return PGF_OK;
 }

@@ -71,6 +71,7 @@ struct Params {
   int64_t L, seg_len;
   int H, segs, dx, dz, start_t, out_f32;
   int gx, gy, gz;              // operator heads per tensor head
+  Link link;
 };
 
 // Barriers behind full[NS] and empty[NS].  A and P take turns where there are two A buffers: X may be a chunk
@@ -433,13 +434,14 @@ struct Walk {
     const uint32_t row = uint32_t(q * 32) << 16;
     const int64_t n_state = int64_t(p.dx) * p.dz;
     float2 s[HC / 2];
+    chain_begin(p.link);    // only the state may come from the launches in front
     {
       const float* st = p.start ? p.start + bh * p.start_stride + int64_t(seg) * n_state : nullptr;
 #pragma unroll
       for (int k = 0; k < HC; ++k) {
         const int c = half * HC + k;
         const float v = st && i < p.dx && i < DX && c < p.dz
-                            ? (p.start_t ? st[int64_t(c) * p.dx + i] : st[int64_t(i) * p.dz + c]) : 0.f;
+                            ? __ldcg(p.start_t ? st + int64_t(c) * p.dx + i : st + int64_t(i) * p.dz + c) : 0.f;
         if (k & 1) s[k / 2].y = v;
         else s[k / 2].x = v;
       }
@@ -585,6 +587,7 @@ walk_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
   __syncthreads();
   if (w.warp == 0)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(w.tmem), "r"(TMEM_COLS));
+  chain_end();
 }
 
 bool fits(const Tensor& t, int64_t B, int64_t L) {
@@ -606,7 +609,7 @@ bool make_store_map(CUtensorMap* m, const Job& j, int cols) {
 }
 
 template <int DX, int DZ, int NT, bool REV>
-int launch(const Job& j, cudaStream_t s) {
+int launch(const Job& j, const Link& link, cudaStream_t s) {
   static int limit = 0;
   using G = Cfg<DX, DZ, NT>;
   CUtensorMap mx, my, mz, mo = {};
@@ -632,27 +635,29 @@ int launch(const Job& j, cudaStream_t s) {
   p.dz = j.z.d;
   p.start_t = j.start_t;
   p.out_f32 = j.out_f32;
+  p.link = link;
   p.gx = j.H / j.x.heads;
   p.gy = j.H / j.y.heads;
   p.gz = j.H / j.z.heads;
   PGF_CUDA(ensure_dynamic_smem(walk_tc_kernel<DX, DZ, NT, REV>, G::BYTES, limit));
-  walk_tc_kernel<DX, DZ, NT, REV><<<unsigned(j.B * j.H * j.segs), THREADS, G::BYTES, s>>>(mx, my, mz, mo, p);
+  PGF_CUDA(launch_link(link, walk_tc_kernel<DX, DZ, NT, REV>, unsigned(j.B * j.H * j.segs), THREADS, G::BYTES, s, mx, my, mz,
+                       mo, p));
   PGF_LAUNCH_CHECK();
   return PGF_OK;
 }
 
 template <int NT, bool REV>
-int dispatch(const Job& j, cudaStream_t s) {
-  if (j.y.d <= 64) return j.z.d <= 64 ? launch<64, 64, NT, REV>(j, s) : launch<64, 128, NT, REV>(j, s);
-  return j.z.d <= 64 ? launch<128, 64, NT, REV>(j, s) : launch<128, 128, NT, REV>(j, s);
+int dispatch(const Job& j, const Link& l, cudaStream_t s) {
+  if (j.y.d <= 64) return j.z.d <= 64 ? launch<64, 64, NT, REV>(j, l, s) : launch<64, 128, NT, REV>(j, l, s);
+  return j.z.d <= 64 ? launch<128, 64, NT, REV>(j, l, s) : launch<128, 128, NT, REV>(j, l, s);
 }
 
 }  // namespace
 
 bool tc_fits(const Tensor& t, int64_t B, int64_t L) { return fits(t, B, L); }
-int tc_walk(const Job& j, cudaStream_t s) {
-  if (j.end) return j.rev ? dispatch<3, true>(j, s) : dispatch<3, false>(j, s);
-  return j.rev ? dispatch<2, true>(j, s) : dispatch<2, false>(j, s);
+int tc_walk(const Job& j, const Link& l, cudaStream_t s) {
+  if (j.end) return j.rev ? dispatch<3, true>(j, l, s) : dispatch<3, false>(j, l, s);
+  return j.rev ? dispatch<2, true>(j, l, s) : dispatch<2, false>(j, l, s);
 }
 
 }  // namespace da

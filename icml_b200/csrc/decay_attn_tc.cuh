@@ -14,9 +14,9 @@ constexpr uint32_t BLK = 16384;   // a tile of 128 rows x 64 bf16 columns, 128B 
 // most 128 wide.
 bool tc_fits(const Tensor& t, int64_t B, int64_t L);
 // One F call.  job.seg_len: a multiple of TC_CHUNK.
-int tc_walk(const Job& job, cudaStream_t s);
+int tc_walk(const Job& job, const Link& link, cudaStream_t s);
 // The pieces' own end states from zero, into job.start.
-int tc_pieces(const Job& job, cudaStream_t s);
+int tc_pieces(const Job& job, const Link& link, cudaStream_t s);
 
 // grad ln a: partial sums (H, B, segs, blocks), blocks = tc_tangent_blocks(Dk, Dv).  start: the state that enters
 // each piece, behind: the adjoint (scaled) of the state behind it; NULL: zeros.
@@ -32,7 +32,7 @@ struct TangentJob {
   int H, segs;
 };
 static inline int tc_tangent_blocks(int64_t dk, int64_t dv) { return ceil_div(dk, 64) * ceil_div(dv, 64); }
-int tc_tangent(const TangentJob& job, cudaStream_t s);
+int tc_tangent(const TangentJob& job, const Link& link, cudaStream_t s);
 
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2, int c3) {
   asm volatile(

@@ -274,3 +274,42 @@ def test_beam_select_over_large_vocabularies(V, dtype):
     assert torch.allclose(so, want[:, :3], rtol=3e-7, atol=2e-6)
     flat = (rows - 3 * torch.arange(2, device=DEV)[:, None]) * V + tokens
     assert torch.allclose(so, c.gather(1, flat), rtol=3e-7, atol=2e-6)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,L,H,Hk", [(1, 4000, 2, 1), (3, 300, 60, 60)])  # cut into pieces; more heads than SMs
+def test_calls_in_a_graph_and_back_to_back(B, L, H, Hk, dtype):
+    """The launches of a call overlap one another but neither the calls before nor those behind: replays and
+    calls in close order, each with the inputs overwritten in between, give the bits of calls on their own."""
+    from icml_b200 import ops
+    torch.manual_seed(L)
+    sets = [[torch.randn(B, L, h, 64, device=DEV).to(dtype) for h in (H, Hk, Hk, H)] for _ in range(4)]
+    ld = -torch.rand(H, device=DEV) * 0.1 - 1e-3
+
+    def call(q, k, v, g):
+        out, end = ops.decay_attn_fwd(q, k, v, ld)
+        r = ops.decay_attn_bwd(q, k, v, ld, g, need_g_log_decay=True)
+        return [out, end, *[r[n] for n in sorted(r)]]
+
+    alone = []
+    for s in sets:
+        torch.cuda.synchronize()
+        alone.append(call(*s))
+        torch.cuda.synchronize()
+    buf = [t.clone() for t in sets[0]]
+    close = []
+    for s in sets * 3:
+        for d, t in zip(buf, s):
+            d.copy_(t)
+        close.append([t.clone() for t in call(*buf)])
+    for i, got in enumerate(close):
+        assert all(torch.equal(a, b) for a, b in zip(got, alone[i % 4])), i
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = call(*buf)
+    for i in (2, 0, 3):
+        for d, t in zip(buf, sets[i]):
+            d.copy_(t)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(got, alone[i])), f"replay {i}"
+    graph.reset()
