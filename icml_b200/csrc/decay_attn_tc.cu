@@ -47,9 +47,9 @@ struct Cfg {
   static constexpr uint32_t XB = DX / 64 * BLK, ZB = DZ / 64 * BLK;
   static constexpr uint32_t SLOT = XB > ZB ? XB : ZB;
   static constexpr int NS = SLOT == BLK ? 8 : NT == 2 ? 5 : 4;
-  static constexpr int NA = NS == 8 ? 2 : 1;                            // A buffers
+  static constexpr int NA = NS == 8 ? 2 : 1;                            // buffers of A, of U and of y's smaller terms
   static constexpr uint32_t RING = NS * SLOT;
-  static constexpr uint32_t MID = RING, LO = MID + XB, ZERO = LO + XB;  // ZERO only with 64-wide y
+  static constexpr uint32_t MID = RING, LO = MID + NA * XB, ZERO = LO + NA * XB;  // ZERO only with 64-wide y
   static constexpr uint32_t ST = NT == 2 ? LO : DX == 64 ? ZERO + BLK : ZERO;  // S: 128 rows x DZ bf16
   static constexpr uint32_t WTAB = ST + ZB;                             // 130 x 8 bytes
   static constexpr uint32_t TAB = WTAB + 1040;                          // 132 + 32 floats
@@ -57,7 +57,7 @@ struct Cfg {
   static constexpr uint32_t BYTES = BARS + 256 + 1024;
   // TMEM columns
   static constexpr uint32_t T_A = 0, T_D1 = NA * 128, T_D2 = T_D1 + DZ, T_U = T_D2 + DZ;
-  static_assert(T_U + DZ <= TMEM_COLS && BYTES <= 232448, "fits an SM");
+  static_assert(T_U + NA * DZ <= TMEM_COLS && BYTES <= 232448, "fits an SM");
 };
 
 struct Params {
@@ -76,7 +76,7 @@ struct Params {
 
 // Barriers behind full[NS] and empty[NS].  A and P take turns where there are two A buffers: X may be a chunk
 // ahead of the product that reads P.
-enum { B_A = 0, B_A1, B_P, B_P1, B_O, B_DFREE, B_K, B_U, B_S, B_OSTAGED, B_SUM, B_DONE, B_COUNT };
+enum { B_A = 0, B_A1, B_P, B_P1, B_K, B_K1, B_U, B_U1, B_O, B_DFREE, B_S, B_OSTAGED, B_SUM, B_DONE, B_COUNT };
 
 template <int DX, int DZ, int NT, bool REV>
 struct Walk {
@@ -151,7 +151,7 @@ struct Walk {
     const uint32_t id_d = (1u << 4) | (1u << 7) | (1u << 10) | (1u << 16) | (uint32_t(DZ >> 3) << 17) |
                           (uint32_t(C >> 4) << 24);
     const uint32_t id_u = id_d | (1u << 15);
-    const Desc d_lo(sbase + G::LO, BLK), d_mid(sbase + G::MID, BLK), d_s(sbase + G::ST, BLK);
+    const Desc d_s(sbase + G::ST, BLK);
     auto at = [&](uint32_t n) { return sbase + slot(n) * G::SLOT; };
     auto product_a = [&](int c) {
       if (!wait_full(tile_y(c)) || !wait_full(tile_x(c))) return false;
@@ -172,26 +172,27 @@ struct Walk {
     for (int c = 0; c < chunks; ++c) {
       const bool more = c + 1 < chunks;
       if (G::NA == 2 && more && !product_a(c + 1)) return;
-      if (!wait_full(tile_z(c)) || !wait(B_K, c)) return;
+      if (!wait_full(tile_z(c)) || !wait_turn(B_K, c)) return;
       tc_after();
       const Desc dz(at(tile_z(c)), BLK);
       if (leader) {
         // small terms first, so that the accumulator drops the least
         const uint32_t yb = at(tile_y(c));
-        const Desc dy(yb, DX == 64 ? sbase + G::MID - yb : BLK);
+        const uint32_t mid = sbase + G::MID + uint32_t(c % G::NA) * G::XB, lo = sbase + G::LO + uint32_t(c % G::NA) * G::XB;
+        const Desc dy(yb, DX == 64 ? mid - yb : BLK), d_mid(mid, BLK), d_lo(lo, DX == 64 ? sbase + G::ZERO - lo : BLK);
         if (NT == 3) {
 #pragma unroll
-          for (int kk = 0; kk < 8; ++kk) umma_bf16(tmem + G::T_U, d_lo.at(kk * 2048), dz.at(kk * 2048), id_u, kk > 0);
+          for (int kk = 0; kk < 8; ++kk) umma_bf16(tmem + G::T_U + uint32_t(c % G::NA) * DZ, d_lo.at(kk * 2048), dz.at(kk * 2048), id_u, kk > 0);
         }
         if (DX == 128) {
 #pragma unroll
           for (int kk = 0; kk < 8; ++kk)
-            umma_bf16(tmem + G::T_U, d_mid.at(kk * 2048), dz.at(kk * 2048), id_u, NT == 3 || kk > 0);
+            umma_bf16(tmem + G::T_U + uint32_t(c % G::NA) * DZ, d_mid.at(kk * 2048), dz.at(kk * 2048), id_u, NT == 3 || kk > 0);
         }
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
-          umma_bf16(tmem + G::T_U, dy.at(kk * 2048), dz.at(kk * 2048), id_u, NT == 3 || DX == 128 || kk > 0);
-        umma_commit(&bars[B_U]);
+          umma_bf16(tmem + G::T_U + uint32_t(c % G::NA) * DZ, dy.at(kk * 2048), dz.at(kk * 2048), id_u, NT == 3 || DX == 128 || kk > 0);
+        umma_commit(&bars[B_U + c % G::NA]);
         umma_commit(&empty[slot(tile_y(c))]);
       }
       __syncwarp();
@@ -370,7 +371,7 @@ struct Walk {
   __device__ __forceinline__ bool weigh(int c, int tid) const {
     const uint32_t ny = tile_y(c), nz = tile_z(c);
     const int n = tokens(c);
-    const uint32_t yb = sbase + slot(ny) * G::SLOT;
+    const uint32_t yb = sbase + slot(ny) * G::SLOT, buf = sbase + uint32_t(c % G::NA) * G::XB;
     if (!wait_turn(B_A, c)) return false;
     constexpr int PIECES = DX / 64 * 1024 / CONV, BATCH = PIECES < 4 ? PIECES : 4;
 #pragma unroll
@@ -412,8 +413,8 @@ struct Walk {
           }
         }
         sts128(yb + off, hi);
-        sts128(sbase + G::MID + off, mid);
-        if (NT == 3) sts128(sbase + G::LO + off, lo);
+        sts128(buf + G::MID + off, mid);
+        if (NT == 3) sts128(buf + G::LO + off, lo);
       }
     }
     if (n < C) {
@@ -423,7 +424,7 @@ struct Walk {
         if ((int(u >> 3) & 127) >= n) sts128(sbase + slot(nz) * G::SLOT + u * 16, zero);
     }
     fence_async();
-    arrive(B_K);
+    arrive(B_K + c % G::NA);
     return true;
   }
 
@@ -446,8 +447,9 @@ struct Walk {
         else s[k / 2].x = v;
       }
     }
+    if (G::NA == 2 && chunks > 0 && !weigh(0, tid)) return;
     for (int c = 0; c < chunks; ++c) {
-      if (!weigh(c, tid)) return;
+      if (G::NA == 1 && !weigh(c, tid)) return;
       {
         // S as the bf16 operand of D1, once D1 of the chunk before has read its own
         if (c > 0 && !wait(B_O, c - 1)) return;
@@ -460,14 +462,16 @@ struct Walk {
         fence_async();
         arrive(B_S);
       }
-      if (!wait(B_U, c)) return;
+      // with two buffers y of the next chunk is weighed while this one's U is formed
+      if (G::NA == 2 && c + 1 < chunks && !weigh(c + 1, tid)) return;
+      if (!wait_turn(B_U, c)) return;
       tc_after();
       const float an = pw(tokens(c));
       const float2 an2 = make_float2(an, an), zs = make_float2(p.z_scale, p.z_scale);
 #pragma unroll
       for (int g = 0; g < HC / 16; ++g) {
         uint32_t u[16];
-        tmem_ld16_nowait(tmem + G::T_U + row + half * HC + g * 16, u);
+        tmem_ld16_nowait(tmem + G::T_U + uint32_t(c % G::NA) * DZ + row + half * HC + g * 16, u);
         tmem_wait_ld();
 #pragma unroll
         for (int k = 0; k < 8; ++k)
@@ -540,7 +544,7 @@ walk_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
   if (threadIdx.x < 32) tab[132 + threadIdx.x] = exp2f(l2 * float(REV ? threadIdx.x : 31 - threadIdx.x));
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2 * G::NS; ++s) mbar_init(&full[s], 1);
-    for (int k = 0; k < B_COUNT; ++k) mbar_init(&bars[k], k == B_A || k == B_A1 || k == B_O || k == B_U || k == B_DONE ? 1 : k == B_K ? W::CONV / 32 : 8);
+    for (int k = 0; k < B_COUNT; ++k) mbar_init(&bars[k], k <= B_A1 || k == B_U || k == B_U1 || k == B_O || k == B_DONE ? 1 : 8);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmX)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmY)) : "memory");
