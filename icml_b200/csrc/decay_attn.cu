@@ -740,7 +740,7 @@ extern "C" int pgf_decay_attn_fwd(const void* q, const pgf_strides* q_strides, c
     }
   }
   da::Entering S;
-  da::Chain chain;
+  Chain chain;
   da::Job js = job;
   PGF_TRY(da::entering(&js, 1, pl, &state, &pieces, &state_out, &S, chain, dtype, s));
   if (job.segs > 1) job.end = nullptr;
@@ -793,7 +793,7 @@ extern "C" int pgf_decay_attn_bwd(const void* q, const pgf_strides* q_strides, c
   }
   // what enters the pieces from both ends; X carries the scale of g
   da::Entering ends[2];
-  da::Chain chain;
+  Chain chain;
   {
     da::Job js[2] = {job, job};
     js[0].x = js[0].y = tk; js[0].z = tv;
@@ -859,8 +859,8 @@ extern "C" int pgf_decay_attn_bwd(const void* q, const pgf_strides* q_strides, c
       parts = ceil_div(Dv, da::E);
     }
     chain.wait = 1;
-    const da::Link sum = chain.next();
-    PGF_CUDA(da::launch_link(sum, da::decay_sum_kernel, unsigned(H), 256, 0, s, part, grad_log_decay,
+    const Link sum = chain.next();
+    PGF_CUDA(launch_link(sum, da::decay_sum_kernel, unsigned(H), 256, 0, s, part, grad_log_decay,
                              int64_t(Bsz * job.segs * parts), accumulate, sum));
     PGF_LAUNCH_CHECK();
   }
@@ -885,7 +885,7 @@ extern "C" int pgf_decay_attn_bwd(const void* q, const pgf_strides* q_strides, c
     if (ctas > 148 * 16) ctas = 148 * 16;
     chain.wait = 1;
     set.link = chain.next();
-    PGF_CUDA(da::launch_link(set.link, f32 ? da::share_sum_kernel<float> : da::share_sum_kernel<__nv_bfloat16>,
+    PGF_CUDA(launch_link(set.link, f32 ? da::share_sum_kernel<float> : da::share_sum_kernel<__nv_bfloat16>,
                              dim3(unsigned(ctas), unsigned(count)), 256, 0, s, set));
     PGF_LAUNCH_CHECK();
   }

@@ -17,7 +17,7 @@
 //   grad k = F(v, g, q; X^T)          from the end
 // with g the output's gradient.  X' before the first token is the initial state's gradient.
 #pragma once
-#include "common.cuh"
+#include "chain.cuh"
 
 namespace pgf {
 namespace da {
@@ -52,46 +52,6 @@ struct Job {
   int64_t seg_len;           // tokens of a piece, a multiple of the engine's chunk
   int last_too;              // pieces' own end states: the walk's last piece as well
 };
-
-// The launches of one call.  The first waits for what is in front of it in the stream, as any launch.  A later one
-// (chained) may start as soon as all CTAs of the one before have begun, so that it fills the SMs which that one's
-// last wave leaves idle (programmatic dependent launch).  What it must not read too early it waits for (wait: the
-// launch before has ended); and one CTA of each waits for it at its own end, so that the end of the last launch
-// is the end of all.  What a launch reads that one further in front has written it reads past the L1 cache.
-struct Link {
-  int chained, wait;
-};
-struct Chain {
-  int n = 0, wait = 0;     // wait: the next launch reads what the one before writes
-  Link next() {
-    const Link l = {n++ > 0, wait};
-    wait = 0;
-    return l;
-  }
-};
-__device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void chain_begin(const Link& l) {
-  if (l.wait) chain_wait();
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-__device__ __forceinline__ void chain_end() {
-  if (blockIdx.x == gridDim.x - 1 && threadIdx.x == 0) chain_wait();
-}
-template <class... P, class... A>
-cudaError_t launch_link(const Link& l, void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t s,
-                        const A&... args) {
-  cudaLaunchAttribute at = {};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cfg.attrs = &at;
-  cfg.numAttrs = l.chained ? 1 : 0;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
 
 // a^e for the exponents of one head.  log2(a) is clamped so that e = 0 gives 1 for a decay of zero.
 __device__ __forceinline__ float log2_decay(float log_decay) {

@@ -20,6 +20,7 @@
 // rotation needs no exchange between lanes and the row sums are a few shuffles.  The backward's CTAs
 // walk the tiles in a fixed order and leave one partial of grad w each, added in CTA order by a second
 // kernel: no atomics, the same bits on every run.
+#include "chain.cuh"
 #include "f32x2.cuh"
 
 namespace pgf {
@@ -163,6 +164,7 @@ __global__ void __launch_bounds__(THREADS, 2) rotate_kernel(const Args a, int G)
   constexpr int PIECES = PER * U;              // and of an item
   constexpr int STAGES = RING / (PIECES * THREADS * 16);
   extern __shared__ __align__(16) uint8_t smem[];
+  if (BWD) chain_begin(Link{0, 0});
   const int z = int(blockIdx.x) >= a.ctas[0];
   const int cta = int(blockIdx.x) - (z ? a.ctas[0] : 0);
   const int D = a.D, np = D / 2, tw = a.tw[z], H = a.H[z];
@@ -381,6 +383,7 @@ template <class T, bool BWD>
 __global__ void __launch_bounds__(THREADS) rotate_any_kernel(const Args a, bool halves) {
   constexpr int UPL = MAX_D / 32;  // units per lane: a unit is a rotated pair or a single element behind R
   __shared__ float sacc[MAX_D];
+  if (BWD) chain_begin(Link{0, 0});
   const int z = int(blockIdx.x) >= a.ctas[0];
   const int cta = int(blockIdx.x) - (z ? a.ctas[0] : 0);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = THREADS / 32;
@@ -470,8 +473,9 @@ __global__ void __launch_bounds__(THREADS) rotate_any_kernel(const Args a, bool 
 // grad w of the queries (blockIdx.y 0) and keys: the CTAs' partials in CTA order, 32 warps' strided sums joined
 // in warp order.
 __global__ void __launch_bounds__(1024) weight_reduce_kernel(const float* part, int n_q, int n_k, int D, float* gq,
-                                                             float* gk, int accumulate) {
+                                                             float* gk, int accumulate, const Link link) {
   __shared__ float red[32][33];
+  chain_begin(link);
   float* out = blockIdx.y ? gk : gq;
   if (!out) return;
   const float* p = part + (blockIdx.y ? int64_t(n_q) * D : 0);
@@ -624,8 +628,9 @@ extern "C" int pgf_qk_norm_rotate_bwd(const void* q, const pgf_strides* q_stride
       PGF_TRY((qkr::launch<float, true>(a, pairs == PGF_PAIRS_HALVES, s)));
   }
   if (!grad_wq && !grad_wk) return PGF_OK;
-  qkr::weight_reduce_kernel<<<dim3(unsigned(ceil_div(D, 32)), 2), 1024, 0, s>>>(a.part, a.ctas[0], a.ctas[1], int(D), grad_wq, grad_wk,
-                                                                               accumulate);
+  const Link link = {1, 1};
+  PGF_CUDA(launch_link(link, qkr::weight_reduce_kernel, dim3(unsigned(ceil_div(D, 32)), 2), 1024, 0, s, a.part, a.ctas[0],
+                       a.ctas[1], int(D), grad_wq, grad_wk, accumulate, link));
   PGF_LAUNCH_CHECK();
   return PGF_OK;
 }
