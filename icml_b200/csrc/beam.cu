@@ -382,9 +382,12 @@ static bool wide_clusters() {
   static const bool ok = [] {
     for (auto* k : {select_kernel<T, 16, true>, select_kernel<T, 16, false>})
       if (cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return false;
+    if (cudaFuncSetAttribute(select_kernel<T, 16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, HELD_MOST) != cudaSuccess)
+      return false;
     cudaLaunchConfig_t c = {};
     c.gridDim = dim3(16);
     c.blockDim = dim3(THREADS);
+    c.dynamicSmemBytes = HELD_MOST;   // also when each CTA fills an SM
     cudaLaunchAttribute at;
     at.id = cudaLaunchAttributeClusterDimension;
     at.val.clusterDim.x = 16;
