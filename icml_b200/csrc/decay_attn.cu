@@ -726,7 +726,7 @@ extern "C" int pgf_decay_attn_fwd(const void* q, const pgf_strides* q_strides, c
   job.z_scale = 1.f;
   job.B = Bsz; job.L = L; job.H = int(H);
   const bool tc = dtype == PGF_DTYPE_BF16 && L > 0 && da::tc_fits(job.x, Bsz, L) && da::tc_fits(job.y, Bsz, L) &&
-                  da::tc_fits(job.z, Bsz, L) && aligned(out, 16);
+                  da::tc_fits(job.z, Bsz, L) && aligned(out, 16) && aligned(state, 16) && aligned(state_out, 16);
   const da::Plan pl = da::plan(p, tc, false);
   job.segs = pl.c.segs;
   job.seg_len = pl.c.seg_len;
@@ -769,7 +769,7 @@ extern "C" int pgf_decay_attn_bwd(const void* q, const pgf_strides* q_strides, c
                    tv = da::tensor(v, v_strides, L, Hv, Dv), tg = da::tensor(g, g_strides, L, H, Dv);
   const bool tc = dtype == PGF_DTYPE_BF16 && L > 0 && da::tc_fits(tq, Bsz, L) && da::tc_fits(tk, Bsz, L) &&
                   da::tc_fits(tv, Bsz, L) && da::tc_fits(tg, Bsz, L) && aligned(grad_q, 16) && aligned(grad_k, 16) &&
-                  aligned(grad_v, 16);
+                  aligned(grad_v, 16) && aligned(state, 16) && aligned(g_state, 16) && aligned(grad_state, 16);
   const da::Plan pl = da::plan(p, tc, true);
   da::Job job = {};
   job.log_decay = log_decay;

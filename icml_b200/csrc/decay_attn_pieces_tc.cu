@@ -30,7 +30,7 @@ struct Cfg {
   static constexpr uint32_t TAB = TERMS + 2 * BUF;
   static constexpr uint32_t BARS = TAB + 528;
   static constexpr uint32_t BYTES = BARS + 256 + 1024;
-  static_assert(BYTES <= 232448 && 64 * DZ * 4 <= TERMS, "fits an SM");
+  static_assert(BYTES <= 232448 && 128 * DZ * 4 <= TERMS, "fits an SM");
 };
 
 struct Params {
@@ -232,14 +232,10 @@ pieces_tc_kernel(const __grid_constant__ CUtensorMap tmY, const __grid_constant_
         for (int k = 0; k < HC / 2; ++k) s[k] = add2(s[k], sum[i + (cg * (HC / 2) + k) * 64]);
       }
     }
-    if (ok && i < DX && i < p.dx) {
-#pragma unroll
-      for (int k = 0; k < HC; k += 4) {
-        const int c = cg * HC + k;
-        if (c < p.dz)
-          *reinterpret_cast<float4*>(end + int64_t(i) * p.dz + c) = make_float4(s[k / 2].x, s[k / 2].y, s[k / 2 + 1].x, s[k / 2 + 1].y);
-      }
-    }
+    const int r0 = q * 32, c0 = cg * HC;
+    if (ok && r0 < DX)      // through the tiles' places, 64-wide: behind the sum
+      state_store<HC>(s, sbase + (DX == 64 ? 64 * DZ * 4 : 0) + uint32_t(q * 4 + cg) * HC * 128,
+                      end + int64_t(r0) * p.dz + c0, p.dz, p.dx - r0, p.dz - c0);
   }
   tc_before();
   __syncthreads();

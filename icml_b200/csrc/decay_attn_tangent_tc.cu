@@ -222,9 +222,13 @@ tangent_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     {
       const float* st = p.start && !tangent ? p.start + bh * p.start_stride + int64_t(seg) * n_state + int64_t(sr) * p.dv : nullptr;
 #pragma unroll
-      for (int k = 0; k < 16; ++k) {
+      for (int k = 0; k < 16; k += 4) {
         const int cc = c0 + cg * 16 + k;
-        s[k] = st && sr < p.dk && cc < p.dv ? __ldcg(st + cc) : 0.f;
+        const float4 v = st && sr < p.dk && cc < p.dv ? __ldcg(reinterpret_cast<const float4*>(st + cc)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        s[k] = v.x;
+        s[k + 1] = v.y;
+        s[k + 2] = v.z;
+        s[k + 3] = v.w;
       }
     }
     float* xch = reinterpret_cast<float*>(base + XCH) + cg * 16 * 64 + (i & 63);
@@ -319,9 +323,11 @@ tangent_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     if (tangent && p.behind && sr < p.dk) {
       const float* x = p.behind + bh * p.behind_stride + int64_t(seg) * n_state + int64_t(sr) * p.dv;
 #pragma unroll
-      for (int k = 0; k < 16; ++k) {
+      for (int k = 0; k < 16; k += 4) {
         const int cc = c0 + cg * 16 + k;
-        if (cc < p.dv) acc_end = fmaf(__ldcg(x + cc), s[k], acc_end);
+        if (cc >= p.dv) continue;
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(x + cc));
+        acc_end = fmaf(v.x, s[k], fmaf(v.y, s[k + 1], fmaf(v.z, s[k + 2], fmaf(v.w, s[k + 3], acc_end))));
       }
     }
     const float sum = warp_sum(fmaf(acc, p.scale, acc_end));

@@ -436,17 +436,23 @@ struct Walk {
     const int64_t n_state = int64_t(p.dx) * p.dz;
     float2 s[HC / 2];
     chain_begin(p.link);    // only the state may come from the launches in front
-    {
-      const float* st = p.start ? p.start + bh * p.start_stride + int64_t(seg) * n_state : nullptr;
+    const float* st = p.start ? p.start + bh * p.start_stride + int64_t(seg) * n_state : nullptr;
+    if (st && !p.start_t && q * 32 < DX) {
+      // through where the terms of y and S will be
+      static_assert(G::MID + DX * DZ * 4 <= (DX == 64 && NT == 3 ? G::ZERO : G::ST + G::ZB), "the states fit");
+      const int r0 = q * 32, c0 = half * HC;
+      state_load<HC>(s, sbase + G::MID + uint32_t(q * 2 + half) * HC * 128, st + int64_t(r0) * p.dz + c0, p.dz,
+                     p.dx - r0, p.dz - c0);
+    } else {
 #pragma unroll
       for (int k = 0; k < HC; ++k) {
         const int c = half * HC + k;
-        const float v = st && i < p.dx && i < DX && c < p.dz
-                            ? __ldcg(p.start_t ? st + int64_t(c) * p.dx + i : st + int64_t(i) * p.dz + c) : 0.f;
+        const float v = st && i < p.dx && i < DX && c < p.dz ? __ldcg(st + int64_t(c) * p.dx + i) : 0.f;
         if (k & 1) s[k / 2].y = v;
         else s[k / 2].x = v;
       }
     }
+    asm volatile("bar.sync 1, 256;" ::: "memory");   // all Y: the states have left where y's terms go
     if (G::NA == 2 && chunks > 0 && !weigh(0, tid)) return;
     for (int c = 0; c < chunks; ++c) {
       if (G::NA == 1 && !weigh(c, tid)) return;
@@ -498,13 +504,12 @@ struct Walk {
         for (int k = 0; k < HC / 2; ++k) s[k] = __fadd2_rn(s[k], sum[i + (half * (HC / 2) + k) * 64]);
       }
     }
-    if (i < DX && i < p.dx) {
-#pragma unroll
-      for (int k = 0; k < HC; k += 4) {
-        const int c = half * HC + k;
-        if (c < p.dz)
-          *reinterpret_cast<float4*>(end + int64_t(i) * p.dz + c) = make_float4(s[k / 2].x, s[k / 2].y, s[k / 2 + 1].x, s[k / 2 + 1].y);
-      }
+    const int r0 = q * 32, c0 = half * HC;
+    if (r0 < DX) {
+      // (all products that read y's terms are done; 64-wide: behind the sum)
+      static_assert(NT == 2 || (DX == 64 ? G::LO : G::MID) + DX * DZ * 4 <= G::ST, "the states fit");
+      state_store<HC>(s, sbase + (DX == 64 ? G::LO : G::MID) + uint32_t(q * 2 + half) * HC * 128,
+                      end + int64_t(r0) * p.dz + c0, p.dz, p.dx - r0, p.dz - c0);
     }
   }
 };

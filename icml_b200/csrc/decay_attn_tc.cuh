@@ -106,6 +106,63 @@ __device__ __forceinline__ void products_done(uint64_t* done, bool leader) {
   __syncwarp();
   warp_wait(done, 0);
 }
+// A warp's 32 rows x HC columns of a float32 state, a row per lane, from and to global memory in whole lines: the
+// 16-byte pieces cross from lane to lane in 32 HC floats of shared memory of the warp's own, permuted so that
+// neither side meets a bank twice.  (A lane that read its own row alone cost 12 us a CTA at 128 x 128: every
+// request touched 32 lines.)  ld: a multiple of 4; rows and cols (a multiple of 4) that are not there are zeros.
+template <int HC>
+__device__ __forceinline__ uint32_t state_at(int row, int ch) {
+  constexpr int CH = HC / 4;
+  static_assert(CH == 4 || CH == 8 || CH == 16, "columns of a warp");
+  return uint32_t(row * CH + (ch ^ (CH == 4 ? (row >> 1) & 3 : row & (CH - 1)))) * 16;
+}
+template <int HC>
+__device__ __forceinline__ void state_load(float2 (&s)[HC / 2], uint32_t tile, const float* g, int64_t ld, int rows, int cols) {
+  constexpr int CH = HC / 4, BATCH = CH < 8 ? CH : 8;
+  const int lane = threadIdx.x & 31, ch = lane % CH;
+#pragma unroll
+  for (int t0 = 0; t0 < CH; t0 += BATCH) {
+    float4 v[BATCH];
+#pragma unroll
+    for (int t = 0; t < BATCH; ++t) {
+      const int row = (t0 + t) * (32 / CH) + lane / CH;
+      v[t] = row < rows && ch * 4 < cols ? __ldcg(reinterpret_cast<const float4*>(g + row * ld + ch * 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+#pragma unroll
+    for (int t = 0; t < BATCH; ++t) {
+      const uint32_t w[4] = {__float_as_uint(v[t].x), __float_as_uint(v[t].y), __float_as_uint(v[t].z), __float_as_uint(v[t].w)};
+      sts128(tile + state_at<HC>((t0 + t) * (32 / CH) + lane / CH, ch), w);
+    }
+  }
+  __syncwarp();
+#pragma unroll
+  for (int k = 0; k < CH; ++k) {
+    uint32_t w[4];
+    lds128(tile + state_at<HC>(lane, k), w);
+    s[2 * k] = make_float2(__uint_as_float(w[0]), __uint_as_float(w[1]));
+    s[2 * k + 1] = make_float2(__uint_as_float(w[2]), __uint_as_float(w[3]));
+  }
+}
+template <int HC>
+__device__ __forceinline__ void state_store(const float2 (&s)[HC / 2], uint32_t tile, float* g, int64_t ld, int rows, int cols) {
+  constexpr int CH = HC / 4;
+  const int lane = threadIdx.x & 31, ch = lane % CH;
+#pragma unroll
+  for (int k = 0; k < CH; ++k) {
+    const uint32_t w[4] = {__float_as_uint(s[2 * k].x), __float_as_uint(s[2 * k].y), __float_as_uint(s[2 * k + 1].x),
+                           __float_as_uint(s[2 * k + 1].y)};
+    sts128(tile + state_at<HC>(lane, k), w);
+  }
+  __syncwarp();
+#pragma unroll
+  for (int t = 0; t < CH; ++t) {
+    const int row = t * (32 / CH) + lane / CH;
+    uint32_t w[4];
+    lds128(tile + state_at<HC>(row, ch), w);
+    if (row < rows && ch * 4 < cols)
+      *reinterpret_cast<uint4*>(g + row * ld + ch * 4) = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
 // A matrix descriptor (sdesc) whose start moves by whole 16-byte units: the address field is the low 14 bits
 // and shared memory ends below 2^18, so a step never carries out of it.
 struct Desc {
