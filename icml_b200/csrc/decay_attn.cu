@@ -550,23 +550,32 @@ __global__ void __launch_bounds__(256) step_kernel(const StepArgs a) {
 // host
 // ---------------------------------------------------------------------------------------------
 // How the sequence is cut.  Pieces run side by side, but all except one have their y and z read a second time
-// (for the states that enter the others), so the cut is the one with the least time over the waves of CTAs:
-// chunks of a piece (1.5 x when cut) plus a fixed 2.5 chunks of start and end per piece and 3 for the extra
-// launches, in units of one chunk's time.
+// (for the states that enter the others), so the cut is the one with the least time over the waves of CTAs, in
+// units of a chunk's time in a walk: a piece's chunks plus 2.5 for its start and end, the same for the states' pass
+// at 0.6 of the walk's pace (0.8 in a backward, whose two passes end before its walks begin), and 3 for the two more
+// launches.  walks and passes count what one call runs side by side
+// (a backward's launches overlap).  Measured with and without a cut: 65536 tokens x 8 heads of 128, forward,
+// 188 and 1929 us; 7 rows of 1999 x 8 heads of 64, 37 and 34 us; backward of 9 x 3000 x 8 heads of 128,
+// 440 and 355 us; of 1 x 2000 x 8 heads of 128, 65 and 73 us.
+// The float32 engine's walk of a chunk is longer beside its other parts and several CTAs share an SM: with its own
+// constants below, 2 x 777 tokens x 6 heads take 94 us backward in 13 pieces, 100 in 7, 138 in 4 and 425 in one.
 struct Cut {
   int segs;
   int64_t seg_len;
 };
-static Cut cut(int64_t ctas, int64_t L, int chunk, int resident) {
+static Cut cut(int64_t ctas, int64_t L, int chunk, bool tc, int resident, int walks, int passes) {
   const int64_t chunks = (L + chunk - 1) / chunk, slots = 148 * resident;
   Cut best = {1, (chunks ? chunks : 1) * chunk};
   if (ctas == 0) return best;
+  auto waves = [&](int64_t n) { return double((ctas * n + slots - 1) / slots); };
   double least = 0;
   // (more than two waves of pieces never pay)
   for (int64_t s = 1; s <= chunks && (s == 1 || ctas * s <= 2 * slots); ++s) {
     const int64_t per = (chunks + s - 1) / s, n = (chunks + per - 1) / per;
     if (n != s) continue;
-    const double t = double((ctas * n + slots - 1) / slots) * (double(per) * (n > 1 ? 1.5 : 1.0) + 2.5) + (n > 1 ? 3.0 : 0.0);
+    double t;
+    if (tc) t = waves(walks * n) * (per + 2.5) + (n > 1 ? waves(passes * n) * (per + 2.5) * (passes > 1 ? 0.8 : 0.6) + 3.0 : 0.0);
+    else t = waves(n) * (per * (n > 1 ? 1.5 : 1.0) + 2.5) + (n > 1 ? 3.0 : 0.0);
     if (s == 1 || t < least) {
       least = t;
       best = {int(n), per * chunk};
@@ -609,11 +618,12 @@ struct Plan {
   Cut c;
 };
 static Plan plan(const Shape& p, bool tc, bool backward) {
-  if (tc) return {true, cut(p.B * p.H, p.L, TC_CHUNK, 1)};
+  const int walks = backward ? 4 : 1, passes = backward ? 2 : 1;   // (grad ln a is a walk of its own)
+  if (tc) return {true, cut(p.B * p.H, p.L, TC_CHUNK, true, 1, walks, passes)};
   // a backward's calls have either width as columns and either as rows
   const int64_t cols = backward && p.Dk < p.Dv ? p.Dk : p.Dv, rows = backward && p.Dv > p.Dk ? p.Dv : p.Dk;
   const int resident = int(233472 / (smem_bytes((int(rows) + 3) & ~3, MODE_OUT) + 1024));
-  return {false, cut(p.B * p.H * ceil_div(cols, E), p.L, chunk_of(int(rows)), resident)};
+  return {false, cut(p.B * p.H * ceil_div(cols, E), p.L, chunk_of(int(rows)), false, resident, walks, passes)};
 }
 
 // The state that enters each piece of a walk: (B, H, segs, rows, columns).
