@@ -76,7 +76,7 @@ struct Params {
 
 // Barriers behind full[NS] and empty[NS].  A and P take turns where there are two A buffers: X may be a chunk
 // ahead of the product that reads P.
-enum { B_A = 0, B_A1, B_P, B_P1, B_K, B_K1, B_U, B_U1, B_O, B_DFREE, B_S, B_OSTAGED, B_SUM, B_DONE, B_COUNT };
+enum { B_A = 0, B_A1, B_P, B_P1, B_K, B_K1, B_U, B_U1, B_O, B_DFREE, B_S, B_OSTAGED, B_STORED, B_SUM, B_DONE, B_COUNT };
 
 template <int DX, int DZ, int NT, bool REV>
 struct Walk {
@@ -321,6 +321,9 @@ struct Walk {
       }
     }
     fence_async();
+    // The store warp has seen the chunk before: with eight slots X could otherwise stage two more chunks while that
+    // warp waits for a slow store, and a barrier two phases ahead looks as if it had not moved.
+    if (c > 0 && !wait(B_STORED, c - 1)) return false;
     arrive(B_OSTAGED);
     return true;
   }
@@ -348,6 +351,7 @@ struct Walk {
     for (int c = 0; c < chunks; ++c) {
       const uint32_t nz = tile_z(c);
       if (!wait(B_OSTAGED, c)) return;
+      arrive(B_STORED);
       if (lane == 0) {
         if (!p.out_f32) {
           const int t0 = int(first_token(c));
@@ -549,7 +553,7 @@ walk_tc_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
   if (threadIdx.x < 32) tab[132 + threadIdx.x] = exp2f(l2 * float(REV ? threadIdx.x : 31 - threadIdx.x));
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2 * G::NS; ++s) mbar_init(&full[s], 1);
-    for (int k = 0; k < B_COUNT; ++k) mbar_init(&bars[k], k <= B_A1 || k == B_U || k == B_U1 || k == B_O || k == B_DONE ? 1 : 8);
+    for (int k = 0; k < B_COUNT; ++k) mbar_init(&bars[k], k <= B_A1 || k == B_U || k == B_U1 || k == B_O || k == B_STORED || k == B_DONE ? 1 : 8);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmX)) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(&tmY)) : "memory");
