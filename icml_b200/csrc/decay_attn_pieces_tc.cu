@@ -4,7 +4,8 @@
 //   S' = a^n S + (a^(n-1-j) y)^T z       chunk by chunk of n <= 128 tokens, to float32 accuracy
 //
 // with y's weighted rows as three bf16 terms, a fresh accumulator per chunk and the state in registers, as in the
-// walk itself (decay_attn_tc.cu).  Nothing else is formed, so the reads of y and z and shared memory set the
+// walk itself (decay_attn_tc.cu).  65536 tokens x 8 heads of 128: 61 us, 4.3 TB/s (77 with whole chunks and one
+// accumulator, weigh - product - state one after the other).  Nothing else is formed, so the reads of y and z and shared memory set the
 // pace: per chunk and 128 x 128 state 1,000 wavefronts to weigh y, 1,500 for the products' operands, 500 for the
 // tiles.  y is weighed by halves of 64 tokens into two buffers and there are two accumulators, so that the
 // products of one half run while the next is weighed and the state of a chunk is stepped a chunk later.

@@ -20,7 +20,8 @@
 // by halves of 64 tokens (k, q, k, q: two buffers, so that the products of one run while the other is weighed),
 // adds its block of the pair sum, adds its part of <S, V1> + <S', V2> and steps its 16 columns of the state.
 // Shared memory is what it needs most: per chunk 1,500 wavefronts to write the weighted terms, 2,800 for the
-// products to read them and 512 for the tiles.
+// products to read them and 512 for the tiles.  16 x 2048 tokens x 16 heads of 64: 132 us (161 with whole chunks
+// weighed before their products).
 #include "decay_attn_tc.cuh"
 
 namespace pgf {

@@ -23,9 +23,18 @@
 // Roles (640 threads): warp 0 TMA loads, warp 1 MMA, warps 2..9 scores and output ("X"), warps 10..17 the
 // weighted y and the state ("Y"), warp 18 the output's TMA stores.  The chunk's steps overlap with its
 // neighbours': X forms P of chunk c beside the output of c - 1, so that it seldom waits for a product;
-// Y weighs y of c, publishes S and only then waits for U.  Input tiles pass through a ring of slots in the order
-// y, x, z; hi overwrites y in its slot once A is done, and the output is staged in z's slot.  Every wait is
+// Y publishes S and weighs y before it waits for U (64-wide heads have two buffers of A, U and y's smaller terms, so
+// that y of the next chunk is weighed while this one's U is formed).  Input tiles pass through a ring of slots in the
+// order y, x, z; hi overwrites y in its slot once A is done, and the output is staged in z's slot.  Every wait is
 // bounded.
+//
+// What bounds it: shared memory, which the products' operands and the warps share.  65536 tokens x 8 heads of 128
+// take 129 us (16 x 2048 x 16 heads of 64: 72 us), 4.2 TB/s of its four tensors; a 128-wide chunk takes 3.2 us where
+// 32 SMs walk and 4.2 where all do, and the warps that weigh y are the ones that the others wait for.  Measured
+// and slower: the output stored straight from registers (157 against 129 us), half of y weighed by X (148 against
+// 137), y weighed by parts of 32 tokens out of place (139 against 128), the next A in front of D1 (144 against 129).
+// The float32 engine (decay_attn.cu) takes 3350 us for the first of these sizes: bf16 inputs of widths that are
+// multiples of 8 up to 128, in 16-byte aligned tensors, go here whatever their number.
 //
 // P takes two multiplications for 32 x 32 blocks off the diagonal (a^(i-j) as a row factor times a column factor,
 // both with exponents >= 0: no overflow for any decay), a table look-up for the four on it, nothing for the rest.

@@ -15,11 +15,15 @@
 //   grad x = r (gu w - xh mean(gu w xh))
 //
 // Bound by HBM: the forward reads and writes each element once, the backward reads x and g and writes
-// grad x.  A warp takes a token with all its heads: it forms the token's cosines and sines once (the
-// heads share them) and then walks the rows (token, head), a power-of-two group of lanes per row.  A lane holds two 16-byte chunks that are each other's rotation partners, so the
-// rotation needs no exchange between lanes and the row sums are a few shuffles.  The backward's CTAs
-// walk the tiles in a fixed order and leave one partial of grad w each, added in CTA order by a second
-// kernel: no atomics, the same bits on every run.
+// grad x.  Measured (bf16): forward 16 x 2048 x 32 heads of 64 49 us, 5.5 TB/s; backward 65536 x 16 heads of 128
+// 153 us, 5.3 TB/s.  Widths or tensors that 16-byte pieces do not fit take rotate_any_kernel, a warp per row (765
+// and 3,050 us at these sizes).
+//
+// A warp takes a token with all its heads: it forms the token's cosines and sines once (the heads share them) and
+// then walks the rows (token, head), a power-of-two group of lanes per row.  A lane holds two 16-byte chunks that
+// are each other's rotation partners, so the rotation needs no exchange between lanes and the row sums are a few
+// shuffles.  The backward's CTAs walk the tiles in a fixed order and leave one partial of grad w each, added in CTA
+// order by a second kernel: no atomics, the same bits on every run.
 #include "chain.cuh"
 #include "f32x2.cuh"
 
@@ -510,6 +514,7 @@ static int launch(Args& a, bool halves, cudaStream_t s) {
   for (int z = 0; z < 2; ++z) {
     int64_t ctas;
     if (vec) {
+      // (131072 tokens x 2 + 2 heads of 64: 62 us in tiles of 4, 164 in tiles of one)
       // more tokens a tile while the heads of one leave groups idle and there are tiles enough for the warps
       a.tw[z] = 1;
       while (2 * a.tw[z] <= 32 / G && 32 / G / a.tw[z] > a.H[z] && a.tokens / (2 * a.tw[z]) >= 148 * 16) a.tw[z] *= 2;
