@@ -28,7 +28,8 @@
 // order y, x, z; hi overwrites y in its slot once A is done, and the output is staged in z's slot.  Every wait is
 // bounded.
 //
-// What bounds it: shared memory, which the products' operands and the warps share.  65536 tokens x 8 heads of 128
+// What bounds it: the chain of a chunk's steps (weigh, product, state) in shared memory, which the products' operands
+// and the warps share (4,350 wavefronts of a 128-wide chunk's 7,500 cycles).  65536 tokens x 8 heads of 128
 // take 129 us (16 x 2048 x 16 heads of 64: 72 us), 4.2 TB/s of its four tensors; a 128-wide chunk takes 3.2 us where
 // 32 SMs walk and 4.2 where all do, and the warps that weigh y are the ones that the others wait for.  Measured
 // and slower: the output stored straight from registers (157 against 129 us), half of y weighed by X (148 against
