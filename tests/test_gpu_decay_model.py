@@ -313,3 +313,31 @@ def test_calls_in_a_graph_and_back_to_back(B, L, H, Hk, dtype):
         graph.replay()
         assert all(torch.equal(a, b) for a, b in zip(got, alone[i])), f"replay {i}"
     graph.reset()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_states_at_any_address(dtype):
+    """States that begin 4 bytes behind a 16-byte boundary: the same results within both paths' roundings."""
+    from icml_b200 import ops
+    torch.manual_seed(8)
+    q, k, v, g = (torch.randn(2, 300, 3, 64, device=DEV).to(dtype) for _ in range(4))
+    ld = torch.tensor([-0.01, -0.1, -1.0], device=DEV)
+    s, gs = torch.randn(2, 3, 64, 64, device=DEV), torch.randn(2, 3, 64, 64, device=DEV)
+
+    def moved(t):
+        u = torch.empty(t.numel() + 1, device=DEV)[1:].view(t.shape)
+        u.copy_(t)
+        assert u.is_contiguous() and u.data_ptr() % 16 == 4
+        return u
+
+    def call(s, gs):
+        out, end = ops.decay_attn_fwd(q, k, v, ld, state=s)
+        r = ops.decay_attn_bwd(q, k, v, ld, g, state=s, g_state=gs, need_g_log_decay=True)
+        one, new = ops.decay_attn_step(q[:, 0], k[:, 0], v[:, 0], ld, s)
+        return dict(r, out=out, end=end, one=one, new=new)
+
+    a, b = call(s, gs), call(moved(s), moved(gs))
+    for n, t in a.items():
+        # float32 results: 1e-5 each; bfloat16: three roundings of 2^-9 each
+        tol = 2 * (1e-5 if t.dtype == torch.float32 else 6e-3)
+        assert (t.double() - b[n].double()).norm() <= tol * t.double().norm(), n
