@@ -61,6 +61,9 @@ struct Cfg {
   static constexpr uint32_t RING = NS * SLOT;
   static constexpr uint32_t MID = RING, LO = MID + NA * XB, ZERO = LO + NA * XB;  // ZERO only with 64-wide y
   static constexpr uint32_t ST = NT == 2 ? LO : DX == 64 ? ZERO + BLK : ZERO;  // S: 128 rows x DZ bf16
+  // at the walk's end: the middle terms' part of a 64-wide y's state lies in MID .. SUM_END, and the state leaves
+  // through LEAVES on
+  static constexpr uint32_t SUM_END = MID + (DX == 64 ? 64 * DZ * 4 : 0), LEAVES = DX == 64 ? LO : MID;
   static constexpr uint32_t WTAB = ST + ZB;                             // 130 x 8 bytes
   static constexpr uint32_t TAB = WTAB + 1040;                          // 132 + 32 floats
   static constexpr uint32_t BARS = TAB + 656;
@@ -506,7 +509,7 @@ struct Walk {
     if (DX == 64) {
       // rows 64..127 hold the middle terms' part; the ring is done with
       float2* sum = reinterpret_cast<float2*>(base + G::MID);
-      static_assert(DX != 64 || G::MID + 64 * DZ * 4 <= G::TAB, "the sum fits");
+      static_assert(NT == 2 || G::SUM_END <= G::ST, "the sum fits");
       if (i >= 64) {
 #pragma unroll
         for (int k = 0; k < HC / 2; ++k) sum[(i - 64) + (half * (HC / 2) + k) * 64] = s[k];
@@ -517,13 +520,19 @@ struct Walk {
 #pragma unroll
         for (int k = 0; k < HC / 2; ++k) s[k] = __fadd2_rn(s[k], sum[i + (half * (HC / 2) + k) * 64]);
       }
+      // 128-wide z: the sum takes both terms' places, the second of which the state leaves through; no warp writes
+      // there before all have read
+      if constexpr (G::SUM_END > G::LEAVES) {
+        arrive(B_SUM);
+        if (!mbar_wait_warp(&bars[B_SUM], 1)) return;
+      }
     }
     const int r0 = q * 32, c0 = half * HC;
     if (r0 < DX) {
-      // (all products that read y's terms are done; 64-wide: behind the sum)
-      static_assert(NT == 2 || (DX == 64 ? G::LO : G::MID) + DX * DZ * 4 <= G::ST, "the states fit");
-      state_store<HC>(s, sbase + (DX == 64 ? G::LO : G::MID) + uint32_t(q * 2 + half) * HC * 128,
-                      end + int64_t(r0) * p.dz + c0, p.dz, p.dx - r0, p.dz - c0);
+      // (all products that read y's terms are done; D1 of the last chunk may still read S)
+      static_assert(NT == 2 || G::LEAVES + DX * DZ * 4 <= G::ST, "the states fit");
+      state_store<HC>(s, sbase + G::LEAVES + uint32_t(q * 2 + half) * HC * 128, end + int64_t(r0) * p.dz + c0, p.dz,
+                      p.dx - r0, p.dz - c0);
     }
   }
 };

@@ -1,0 +1,51 @@
+"""Edges of the decay-attention layer's operators on the GPU: states that leave in shared memory's last places,
+rows that need no reading, values that are no numbers, lengths of any whole type.
+
+Tolerances are those of test_gpu_decay.py: 1e-5 of the 2-norm for what comes back as float32, 6e-3 for bfloat16;
+whatever is called twice gives the same bits.
+"""
+import math
+
+import pytest
+import torch
+
+from tests import decay_oracle as O
+from tests.test_gpu_decay import BOTH, DEV, TOL, _beam_check, _close, _gen, _n
+
+pytestmark = pytest.mark.gpu
+
+
+def _same(a, b):
+    """Equal values, NaN equal to NaN."""
+    return torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(nan=0.0), b.nan_to_num(nan=0.0))
+
+
+# --------------------------------------------------------------------------------------- states that leave
+@pytest.mark.parametrize("Dk,Dv", [(64, 128), (48, 80), (64, 64), (128, 128), (128, 64)])
+def test_final_states_of_whole_walks_repeat(Dk, Dv):
+    """bfloat16 calls that are not cut hand their states over inside the kernel: the same bits in every one of a
+    thousand calls, within the bound of float64."""
+    from icml_b200 import ops
+    from icml_b200._lib import lib
+    B, L, H = 8, 130, 16
+    assert lib().pgf_decay_attn_workspace(B, L, H, H, H, H, Dk, Dv, 1, 0) == 0, "cut"
+    g = _gen(Dk * 1000 + Dv)
+    q, k, v, go = (_n(g, B, L, H, d).bfloat16() for d in (Dk, Dk, Dv, Dv))
+    ld = -torch.exp2(-1.0 - 0.5 * torch.arange(H, device=DEV)).float()
+    s, gs = _n(g, B, H, Dk, Dv), _n(g, B, H, Dk, Dv)
+
+    def call():
+        _, end = ops.decay_attn_fwd(q, k, v, ld, state=s)
+        return end, ops.decay_attn_bwd(q, k, v, ld, go, state=s, g_state=gs)["grad_state"]
+
+    end, grad = call()
+    s64 = s.double().requires_grad_()
+    o, want = O.decay_attn(q.double(), k.double(), v.double(), ld.double(), Dk ** -0.5, s64, None)
+    (g64,) = torch.autograd.grad((o * go.double()).sum() + (want * gs.double()).sum(), s64)
+    _close(end, want, 1e-5, "state", 2)
+    _close(grad, g64, 1e-5, "grad_state", 2)
+    off = torch.zeros(2, dtype=torch.int64, device=DEV)
+    for _ in range(1000):
+        e, r = call()
+        off += torch.stack([(e != end).sum(), (r != grad).sum()])
+    assert not off.any(), off.tolist()
