@@ -148,6 +148,7 @@ __global__ void __cluster_dims__(CS, 1, 1) __launch_bounds__(THREADS, 1) select_
   __shared__ float s_score[UNITS];
   __shared__ bool s_done[UNITS], s_fixed[UNITS];
   __shared__ uint64_t s_wk[WARPS];
+  __shared__ bool s_failed;                          // a wait for the held part ran out
   cg::cluster_group cl = cg::this_cluster();
   const int rank = int(cl.block_rank());
   const int64_t b = blockIdx.x / CS;
@@ -174,9 +175,12 @@ __global__ void __cluster_dims__(CS, 1, 1) __launch_bounds__(THREADS, 1) select_
     extern __shared__ __align__(128) uint8_t smem[];
     held = smem_u32(smem);
     if (threadIdx.x == 0) {
+      s_failed = false;
       for (int c = 0; c < CHUNKS; ++c) mbar_init(&s_bars[c], 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-      if (rank < U) {
+      // every copy that begins is waited for in pass 1, so a unit that pass 1 does not read copies nothing (thread 0
+      // has just formed s_fixed[0])
+      if (rank < U && !s_fixed[0]) {
         const Span<T> sp = span(rank);
         const int per = (sp.nv + CHUNKS - 1) / CHUNKS;
         for (int c = 0; c < CHUNKS; ++c) {
@@ -190,14 +194,13 @@ __global__ void __cluster_dims__(CS, 1, 1) __launch_bounds__(THREADS, 1) select_
       }
     }
   }
-  bool ok = true;
   __syncthreads();
 
   // ---- pass 1: maximum, sum of exponentials, group maxima
   for (int u = rank, n = 0; u < U; u += CS, ++n) {
     float m = -INFINITY, s = 0.f;
     if (!s_fixed[n]) {
-      ok = scan<HOLD>(span(u), held, s_bars, [&](const auto& f, int) {
+      const bool ok = scan<HOLD>(span(u), held, s_bars, [&](const auto& f, int) {
         constexpr int n = int(sizeof(f) / sizeof(float));
         float mm = f[0];
 #pragma unroll
@@ -213,6 +216,11 @@ __global__ void __cluster_dims__(CS, 1, 1) __launch_bounds__(THREADS, 1) select_
           s += q;
         }
       });
+      if (HOLD && !ok) {
+        // a wait ran out: the step writes no outputs, and no copy is in flight when the block leaves
+        if (lane == 0) s_failed = true;
+        for (int c = 0; c < CHUNKS; ++c) mbar_wait_warp(&s_bars[c], 0);
+      }
     }
     // the K-th largest of the maxima of 16 warps (K <= 16) or 32 half warps: that many candidates reach it
     float gm = m;
@@ -339,8 +347,9 @@ __global__ void __cluster_dims__(CS, 1, 1) __launch_bounds__(THREADS, 1) select_
       const int u = i / K;
       s_list[i] = cl.map_shared_rank(&s_best[0][0], u % CS)[(u / CS) * MAX_K + i % K];
     }
-    __syncthreads();
-    for (int i = threadIdx.x; i < U * K; i += THREADS) {
+    const bool failed = HOLD && threadIdx.x < CS && *cl.map_shared_rank(&s_failed, int(threadIdx.x));
+    const bool skip = __syncthreads_or(failed);
+    for (int i = threadIdx.x; i < U * K && !skip; i += THREADS) {
       const uint64_t mine = s_list[i];
       if (mine == 0) continue;
       int before = 0;

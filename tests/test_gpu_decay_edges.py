@@ -49,3 +49,34 @@ def test_final_states_of_whole_walks_repeat(Dk, Dv):
         e, r = call()
         off += torch.stack([(e != end).sum(), (r != grad).sum()])
     assert not off.any(), off.tolist()
+
+
+# ------------------------------------------------------------------------------------- rows without a choice
+@pytest.mark.parametrize("live", [0, 1])
+@pytest.mark.parametrize("B,K,V,dtype", [(16, 8, 50257, torch.bfloat16), (2, 4, 100003, torch.float32), (2, 16, 33000, torch.float32)])
+def test_beam_rows_that_need_no_reading_leave_nothing_behind(B, K, V, dtype, live):
+    """Sequences whose beams have all finished, and whose beams but one stand at -inf, at sizes whose rows are copied
+    into shared memory: the selection is right, and the calls that follow at once give the bits of calls alone."""
+    from icml_b200 import ops
+    g = _gen(B + K)
+    logits, scores = (3 * _n(g, B, K, V)).to(dtype), -10 + _n(g, B, K)
+    q, k, v = (_n(g, 4, 256, 4, 64).bfloat16() for _ in range(3))
+    ld = torch.full((4,), -0.05, device=DEV)
+    done = torch.ones(B, K, dtype=torch.bool, device=DEV)
+    if live:
+        scores[:, 1:] = -math.inf
+        done[:] = False
+    torch.cuda.synchronize()
+    alone, s_alone = ops.decay_attn_fwd(q, k, v, ld)
+    torch.cuda.synchronize()
+    _beam_check(logits, scores, done, V - 1)
+    first = ops.beam_select(logits, scores, done, end_id=V - 1)
+    if not live:
+        order = torch.sort(scores, dim=1, descending=True, stable=True)
+        assert torch.equal(first[0], order.values) and bool((first[2] == V - 1).all()) and bool(first[3].all())
+        assert torch.equal(first[1], order.indices + K * torch.arange(B, device=DEV)[:, None])
+    for _ in range(50):
+        again = ops.beam_select(logits, scores, done, end_id=V - 1)
+        out, end = ops.decay_attn_fwd(q, k, v, ld)
+        assert all(torch.equal(a, b) for a, b in zip(first, again))
+        assert torch.equal(out, alone) and torch.equal(end, s_alone)
