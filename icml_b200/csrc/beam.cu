@@ -209,12 +209,12 @@ __global__ void __cluster_dims__(CS, 1, 1) __launch_bounds__(THREADS, 1) select_
           s *= ex2f((m - mm) * L2E);
           m = mm;
         }
-        if (m != -INFINITY) {
-          float q = 0.f;
+        // nothing but -inf so far: terms of zero, and a NaN enters the sum wherever it stands
+        const float ref = m == -INFINITY ? 0.f : m;
+        float q = 0.f;
 #pragma unroll
-          for (int e = 0; e < n; ++e) q += ex2f((f[e] - m) * L2E);
-          s += q;
-        }
+        for (int e = 0; e < n; ++e) q += ex2f((f[e] - ref) * L2E);
+        s += q;
       });
       if (HOLD && !ok) {
         // a wait ran out: the step writes no outputs, and no copy is in flight when the block leaves

@@ -80,3 +80,30 @@ def test_beam_rows_that_need_no_reading_leave_nothing_behind(B, K, V, dtype, liv
         out, end = ops.decay_attn_fwd(q, k, v, ld)
         assert all(torch.equal(a, b) for a, b in zip(first, again))
         assert torch.equal(out, alone) and torch.equal(end, s_alone)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("V", [50257, 1029, 100003])
+def test_beam_nan_counts_in_every_column(V, dtype):
+    """A NaN logit makes its row's log sum NaN and the row's candidates -inf wherever it stands: first and last
+    column (single elements in front of and behind the 16-byte pieces, as rows of an odd width start anywhere), in a
+    piece of its own kind, and among banned tokens."""
+    g = _gen(V)
+    B, K = 4, 4
+    base = (3 * _n(g, B, K, V)).to(dtype)
+    scores = -_n(g, B, K).abs()
+    banned = slice(V // 2 - 100, V // 2 + 100)
+    spots = [slice(0, 1), slice(V - 1, V), slice(1, 2), slice(V // 2, V // 2 + 1), slice(V // 2, V // 2 + 32), slice(7, 8)]
+    for n, at in enumerate(spots):
+        for k in range(K):
+            logits = base.clone()
+            logits[:, :, banned] = -math.inf
+            logits[:, k, at] = math.nan
+            so, flat, _ = _beam_check(logits, scores, None, None)
+            assert not (flat // V == k).any(), (n, k)
+    logits = base.clone()
+    logits[:] = -math.inf
+    logits[:, 1:, V - 1] = math.nan
+    logits[:, 0, 3] = 1.0
+    so, flat, _ = _beam_check(logits, scores, None, None)
+    assert torch.equal(flat[:, 0], torch.full((B,), 3, device=DEV)) and bool((so[:, 1:] == -math.inf).all())
