@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(128) enter_kernel(const __grid_constant__ Ente
       if (k >= segs) break;
       const int64_t s0 = min(len, s * a.seg_len), s1 = min(len, s0 + a.seg_len);
       p[int64_t(s) * n] = cur;
-      cur = fmaf(exp2f(l2 * float(s1 - s0)), cur, own[u]);
+      if (s1 > s0) cur = fmaf(exp2f(l2 * float(s1 - s0)), cur, own[u]);   // (no tokens: a^0, of a NaN too)
     }
   }
   if (a.last[w]) a.last[w][bh * n + i] = cur;

@@ -53,9 +53,10 @@ struct Job {
   int last_too;              // pieces' own end states: the walk's last piece as well
 };
 
-// a^e for the exponents of one head.  log2(a) is clamped so that e = 0 gives 1 for a decay of zero.
+// a^e for the exponents of one head.  log2(a) is clamped so that e = 0 gives 1 for a decay of zero; a NaN stays one.
 __device__ __forceinline__ float log2_decay(float log_decay) {
-  return fmaxf(log_decay * 1.4426950408889634f, -1.0e4f);
+  const float l2 = log_decay * 1.4426950408889634f;
+  return l2 < -1.0e4f ? -1.0e4f : l2;
 }
 
 __device__ __forceinline__ int64_t row_length(const int32_t* lengths, int64_t b, int64_t L) {

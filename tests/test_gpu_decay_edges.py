@@ -107,3 +107,31 @@ def test_beam_nan_counts_in_every_column(V, dtype):
     logits[:, 0, 3] = 1.0
     so, flat, _ = _beam_check(logits, scores, None, None)
     assert torch.equal(flat[:, 0], torch.full((B,), 3, device=DEV)) and bool((so[:, 1:] == -math.inf).all())
+
+
+# ---------------------------------------------------------------------------------------------- decays, lengths
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("B,L", [(3, 70), (1, 4000)])
+def test_a_decay_that_is_no_number_shows(B, L, dtype):
+    """A NaN decay makes its head's outputs, states and gradients NaN, at one token and over cut walks, and leaves the
+    other heads' bits alone; a row without tokens keeps its state."""
+    from icml_b200 import ops
+    g = _gen(L)
+    q, k, v, go = (_n(g, B, L, 2, 64).to(dtype) for _ in range(4))
+    s, gs = _n(g, B, 2, 64, 64), _n(g, B, 2, 64, 64)
+    good, bad = torch.tensor([-0.1, -0.1], device=DEV), torch.tensor([math.nan, -0.1], device=DEV)
+
+    def call(ld, lengths=None):
+        out, end = ops.decay_attn_fwd(q, k, v, ld, state=s, lengths=lengths)
+        r = ops.decay_attn_bwd(q, k, v, ld, go, state=s, g_state=gs, lengths=lengths, need_g_log_decay=True)
+        one, new = ops.decay_attn_step(q[:, 0], k[:, 0], v[:, 0], ld, s)
+        heads = [out.transpose(1, 2), end, r["grad_q"].transpose(1, 2), r["grad_k"].transpose(1, 2),
+                 r["grad_v"].transpose(1, 2), r["grad_state"], one, new]
+        return [t.transpose(0, 1) for t in heads] + [r["grad_log_decay"]]
+
+    for i, (a, b) in enumerate(zip(call(good), call(bad))):
+        assert torch.equal(a[1], b[1]), i
+        assert bool(b[0].isnan().all() if i not in (3, 4) else b[0].isnan().any()), i
+    none = torch.zeros(B, dtype=torch.int32, device=DEV)
+    out, end, *_, g0, _, _, gl = call(bad, none)
+    assert not out.any() and torch.equal(end.transpose(0, 1), s) and torch.equal(g0.transpose(0, 1), gs)
