@@ -893,6 +893,13 @@ def _whole(name: str, what: str, t: torch.Tensor, shape, dev: int, dtype) -> tor
     return t if t.is_contiguous() else t.contiguous()
 
 
+def _lengths(name: str, t: torch.Tensor, B: int, L: int, dev: int) -> torch.Tensor:
+    """A row's length each, as int32: below zero counts as none, beyond the sequence as all of it."""
+    if t.dtype is not torch.int32 and t.element_size() >= 4 and not t.is_floating_point():
+        t = t.clamp(0, L)  # (the kernels clamp what 32 bits hold)
+    return _whole(name, "lengths", t, (B,), dev, torch.int32)
+
+
 def _raw_stream(dev: int) -> int:
     """The current stream of the tensors' device, which has to be the current device."""
     if dev != torch._C._cuda_getDevice():
@@ -1007,7 +1014,7 @@ def decay_attn_fwd(q, k, v, log_decay, *, scale: Optional[float] = None, state=N
     if state is not None:
         state = _param(f"{name}: state", state, (B, H, Dk, Dv), dev)
     if lengths is not None:
-        lengths = _whole(name, "lengths", lengths, (B,), dev, torch.int32)
+        lengths = _lengths(name, lengths, B, L_, dev)
     (q, qs), (k, ks), (v, vs) = _view(q), _view(k), _view(v)
     out = v.new_empty((B, L_, H, Dv))
     end = log_decay.new_empty((B, H, Dk, Dv)) if want_state else None
@@ -1035,7 +1042,7 @@ def decay_attn_bwd(q, k, v, log_decay, g, *, scale: Optional[float] = None, stat
     if g_state is not None:
         g_state = _param(f"{name}: g_state", g_state, (B, H, Dk, Dv), dev)
     if lengths is not None:
-        lengths = _whole(name, "lengths", lengths, (B,), dev, torch.int32)
+        lengths = _lengths(name, lengths, B, L_, dev)
     (q, qs), (k, ks), (v, vs), (g, gs) = _view(q), _view(k), _view(v), _view(g)
     gq, gk, gv = q.new_empty(q.shape), k.new_empty(k.shape), v.new_empty(v.shape)
     g0 = log_decay.new_empty((B, H, Dk, Dv))

@@ -135,3 +135,22 @@ def test_a_decay_that_is_no_number_shows(B, L, dtype):
     none = torch.zeros(B, dtype=torch.int32, device=DEV)
     out, end, *_, g0, _, _, gl = call(bad, none)
     assert not out.any() and torch.equal(end.transpose(0, 1), s) and torch.equal(g0.transpose(0, 1), gs)
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+def test_lengths_of_any_whole_type(dtype):
+    """Lengths below zero and beyond the sequence, in 64 bits too, count as none and all."""
+    from icml_b200 import ops
+    g = _gen(11)
+    B, L = 6, 200
+    q, k, v, go = (_n(g, B, L, 2, 64).to(dtype) for _ in range(4))
+    ld = torch.tensor([-0.1, -0.01], device=DEV)
+
+    def call(n):
+        out, end = ops.decay_attn_fwd(q, k, v, ld, lengths=n)
+        return [out, end, *ops.decay_attn_bwd(q, k, v, ld, go, lengths=n, need_g_log_decay=True).values()]
+
+    far = torch.tensor([2 ** 63 - 1, 2 ** 32 + 5, 2 ** 31, -1, -2 ** 63, 77], device=DEV)
+    want = call(torch.tensor([L, L, L, 0, 0, 77], dtype=torch.int32, device=DEV))
+    assert all(torch.equal(a, b) for a, b in zip(call(far), want))
+    assert all(torch.equal(a, b) for a, b in zip(call(far.clamp(-2 ** 15, 2 ** 15 - 1).short()), want))
