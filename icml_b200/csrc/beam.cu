@@ -388,29 +388,27 @@ static int select_as(Args a, int64_t Bsz, cudaStream_t s) {
 // Few sequences (up to 4) take clusters of 16, more of them 8 (one sequence of 4 x 50257: 9 us against 12; 16 of
 // them fill the GPU either way).  Clusters of 16 are beyond the portable size: asked for once, and used if the device can place one.
 template <class T>
+static bool ask_wide() {
+  for (auto* k : {select_kernel<T, 16, true>, select_kernel<T, 16, false>})
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return false;
+  if (cudaFuncSetAttribute(select_kernel<T, 16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, HELD_MOST) != cudaSuccess)
+    return false;
+  cudaLaunchConfig_t c = {};
+  c.gridDim = dim3(16);
+  c.blockDim = dim3(THREADS);
+  c.dynamicSmemBytes = HELD_MOST;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = 16;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  c.attrs = &at;
+  c.numAttrs = 1;
+  int n = 0;
+  return cudaOccupancyMaxActiveClusters(&n, select_kernel<T, 16, true>, &c) == cudaSuccess && n >= 1;
+}
+template <class T>
 static bool wide_clusters() {
-  static const bool ok = [] {
-    for (auto* k : {select_kernel<T, 16, true>, select_kernel<T, 16, false>})
-      if (cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) return false;
-    if (cudaFuncSetAttribute(select_kernel<T, 16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, HELD_MOST) != cudaSuccess)
-      return false;
-    cudaLaunchConfig_t c = {};
-    c.gridDim = dim3(16);
-    c.blockDim = dim3(THREADS);
-    c.dynamicSmemBytes = HELD_MOST;   // also when each CTA fills an SM
-    cudaLaunchAttribute at;
-    at.id = cudaLaunchAttributeClusterDimension;
-    at.val.clusterDim.x = 16;
-    at.val.clusterDim.y = at.val.clusterDim.z = 1;
-    c.attrs = &at;
-    c.numAttrs = 1;
-    int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, select_kernel<T, 16, true>, &c) != cudaSuccess || n < 1) {
-      cudaGetLastError();
-      return false;
-    }
-    return true;
-  }();
+  static const bool ok = ask_wide<T>() || (cudaGetLastError(), false);   // a refusal is an answer, not the launch's error
   return ok;
 }
 
