@@ -69,15 +69,19 @@ static inline cudaStream_t as_stream(pgf_stream_t s) { return reinterpret_cast<c
 
 static inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
-// Raises `kernel`'s dynamic shared-memory limit to `bytes` the first time a launch needs more than
-// the limit already set through `limit` (one per kernel, per process; the default limit is 48 KB
-// minus the kernel's static shared memory, so any size is set once).  Calls that need no more
-// touch nothing, so launches inside a CUDA-graph capture make no runtime calls beyond the launch.
+// Raises `kernel`'s dynamic shared-memory limit to `bytes` where the current device's is not known to be that large:
+// `limit` (one per kernel, starting at 0) holds the limit last set and the device that it was set on, as a
+// function's attributes belong to a device.  (The default limit is 48 KB minus the kernel's static shared memory, so
+// any size is set once.)  Calls that need no more set nothing, so launches inside a CUDA-graph capture make no
+// runtime calls beyond the launch and the question for the device.
 template <class Kernel>
 static inline cudaError_t ensure_dynamic_smem(Kernel kernel, size_t bytes, int& limit) {
-  if (int(bytes) <= limit) return cudaSuccess;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
-  if (e == cudaSuccess) limit = int(bytes);
+  constexpr int BYTES = (1 << 20) - 1;
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (limit >> 20 == dev && int(bytes) <= (limit & BYTES))) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+  if (e == cudaSuccess) limit = dev << 20 | int(bytes);
   return e;
 }
 
