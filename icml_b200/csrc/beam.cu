@@ -26,6 +26,8 @@
 
 #include <cooperative_groups.h>
 
+#include <atomic>
+
 namespace pgf {
 namespace beam {
 
@@ -386,7 +388,8 @@ static int select_as(Args a, int64_t Bsz, cudaStream_t s) {
 }
 
 // Few sequences (up to 4) take clusters of 16, more of them 8 (one sequence of 4 x 50257: 9 us against 12; 16 of
-// them fill the GPU either way).  Clusters of 16 are beyond the portable size: asked for once, and used if the device can place one.
+// them fill the GPU either way).  Clusters of 16 are beyond the portable size: asked for once on each device, and used
+// if that can place one, also when each CTA fills an SM.
 template <class T>
 static bool ask_wide() {
   for (auto* k : {select_kernel<T, 16, true>, select_kernel<T, 16, false>})
@@ -408,8 +411,19 @@ static bool ask_wide() {
 }
 template <class T>
 static bool wide_clusters() {
-  static const bool ok = ask_wide<T>() || (cudaGetLastError(), false);   // a refusal is an answer, not the launch's error
-  return ok;
+  constexpr int DEVICES = 64;                              // (further ones go without)
+  static std::atomic<signed char> answer[DEVICES];         // 0: not asked
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= DEVICES) {
+    cudaGetLastError();
+    return false;
+  }
+  if (answer[dev] == 0) {
+    const bool ok = ask_wide<T>();
+    if (!ok) cudaGetLastError();                           // a refusal is an answer, not the launch's error
+    answer[dev] = ok ? 1 : -1;
+  }
+  return answer[dev] > 0;
 }
 
 // 16 CTAs a sequence while all of them run at once (a GPC holds one such cluster).
