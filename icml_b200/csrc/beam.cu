@@ -510,9 +510,18 @@ extern "C" int pgf_beam_reorder(const void* const* src, void* const* dst, const 
     PGF_CHECK_ARG(row_bytes[i] >= 0, "beam_reorder: row of %lld bytes", (long long)row_bytes[i]);
     if (row_bytes[i] == 0) continue;
     PGF_CHECK_ARG(dst[i] && (src[i] || n_src == 0), "beam_reorder: null pointer");
-    const char *s0 = static_cast<const char*>(src[i]), *s1 = s0 + n_src * row_bytes[i];
+    // the tensors are copied side by side: no output may lie over any state, nor over another output
     const char *d0 = static_cast<const char*>(dst[i]), *d1 = d0 + n_rows * row_bytes[i];
-    PGF_CHECK_ARG(d1 <= s0 || s1 <= d0, "beam_reorder: tensor %d would overwrite rows that it reads", i);
+    const char *r0 = reinterpret_cast<const char*>(rows), *r1 = r0 + n_rows * int64_t(sizeof(int64_t));
+    PGF_CHECK_ARG(d1 <= r0 || r1 <= d0, "beam_reorder: tensor %d would overwrite the order", i);
+    for (int j = 0; j < count; ++j) {
+      if (row_bytes[j] <= 0) continue;
+      const char *s0 = static_cast<const char*>(src[j]), *s1 = s0 + n_src * row_bytes[j];
+      PGF_CHECK_ARG(d1 <= s0 || s1 <= d0, "beam_reorder: tensor %d would overwrite rows that tensor %d reads", i, j);
+      if (j >= i) continue;
+      const char *o0 = static_cast<const char*>(dst[j]), *o1 = o0 + n_rows * row_bytes[j];
+      PGF_CHECK_ARG(d1 <= o0 || o1 <= d0, "beam_reorder: tensor %d would overwrite the output of tensor %d", i, j);
+    }
   }
   for (int i = 0; i < count;) {
     beam::Table t;

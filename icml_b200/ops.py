@@ -1118,7 +1118,7 @@ def beam_select(logits, scores, finished=None, *, end_id: Optional[int] = None):
 
 def beam_reorder(states, rows, out=None):
     """[s[rows] for s in states], in one launch: states of any type, (n, ...) contiguous; rows of any
-    shape (flattened).  out: contiguous tensors to write (not the states themselves)."""
+    shape (flattened).  out: contiguous tensors to write, apart from all the states and from one another."""
     name = "beam_reorder"
     dev = rows.get_device()
     if dev < 0:

@@ -622,7 +622,8 @@ int pgf_decay_attn_step(const void* q, const pgf_strides* q_strides, const void*
  * as -inf.  Outputs (B, K), best first: scores, rows (flat row b K + k that goes on), tokens, and
  * finished (may be NULL): the row had finished or the token is end_id (-1: none).  K <= 32, K V < 2^31.
  * pgf_beam_reorder copies dst[i] = src[rows[i]] for `count` tensors of n_src rows of row_bytes each
- * (host arrays, read during the call); a row out of range gives zeros. */
+ * (host arrays, read during the call), side by side: no dst may overlap a src, another dst or rows.  A row
+ * out of range gives zeros. */
 int pgf_beam_select(const void* logits, const float* scores, const uint8_t* finished, float* out_scores,
                     int64_t* out_rows, int64_t* out_tokens, uint8_t* out_finished, int64_t Bsz, int64_t K, int64_t V,
                     int64_t end_id, int dtype, pgf_stream_t stream);
