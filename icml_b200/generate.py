@@ -28,8 +28,9 @@ def prefill(model: PGFLanguageModel, prompt: torch.Tensor, lengths: Optional[tor
     """(logits (B, V) behind each row's last token, [state of each layer]) of a prompt (B, L) whose row b has
     lengths[b] tokens (default all), 1 or more."""
     B, L = prompt.shape
-    if L < 1 or (lengths is not None and int(lengths.min()) < 1):
-        raise ValueError("prefill: every row needs a token")
+    least, most = (L, L) if lengths is None or B == 0 else torch.stack(lengths.aminmax()).tolist()
+    if L < 1 or least < 1 or most > L:
+        raise ValueError(f"prefill: lengths from {least} to {most}, every row has 1 to {L} tokens")
     x = ops.embedding_fwd(prompt, model.emb_weight, dtype=model.act_dtype)
     states = []
     for layer in model.backbone.layers:

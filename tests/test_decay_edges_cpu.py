@@ -18,3 +18,18 @@ def test_reorder_refuses_outputs_over_any_state_and_one_another(src, dst, n_rows
     arr = ctypes.c_void_p * 2
     rc = _lib.lib().pgf_beam_reorder(arr(*src), arr(*dst), (ctypes.c_int64 * 2)(64, 64), 2, 1 << 20, n_rows, n_src, None)
     assert rc != 0 and "overwrite" in _lib.last_error()
+
+
+# ----------------------------------------------------------------------------------------- prompts and models
+def _model(variant="decay"):
+    from icml_b200.lm import PGFLanguageModel
+    return PGFLanguageModel(31, 64, 16, 128, 2, 64, "cpu", variant=variant)
+
+
+@pytest.mark.parametrize("lengths", [[6, 3], [5, 2 ** 40], [0, 5], [5, -1]])
+def test_prefill_refuses_lengths_outside_the_prompt(lengths):
+    from icml_b200.generate import beam_search, prefill
+    ids = torch.zeros(2, 5, dtype=torch.int64)
+    for call in (lambda n: prefill(_model(), ids, n), lambda n: beam_search(_model(), ids, 2, 2, n)):
+        with pytest.raises(ValueError, match="1 to 5 tokens"):
+            call(torch.tensor(lengths))
