@@ -22,6 +22,7 @@ import torch
 import torch.distributed as dist
 
 from . import ops as cuda_ops
+from .pgf_mamba_std import MambaMixer
 
 
 @dataclass
@@ -68,7 +69,12 @@ def _wb(m):
 
 
 def _is_std(block) -> bool:
-    return hasattr(block, "mixer")
+    """Which of the two blocks that have a segment form; other blocks are refused."""
+    mixer = getattr(block, "mixer", None)
+    if mixer is not None and not isinstance(mixer, MambaMixer):
+        raise ValueError(f"sequence sharding: {type(block).__name__} has no segment form (PGFMambaBlock and "
+                         "PGFMambaStdBlock have)")
+    return mixer is not None
 
 
 def _prev_rows(sp: SeqGroup, rows: torch.Tensor) -> Optional[torch.Tensor]:
@@ -223,6 +229,8 @@ def lm_forward_backward(model, input_ids: torch.Tensor, targets: torch.Tensor, s
     B, L = input_ids.shape
     d = model.d_model
     T_total = total_tokens if total_tokens is not None else B * L * sp.world
+    for layer in model.backbone.layers:
+        _is_std(layer)
     x = ops.embedding_fwd(input_ids, model.emb_weight, dtype=model.act_dtype)
     stash: List[Tuple[torch.Tensor, Optional[torch.Tensor], Any]] = []
     for layer in model.backbone.layers:

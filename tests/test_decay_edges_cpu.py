@@ -33,3 +33,15 @@ def test_prefill_refuses_lengths_outside_the_prompt(lengths):
     for call in (lambda n: prefill(_model(), ids, n), lambda n: beam_search(_model(), ids, 2, 2, n)):
         with pytest.raises(ValueError, match="1 to 5 tokens"):
             call(torch.tensor(lengths))
+
+
+def test_sequence_sharding_refuses_a_decay_model():
+    """The variant has no segment form: named on the host, before any operator runs."""
+    from icml_b200 import seqpar
+    m, ids = _model(), torch.zeros(1, 8, dtype=torch.int64)
+    x = torch.zeros(1, 8, 64)
+    for call in (lambda: seqpar.lm_forward_backward(m, ids, ids, seqpar.SeqGroup()),
+                 lambda: seqpar.block_forward(m.backbone.layers[0], x, seqpar.SeqGroup()),
+                 lambda: seqpar.block_backward(m.backbone.layers[0], x, x, None, seqpar.SeqGroup())):
+        with pytest.raises(ValueError, match="PGFDecayBlock"):
+            call()
