@@ -22,21 +22,21 @@ from .pgf_rmsnorm import RMSNorm
 
 class _RotateFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, wq, wk, turns, kw):
-        ctx.save_for_backward(q, k, wq, wk, turns)
+    def forward(ctx, q, k, wq, wk, turns, positions, kw):
+        ctx.save_for_backward(q, k, wq, wk, turns, positions)
         ctx.kw = kw
-        return ops.qk_norm_rotate_fwd(q, k, wq, wk, turns, **kw)
+        return ops.qk_norm_rotate_fwd(q, k, wq, wk, turns, positions=positions, **kw)
 
     @staticmethod
     def backward(ctx, gq, gk):
-        q, k, wq, wk, turns = ctx.saved_tensors
-        r = ops.qk_norm_rotate_bwd(q, k, gq, gk, wq, wk, turns, **ctx.kw)
-        return r["grad_q"], r["grad_k"], r.get("grad_wq"), r.get("grad_wk"), None, None
+        q, k, wq, wk, turns, positions = ctx.saved_tensors
+        r = ops.qk_norm_rotate_bwd(q, k, gq, gk, wq, wk, turns, positions=positions, **ctx.kw)
+        return r["grad_q"], r["grad_k"], r.get("grad_wq"), r.get("grad_wk"), None, None, None
 
 
-def qk_norm_rotate(q, k, wq=None, wk=None, turns=None, **kw):
+def qk_norm_rotate(q, k, wq=None, wk=None, turns=None, *, positions=None, **kw):
     """ops.qk_norm_rotate_fwd with its gradient (of q, k, wq and wk)."""
-    return _RotateFn.apply(q, k, wq, wk, turns, kw)
+    return _RotateFn.apply(q, k, wq, wk, turns, positions, kw)
 
 
 class _DecayFn(torch.autograd.Function):

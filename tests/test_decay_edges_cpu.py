@@ -45,3 +45,59 @@ def test_sequence_sharding_refuses_a_decay_model():
                  lambda: seqpar.block_backward(m.backbone.layers[0], x, x, None, seqpar.SeqGroup())):
         with pytest.raises(ValueError, match="PGFDecayBlock"):
             call()
+
+
+# ------------------------------------------------------------------------------------------ autograd rules
+@pytest.fixture
+def plain_ops(monkeypatch):
+    """The layer's operators as host functions that differentiate what they are given (float64)."""
+    from icml_b200 import pgf_decay
+    from tests import decay_oracle as O
+    kw64 = dict(R=8, base=100.0, pairs="halves", eps=1e-6)
+
+    def rotate(q, k, wq, wk, turns, positions):
+        return tuple(O.norm_rotate(x, w, positions, *kw64.values()) for x, w in ((q, wq), (k, wk)))
+
+    def rotate_bwd(q, k, gq, gk, wq, wk, turns, positions):
+        with torch.enable_grad():
+            leaves = [t.detach().requires_grad_() for t in (q, k, wq, wk)]
+            g = torch.autograd.grad(rotate(*leaves, turns, positions), leaves, (gq, gk))
+        return dict(zip(("grad_q", "grad_k", "grad_wq", "grad_wk"), g))
+
+    def attend(q, k, v, ld, scale=None, state=None, lengths=None):
+        return O.decay_attn(q, k, v, ld, scale, state, lengths)
+
+    def attend_bwd(q, k, v, ld, g, scale=None, state=None, g_state=None, lengths=None, need_g_log_decay=False):
+        with torch.enable_grad():
+            leaves = [t.detach().requires_grad_() for t in (q, k, v, state, ld)]
+            out = attend(*leaves[:3], leaves[4], scale, leaves[3])
+            r = torch.autograd.grad(out, leaves, (g, torch.zeros_like(state) if g_state is None else g_state))
+        return dict(zip(("grad_q", "grad_k", "grad_v", "grad_state", "grad_log_decay"), r))
+
+    def gemm(a, b, a_trans=False, b_trans=False, out_dtype=None, addend=None):
+        return (a.t() if a_trans else a) @ (b if b_trans else b.t())
+
+    for name, f in (("qk_norm_rotate_fwd", rotate), ("qk_norm_rotate_bwd", rotate_bwd), ("decay_attn_fwd", attend),
+                    ("decay_attn_bwd", attend_bwd), ("gemm", gemm)):
+        monkeypatch.setattr(pgf_decay.ops, name, f)
+    return pgf_decay
+
+
+def _leaves(*shapes):
+    g = torch.Generator().manual_seed(1)
+    return [torch.randn(*s, generator=g, dtype=torch.float64, requires_grad=True) for s in shapes]
+
+
+def test_positions_changed_before_the_backward_are_noticed(plain_ops):
+    q, k, wq, wk = _leaves((1, 3, 2, 8), (1, 3, 1, 8), (8,), (8,))
+    positions = torch.arange(3)[None]
+    a, b = plain_ops.qk_norm_rotate(q, k, wq, wk, None, positions=positions)
+    want = torch.autograd.grad(a.sum() + b.sum(), [q, k, wq, wk])
+    assert torch.autograd.gradcheck(lambda *t: plain_ops.qk_norm_rotate(*t, None, positions=positions), [q, k, wq, wk])
+    a, b = plain_ops.qk_norm_rotate(q, k, wq, wk, None, positions=positions)
+    positions += 1                         # as a decoding loop moves on
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        (a.sum() + b.sum()).backward()
+    positions -= 1
+    a, b = plain_ops.qk_norm_rotate(q, k, wq, wk, None, positions=positions)
+    assert all(torch.equal(x, y) for x, y in zip(want, torch.autograd.grad(a.sum() + b.sum(), [q, k, wq, wk])))
