@@ -14,6 +14,7 @@ from typing import Any, Dict, Optional
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from . import ops
 from .pgf_ffn import FFNFunction
@@ -28,6 +29,7 @@ class _RotateFn(torch.autograd.Function):
         return ops.qk_norm_rotate_fwd(q, k, wq, wk, turns, positions=positions, **kw)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, gq, gk):
         q, k, wq, wk, turns, positions = ctx.saved_tensors
         r = ops.qk_norm_rotate_bwd(q, k, gq, gk, wq, wk, turns, positions=positions, **ctx.kw)
@@ -48,6 +50,7 @@ class _DecayFn(torch.autograd.Function):
         return ops.decay_attn_fwd(q, k, v, log_decay, scale=scale, state=state, lengths=lengths)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g, g_state):
         q, k, v, log_decay, state, lengths = ctx.saved_tensors
         if g is None:
@@ -70,6 +73,7 @@ class _LinearFn(torch.autograd.Function):
         return _linear(x, W)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g):
         x, W = ctx.saved_tensors
         gW, gx = _linear_bwd(x, g, W)

@@ -101,3 +101,22 @@ def test_positions_changed_before_the_backward_are_noticed(plain_ops):
     positions -= 1
     a, b = plain_ops.qk_norm_rotate(q, k, wq, wk, None, positions=positions)
     assert all(torch.equal(x, y) for x, y in zip(want, torch.autograd.grad(a.sum() + b.sum(), [q, k, wq, wk])))
+
+
+def test_second_derivatives_are_refused(plain_ops):
+    q, k, wq, wk, v, s, ld, x, W = _leaves((1, 3, 2, 8), (1, 3, 1, 8), (8,), (8,), (1, 3, 2, 4), (1, 2, 8, 4), (2,), (3, 8), (4, 8))
+    positions = torch.arange(3)[None]
+
+    def rotated():
+        return plain_ops.qk_norm_rotate(q, k, wq, wk, None, positions=positions)[0], q
+
+    def attended():
+        return plain_ops.decay_attention(q, k, v, ld, scale=0.5, state=s)[0], v
+
+    for f in (rotated, attended, lambda: (plain_ops._LinearFn.apply(x, W), x)):
+        y, leaf = f()
+        (first,) = torch.autograd.grad((y * y).sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            (first * leaf).sum().backward()
+        (plain,) = torch.autograd.grad((lambda y: (y * y).sum())(f()[0]), leaf)
+        assert torch.equal(first, plain)
