@@ -846,8 +846,8 @@ def rotary_turns(dim: int, base: float = 10000.0, device="cuda") -> torch.Tensor
     if dim < 0 or dim % 2:
         raise ValueError(f"rotary_turns: rotated width {dim} must be even")
     f = float(base) ** (-torch.arange(0, dim, 2, dtype=torch.float64) / max(dim, 1)) / 6.283185307179586
-    if bool((f >= 0.5).any()):
-        raise ValueError("rotary_turns: base must keep every frequency below half a turn per position")
+    if not bool((f < 0.5).all()):
+        raise ValueError("rotary_turns: base must give every frequency, below half a turn per position")
     return (f * 2.0 ** 64).to(torch.int64).to(device)
 
 

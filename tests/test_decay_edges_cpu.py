@@ -120,3 +120,10 @@ def test_second_derivatives_are_refused(plain_ops):
             (first * leaf).sum().backward()
         (plain,) = torch.autograd.grad((lambda y: (y * y).sum())(f()[0]), leaf)
         assert torch.equal(first, plain)
+
+
+@pytest.mark.parametrize("base", [-10000.0, float("nan"), 0.0, 0.01])
+def test_rotary_turns_refuse_bases_without_frequencies(base):
+    from icml_b200 import ops
+    with pytest.raises(ValueError):
+        ops.rotary_turns(8, base, "cpu")
