@@ -896,7 +896,7 @@ def _whole(name: str, what: str, t: torch.Tensor, shape, dev: int, dtype) -> tor
 def _lengths(name: str, t: torch.Tensor, B: int, L: int, dev: int) -> torch.Tensor:
     """A row's length each, as int32: below zero counts as none, beyond the sequence as all of it."""
     if t.dtype is not torch.int32 and t.element_size() >= 4 and not t.is_floating_point():
-        t = t.clamp(0, L)  # (the kernels clamp what 32 bits hold)
+        t = t.long().clamp(0, L)  # (the kernels clamp what 32 bits hold)
     return _whole(name, "lengths", t, (B,), dev, torch.int32)
 
 

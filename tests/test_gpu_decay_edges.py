@@ -154,3 +154,5 @@ def test_lengths_of_any_whole_type(dtype):
     want = call(torch.tensor([L, L, L, 0, 0, 77], dtype=torch.int32, device=DEV))
     assert all(torch.equal(a, b) for a, b in zip(call(far), want))
     assert all(torch.equal(a, b) for a, b in zip(call(far.clamp(-2 ** 15, 2 ** 15 - 1).short()), want))
+    high = torch.tensor([2 ** 31 + 9, 2 ** 32 - 1, L, 0, 0, 77], device=DEV).to(torch.uint32)
+    assert all(torch.equal(a, b) for a, b in zip(call(high), want))
