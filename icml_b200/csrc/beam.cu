@@ -19,7 +19,8 @@
 // with two readings); shorter ones are read twice, the second time from L1 and L2 (4 beams x 50257 in float32 over
 // 16 CTAs: 9.2 us, 10.2 through shared memory), and so are longer ones.  The loops stay short on purpose: a part unrolled into
 // registers ran slower (29 us at the first of these sizes), fetching instructions that run once.  The parts' best K keys meet the same way in one
-// CTA, which ranks them and writes the step's outputs.  A key is the order-preserving image of c above
+// CTA, which ranks them and writes the step's outputs.  What a CTA waits for is mostly the others, at its own and the
+// cluster's barriers; DRAM is at 8% at the first of these sizes.  A key is the order-preserving image of c above
 // the complement of the flat index, so one 64-bit comparison is the whole order.  A list that does not
 // fit (rows of equal logits) falls back to K passes of a plain maximum.
 #include "tc_common.cuh"

@@ -458,10 +458,12 @@ static int walk(const Job* job, int count, const TangentArgs& tan, const Link& l
 }
 
 // ---------------------------------------------------------------------------------------------
-// One token: S' = a S + k v^T, o = scale q S'.  Bound by reading and writing the state (8 Dk Dv bytes per
-// head).  A CTA owns a slice of the columns of one (row, head); a thread keeps four columns and walks the
-// rows, its loads ahead of its arithmetic; the row sums of o meet in shared memory in a fixed order.
-// 128 rows x 16 heads of 64 x 64: 16.5 us, 4.1 TB/s (22 with single columns instead of four); 1 row x 8 heads
+// One token: S' = a S + k v^T, o = scale q S'.  It reads and writes the state (8 Dk Dv bytes per head), but what it
+// waits for is the chain of a short CTA (vectors, barrier, state, barrier; 4 resident, 3.5 waves at the first size
+// below): DRAM and L2 are at 24 and 22%, issue slots at 44%.  A CTA owns a slice of the columns of one (row, head); a
+// thread keeps four columns and walks the rows, its loads ahead of its arithmetic; the row sums of o meet in shared
+// memory in a fixed order.
+// 128 rows x 16 heads of 64 x 64: 16.5 us for 67 MB (22 with single columns instead of four); 1 row x 8 heads
 // of 128 x 128: 3.2 us, the length of its chain of loads.
 // ---------------------------------------------------------------------------------------------
 struct StepArgs {

@@ -16,6 +16,10 @@
 //   grad v = F(k, q, g; X)            from the end, X = sum a^(..) q g^T + the final state's gradient
 //   grad k = F(v, g, q; X^T)          from the end
 // with g the output's gradient.  X' before the first token is the initial state's gradient.
+//
+// A chunk's pairs are formed by products whose masked weights are zeros, so a value that is infinite or NaN reaches
+// its column from the first token of its chunk on (at most 128 tokens, counted from the sequence's start), not from
+// its own token.  Rows past the length are replaced by zeros first: whatever lies there reaches nothing.
 #pragma once
 #include "chain.cuh"
 

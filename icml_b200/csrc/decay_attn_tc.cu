@@ -34,6 +34,8 @@
 // 32 SMs walk and 4.2 where all do, and the warps that weigh y are the ones that the others wait for.  Measured
 // and slower: the output stored straight from registers (157 against 129 us), half of y weighed by X (148 against
 // 137), y weighed by parts of 32 tokens out of place (139 against 128), the next A in front of D1 (144 against 129).
+// 640 threads leave 96 registers each: the walks with 128-wide z spill 48 to 144 bytes a thread, those with 64-wide z
+// none.
 // The float32 engine (decay_attn.cu) takes 3350 us for the first of these sizes: bf16 inputs of widths that are
 // multiples of 8 up to 128, in 16-byte aligned tensors, go here whatever their number.
 //

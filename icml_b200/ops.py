@@ -1008,7 +1008,8 @@ def decay_attn_fwd(q, k, v, log_decay, *, scale: Optional[float] = None, state=N
     S_t = exp(log_decay) S_{t-1} + k_t v_t^T, o_t = scale q_t S_t.  q (B, L, Hq, Dk), k (B, L, Hk, Dk),
     v (B, L, Hv, Dv), log_decay (H) float32; each head count divides H, out is (B, L, H, Dv).  scale
     defaults to Dk^-0.5.  state: float32 (B, H, Dk, Dv) that came before (None: zeros); lengths (B):
-    tokens past a row's length are not there."""
+    tokens past a row's length are not there.  Without want_state no state is kept, and bfloat16 calls carry
+    fewer bits of the keys inside (16 for 24): out differs in its last bits."""
     name = "decay_attn_fwd"
     dt, dev, B, L_, H, Hq, Hk, Hv, Dk, Dv, log_decay = _decay_args(name, q, k, v, log_decay, 4)
     if state is not None:

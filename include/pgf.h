@@ -587,8 +587,11 @@ int pgf_qk_norm_rotate_bwd(const void* q, const pgf_strides* q_strides, const vo
  * q (B, L, Hq, Dk), k (B, L, Hk, Dk), v (B, L, Hv, Dv), each head count a divisor of H (head h reads
  * head h / (H / Hq) and so on); out (B, L, H, Dv).  state / state_out: float32 (B, H, Dk, Dv) before
  * the first and after the last token, each may be NULL (zeros / not wanted).  lengths (B): tokens past
- * a row's length are not there (whatever they hold), their outputs and gradients are zeros.
- * log_decay (H) float32, normally <= 0.  1 <= Dk, Dv <= 256.
+ * a row's length are not there (whatever they hold), their outputs and gradients are zeros.  An infinite or
+ * NaN value within the length shows in its column from the start of its 128 tokens on.
+ * log_decay (H) float32, normally <= 0 (a NaN makes its head's results NaN).  1 <= Dk, Dv <= 256.
+ * In bfloat16 the keys enter the state by 24 bits where a state leaves the call and by 16 where none does, so
+ * out's last bits depend on state_out.
  * The backward recomputes every state; g (B, L, H, Dv) is the output's gradient, g_state the final
  * state's (may be NULL); grad_log_decay (H) and grad_state may be NULL; `accumulate` concerns
  * grad_log_decay.

@@ -156,3 +156,22 @@ def test_lengths_of_any_whole_type(dtype):
     assert all(torch.equal(a, b) for a, b in zip(call(far.clamp(-2 ** 15, 2 ** 15 - 1).short()), want))
     high = torch.tensor([2 ** 31 + 9, 2 ** 32 - 1, L, 0, 0, 77], device=DEV).to(torch.uint32)
     assert all(torch.equal(a, b) for a, b in zip(call(high), want))
+
+
+@pytest.mark.parametrize("dtype", BOTH)
+@pytest.mark.parametrize("L", [700, 4000])
+def test_a_value_that_is_no_number_stays_in_its_column(L, dtype):
+    """A NaN value makes its column NaN from its token on, in its row and head; within its 128 tokens, whose products
+    are formed together, earlier outputs may be NaN too, and nothing else changes."""
+    from icml_b200 import ops
+    g = _gen(L)
+    q, k, v = (_n(g, 2, L, 2, 64).to(dtype) for _ in range(3))
+    ld = torch.tensor([-0.1, -0.01], device=DEV)
+    base = ops.decay_attn_fwd(q, k, v, ld)
+    v = v.clone()
+    v[0, 300, 1, 5] = math.nan
+    out, end = ops.decay_attn_fwd(q, k, v, ld)
+    assert bool(out[0, 300:, 1, 5].isnan().all()) and bool(end[0, 1, :, 5].isnan().all())
+    out[0, 256:, 1, 5] = base[0][0, 256:, 1, 5]
+    end[0, 1, :, 5] = base[1][0, 1, :, 5]
+    assert torch.equal(out, base[0]) and torch.equal(end, base[1])
