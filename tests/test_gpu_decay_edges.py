@@ -10,14 +10,9 @@ import pytest
 import torch
 
 from tests import decay_oracle as O
-from tests.test_gpu_decay import BOTH, DEV, TOL, _beam_check, _close, _gen, _n
+from tests.test_gpu_decay import BOTH, DEV, _beam_check, _close, _gen, _n
 
 pytestmark = pytest.mark.gpu
-
-
-def _same(a, b):
-    """Equal values, NaN equal to NaN."""
-    return torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(nan=0.0), b.nan_to_num(nan=0.0))
 
 
 # --------------------------------------------------------------------------------------- states that leave
